@@ -1,0 +1,445 @@
+// khq_paged.cu -- the plan of a step over a raw paged K/V cache, and the pre-step that fills the cache.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "khq_b200.h"
+#include "khq_common.cuh"
+#include "khq_launch.cuh"
+#include "khq_paged.cuh"
+
+namespace khq_paged {
+
+// ---- the plan of a step --------------------------------------------------------------------------
+// One cluster.  Every CTA sums up the lengths of all requests for itself (8 bytes a request) and keeps three running sums in shared
+// memory: tokens, pages taken, pages given back.  From those any token and any moved page is found by bisection, so the CTAs need nothing from each
+// other: the pages of ended requests are read where they stand in their table rows, on top of the free ones.  Only the new
+// number of free pages waits (free_count_out may be free_count).
+constexpr int PLAN_THREADS = 1024, PLAN_CTAS = 8, PLAN_MAX_REQUESTS = 16384, PLAN_MAX_TOKENS = 1 << 20;
+
+struct PlanArgs {
+    const int *ctx_lens, *new_lens;
+    int* table;
+    long long table_stride;
+    int* free_list;
+    const int* free_count;
+    int *free_count_out, *cu_new, *kv_lens, *positions;
+    long long* slots;
+    int *info, *schedule;
+    int requests, max_pages, n_pages, page_shift, max_tokens, max_new, tile_tokens, tile_keys;
+    long long item_cap;
+};
+
+// Inclusive sums of two ints over the block.  `part`: 2 x 32 ints.
+__device__ __forceinline__ void block_scan2(int& a, int& b, int* part, int& total_a, int& total_b) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xFFFFFFFFu, a, o), y = __shfl_up_sync(0xFFFFFFFFu, b, o);
+        if (lane >= o) {
+            a += x;
+            b += y;
+        }
+    }
+    __syncthreads();  // the last use of `part`
+    if (lane == 31) {
+        part[warp] = a;
+        part[32 + warp] = b;
+    }
+    __syncthreads();
+    int wa = part[lane], wb = part[32 + lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xFFFFFFFFu, wa, o), y = __shfl_up_sync(0xFFFFFFFFu, wb, o);
+        if (lane >= o) {
+            wa += x;
+            wb += y;
+        }
+    }
+    total_a = __shfl_sync(0xFFFFFFFFu, wa, 31);
+    total_b = __shfl_sync(0xFFFFFFFFu, wb, 31);
+    const int before_a = __shfl_sync(0xFFFFFFFFu, wa, (warp + 31) & 31), before_b = __shfl_sync(0xFFFFFFFFu, wb, (warp + 31) & 31);
+    if (warp > 0) {
+        a += before_a;
+        b += before_b;
+    }
+}
+
+// The last i in [0, n) with cum[i] <= x; cum[0] = 0 <= x < cum[n].
+__device__ __forceinline__ int find(const int* cum, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cum[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS) khq_paged_plan_kernel(const PlanArgs a) {
+    extern __shared__ int sums[];  // tokens, pages taken, pages given back: requests + 1 running sums each
+    __shared__ int part[64];
+    int *const cu = sums, *const taken = cu + a.requests + 1, *const back = taken + a.requests + 1;
+    const int tid = threadIdx.x, rank = blockIdx.x, B = a.requests, page = 1 << a.page_shift;
+    khq::pdl_wait();
+    khq::pdl_trigger();
+    const bool pool = a.free_list != nullptr;
+    const int count = pool ? min(max(*a.free_count, 0), a.n_pages) : 0;
+    // table pages that `tokens` tokens lie in
+    const auto pages = [&](int tokens) { return (int)min(((long long)tokens + page - 1) >> a.page_shift, (long long)a.max_pages); };
+    const auto ctx_of = [&](int b) { return (int)min((long long)max(a.ctx_lens[b], 0), (long long)a.max_pages << a.page_shift); };
+    int sum_tok = 0, sum_taken = 0, sum_back = 0, dropped = 0;
+    for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
+        const int b = b0 + tid;
+        int ctx = 0, n = 0, asked = 0;
+        if (b < B) {
+            ctx = ctx_of(b);
+            asked = a.new_lens[b];
+            n = min(max(asked, 0), a.max_new);
+        }
+        int incl = min(n, a.max_tokens), unused = 0, total, u;  // sums of up to 2^10 terms of up to 2^20
+        block_scan2(incl, unused, part, total, u);
+        const int first = min(sum_tok + incl - min(n, a.max_tokens), a.max_tokens), end = min(sum_tok + incl, a.max_tokens);
+        sum_tok = min(sum_tok + total, a.max_tokens);
+        const int kept = end - first, held = pages(ctx);
+        int t = 0, r = 0;
+        if (b < B && pool) {
+            if (asked < 0) r = held;
+            else t = pages(ctx + kept) - held;
+        }
+        const int mine_t = t, mine_r = r;
+        int total_t, total_r;
+        block_scan2(t, r, part, total_t, total_r);
+        if (b < B) {
+            cu[b] = first;
+            taken[b] = sum_taken + t - mine_t;
+            back[b] = sum_back + r - mine_r;
+            if (rank == 0) {
+                a.cu_new[b] = first;
+                a.kv_lens[b] = asked < 0 ? 0 : ctx + kept;
+                dropped += min(max(asked, 0) - kept, 1 << 20);
+            }
+        }
+        sum_taken += total_t;
+        sum_back += total_r;
+    }
+    if (tid == 0) {
+        cu[B] = sum_tok;
+        taken[B] = sum_taken;
+        back[B] = sum_back;
+    }
+    __syncthreads();
+    // the free pages with the ones given back on top; pages are taken from the top
+    const int stack = count + sum_back;
+    const auto given_back = [&](int r) {
+        const int b = find(back, B, r);
+        return a.table[b * a.table_stride + (r - back[b])];
+    };
+    const auto nth_taken = [&](int j) {
+        const int i = stack - 1 - j;
+        return i < 0 ? -1 : i < count ? a.free_list[i] : given_back(i - count);
+    };
+    if (rank == 0) {
+        // ---- sums, and the items of the attention --------------------------------------------------
+        int drop = dropped, unused = 0, total_drop, u;
+        block_scan2(drop, unused, part, total_drop, u);
+        if (tid == 0) {
+            a.cu_new[B] = sum_tok;
+            a.info[0] = sum_tok;
+            a.info[1] = min(sum_taken, stack);
+            a.info[2] = sum_back;
+            a.info[3] = max(sum_taken - stack, 0);
+            a.info[4] = total_drop;
+        }
+        // the first sums are not needed any more once all threads are here: items per request
+        int items = 0;
+        for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
+            const int b = b0 + tid;
+            int n = 0, z = 0, total;
+            if (b < B) n = (cu[b + 1] - cu[b] + a.tile_tokens - 1) / a.tile_tokens;
+            const int mine = n;
+            block_scan2(n, z, part, total, u);
+            if (b < B) taken[b] = items + n - mine;
+            items += total;
+        }
+        if (tid == 0) taken[B] = items;
+        __syncthreads();
+        Item* const list = reinterpret_cast<Item*>(a.schedule + SCHED_HEADER);
+        int* const cum = a.schedule + SCHED_HEADER + 4 * a.item_cap;
+        int blocks = 0;
+        for (int i0 = 0; i0 < items; i0 += PLAN_THREADS) {
+            const int i = i0 + tid;
+            Item it = {0, 0, 0, 0};
+            if (i < items) {
+                it.b = find(taken, B, i);
+                it.q0 = (i - taken[it.b]) * a.tile_tokens;
+                it.ntok = min(a.tile_tokens, cu[it.b + 1] - cu[it.b] - it.q0);
+                it.n_blocks = (ctx_of(it.b) + it.q0 + it.ntok + a.tile_keys - 1) / a.tile_keys;
+            }
+            int n = it.n_blocks, z = 0, total;
+            block_scan2(n, z, part, total, u);
+            if (i < items) {
+                list[i] = it;
+                cum[i] = blocks + n - it.n_blocks;
+            }
+            blocks += total;
+        }
+        if (tid == 0) {
+            cum[items] = blocks;
+            a.schedule[0] = items;
+            a.schedule[1] = blocks;
+        }
+    } else {
+        // ---- table entries, the free list, positions and slots --------------------------------------
+        const int at = (rank - 1) * PLAN_THREADS + tid, step = (PLAN_CTAS - 1) * PLAN_THREADS;
+        for (int j = at; j < sum_taken; j += step) {
+            const int b = find(taken, B, j);
+            a.table[b * a.table_stride + pages(ctx_of(b)) + (j - taken[b])] = nth_taken(j);
+        }
+        for (int r = at; r < sum_back; r += step)
+            if (count + r < a.n_pages) a.free_list[count + r] = given_back(r);
+        for (int t = at; t < a.max_tokens; t += step) {
+            int pos = -1;
+            long long slot = -1;
+            if (t < sum_tok) {
+                const int b = find(cu, B, t), ctx = ctx_of(b);
+                pos = ctx + (t - cu[b]);
+                const int col = pos >> a.page_shift, held = pages(ctx);
+                if (col < a.max_pages) {
+                    const int p = pool && col >= held ? nth_taken(taken[b] + col - held) : a.table[b * a.table_stride + col];
+                    if (p >= 0) slot = ((long long)p << a.page_shift) + (pos & (page - 1));
+                }
+            }
+            a.positions[t] = pos;
+            a.slots[t] = slot;
+        }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0 && tid == 0 && pool) {
+        const int left = max(stack - sum_taken, 0);
+        a.info[5] = left;
+        *a.free_count_out = left;
+    }
+}
+
+// ---- the pre-step ------------------------------------------------------------------------------------
+// Per head: x / sqrt(mean(x^2) + eps) * w, then the rotation of the pairs (i, i + r/2), i < r/2, by pos * theta^(-2i/r).  In fp32, one
+// rounding to 16 bits where a value is stored (the rotated K is not made from the rounded un-rotated one).  The angle is
+// formed in fp64 and reduced there: at position 2^18 an fp32 product would be off by 2^-7.
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+    const __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return make_uint4(pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]), pack2<BF16>(x[4], x[5]), pack2<BF16>(x[6], x[7]));
+}
+
+constexpr int PRE_WARPS = 8, MAX_PAIRS = 128;
+struct PrestepArgs {
+    khq_paged_prestep_args a;
+    double freq[MAX_PAIRS];  // theta^(-2i/r) / 2 pi: turns per position
+    int page_shift;
+};
+
+// A CTA takes a token: its cosines and sines once, then a warp per head, 8 values (16 bytes) a lane; d == 128: a head per half warp.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(PRE_WARPS * 32) khq_paged_prestep_kernel(const __grid_constant__ PrestepArgs p) {
+    constexpr int LANES = D / 8;
+    __shared__ float2 turn[MAX_PAIRS];
+    const khq_paged_prestep_args& a = p.a;
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, heads = PRE_WARPS * 32 / LANES;
+    const int t = blockIdx.x, n_pairs = a.rotary_dim / 2, half_lanes = a.rotary_dim / 16;
+    khq::pdl_wait();
+    khq::pdl_trigger();
+    const int pos = static_cast<const int*>(a.positions)[t];
+    if (pos < 0) return;  // behind the last token
+    long long slot = static_cast<const long long*>(a.slots)[t];
+    if (slot >= (long long)a.n_pages << p.page_shift) slot = -1;
+    for (int i = threadIdx.x; i < n_pairs; i += PRE_WARPS * 32) {
+        double turns = (double)pos * p.freq[i];
+        turns -= rint(turns);
+        float s, c;
+        sincospif((float)(2.0 * turns), &s, &c);
+        turn[i] = make_float2(c, s);
+    }
+    __syncthreads();
+    const long long pg = slot >> p.page_shift, at = slot & (a.page_size - 1);
+    for (int h0 = 0; h0 < a.H_q + a.H_kv; h0 += heads) {  // whole warps stay together
+        const int h = min(h0 + sub, a.H_q + a.H_kv - 1);
+        const bool is_q = h < a.H_q, mine = h == h0 + sub;
+        const int hk = h - a.H_q;
+        const uint16_t* src = is_q ? static_cast<const uint16_t*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1]
+                                   : static_cast<const uint16_t*>(a.k) + t * a.k_stride[0] + hk * a.k_stride[1];
+        const uint4 raw = *reinterpret_cast<const uint4*>(src + lane * 8);
+        uint4 vv = make_uint4(0, 0, 0, 0);
+        if (!is_q && slot >= 0) vv = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.v) + t * a.v_stride[0] + hk * a.v_stride[1] + lane * 8);
+        const float* w = static_cast<const float*>(is_q ? a.q_norm_w : a.k_norm_w);
+        float x[8];
+        const uint32_t rw[4] = {raw.x, raw.y, raw.z, raw.w};
+        float sq = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack2<BF16>(rw[e]);
+            x[2 * e] = f.x;
+            x[2 * e + 1] = f.y;
+            sq += f.x * f.x + f.y * f.y;
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xFFFFFFFFu, sq, o, LANES);
+        const float inv = 1.0f / sqrtf(sq / (float)D + a.rms_eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= inv;
+        if (w) {
+            const float4 w0 = reinterpret_cast<const float4*>(w + lane * 8)[0], w1 = reinterpret_cast<const float4*>(w + lane * 8)[1];
+            x[0] *= w0.x; x[1] *= w0.y; x[2] *= w0.z; x[3] *= w0.w;
+            x[4] *= w1.x; x[5] *= w1.y; x[6] *= w1.z; x[7] *= w1.w;
+        }
+        const auto cache_row = [&](void* base, const int64_t (&st)[3]) {
+            return reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + pg * st[0] + at * st[1] + hk * st[2] + lane * 8);
+        };
+        if (mine && !is_q && slot >= 0 && a.u_cache) *cache_row(a.u_cache, a.u_cache_stride) = pack8<BF16>(x);
+        // the rotary pair of value e of lane l is value e of lane l +- half_lanes
+        const bool low = lane < half_lanes, turned = lane < 2 * half_lanes;
+        const int partner = low ? lane + half_lanes : turned ? lane - half_lanes : lane;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float y = __shfl_sync(0xFFFFFFFFu, x[e], partner, LANES);
+            if (turned) {
+                const float2 cs = turn[(low ? lane : partner) * 8 + e];
+                x[e] = low ? x[e] * cs.x - y * cs.y : y * cs.y + x[e] * cs.x;
+            }
+        }
+        const uint4 res = pack8<BF16>(x);
+        if (!mine) continue;
+        if (is_q) {
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + t * a.q_out_stride[0] + h * a.q_out_stride[1] + lane * 8) = res;
+        } else if (slot >= 0) {
+            *cache_row(a.k_cache, a.k_cache_stride) = res;
+            *cache_row(a.v_cache, a.v_cache_stride) = vv;
+        }
+    }
+}
+
+int log2_page(int page_size) {
+    return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : page_size == 128 ? 7 : -1;
+}
+
+int launch_prestep(const khq_paged_prestep_args* args, bool bf16, cudaStream_t stream) {
+    if (!args) return -100;
+    const khq_paged_prestep_args& a = *args;
+    if (a.tokens <= 0 || a.H_q <= 0 || a.H_kv <= 0 || a.n_pages <= 0 || !a.q || !a.k || !a.v || !a.q_out || !a.k_cache || !a.v_cache || !a.slots || !a.positions)
+        return -100;
+    if (!(a.rope_theta > 0.0f) || !(a.rms_eps >= 0.0f)) return -100;
+    if ((a.d != 128 && a.d != 256) || a.rotary_dim < 0 || a.rotary_dim > a.d || a.rotary_dim % 16 != 0 || log2_page(a.page_size) < 0) return -103;
+    const void* ptrs[] = {a.q, a.k, a.v, a.q_out, a.k_cache, a.v_cache, a.u_cache, a.q_norm_w, a.k_norm_w};
+    for (const void* q : ptrs)
+        if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return -104;
+    if ((reinterpret_cast<uintptr_t>(a.slots) & 7) != 0 || (reinterpret_cast<uintptr_t>(a.positions) & 3) != 0) return -104;
+    for (int i = 0; i < 2; ++i)
+        if (((a.q_stride[i] | a.k_stride[i] | a.v_stride[i] | a.q_out_stride[i]) & 7) != 0) return -104;
+    for (int i = 0; i < 3; ++i)
+        if (((a.k_cache_stride[i] | a.v_cache_stride[i] | (a.u_cache ? a.u_cache_stride[i] : 0)) & 7) != 0) return -104;
+    PrestepArgs p;
+    p.a = a;
+    p.page_shift = log2_page(a.page_size);
+    for (int i = 0; i < MAX_PAIRS; ++i)
+        p.freq[i] = i < a.rotary_dim / 2 ? pow((double)a.rope_theta, -2.0 * i / a.rotary_dim) / 6.283185307179586476925 : 0.0;
+    cudaError_t err;
+    const unsigned grid = (unsigned)a.tokens, threads = PRE_WARPS * 32;
+    if (a.d == 256)
+        err = bf16 ? khq::launch_pdl(khq_paged_prestep_kernel<256, true>, grid, 0, 0, stream, threads, p)
+                   : khq::launch_pdl(khq_paged_prestep_kernel<256, false>, grid, 0, 0, stream, threads, p);
+    else
+        err = bf16 ? khq::launch_pdl(khq_paged_prestep_kernel<128, true>, grid, 0, 0, stream, threads, p)
+                   : khq::launch_pdl(khq_paged_prestep_kernel<128, false>, grid, 0, 0, stream, threads, p);
+    return static_cast<int>(err);
+}
+
+}  // namespace khq_paged
+
+extern "C" size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, int H_q, int H_kv) {
+    using namespace khq_paged;
+    if (requests <= 0 || max_tokens <= 0 || max_new <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || H_q / H_kv > MAX_REP) return 0;
+    return (size_t)schedule_ints(max_items(requests, max_tokens, tile_of(H_q, H_kv, max_new).tokens)) * 4;
+}
+
+extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream_t stream) {
+    using namespace khq_paged;
+    if (!args) return -100;
+    const khq_paged_plan_args& p = *args;
+    if (p.requests <= 0 || p.max_tokens <= 0 || p.max_new <= 0 || p.max_pages <= 0 || p.H_q <= 0 || p.H_kv <= 0 || !p.ctx_lens || !p.new_lens || !p.block_table ||
+        !p.cu_new || !p.kv_lens || !p.positions || !p.slots || !p.info || !p.schedule)
+        return -100;
+    if (p.free_list ? (p.n_pages <= 0 || !p.free_count || !p.free_count_out) : (p.free_count || p.free_count_out)) return -100;
+    const int shift = log2_page(p.page_size);
+    if (shift < 0 || p.H_q % p.H_kv != 0 || p.H_q / p.H_kv > MAX_REP || p.requests > PLAN_MAX_REQUESTS || p.max_tokens > PLAN_MAX_TOKENS ||
+        (long long)p.requests * p.max_pages > 0x7FFFFFFFLL || p.table_stride < p.max_pages || (long long)p.max_pages << shift > (1LL << 30))
+        return -103;
+    const void* ptrs[] = {p.ctx_lens, p.new_lens, p.block_table, p.free_list, p.free_count, p.free_count_out, p.cu_new, p.kv_lens, p.positions, p.info};
+    for (const void* q : ptrs)
+        if ((reinterpret_cast<uintptr_t>(q) & 3) != 0) return -104;
+    if ((reinterpret_cast<uintptr_t>(p.slots) & 7) != 0 || (reinterpret_cast<uintptr_t>(p.schedule) & 15) != 0) return -104;
+    const Tile tile = tile_of(p.H_q, p.H_kv, p.max_new);
+    const long long items = max_items(p.requests, p.max_tokens, tile.tokens);
+    if (p.schedule_bytes < (size_t)schedule_ints(items) * 4) return -105;
+    // the key blocks of all items are counted in 32 bits
+    if (items * ((((long long)p.max_pages << shift) + p.max_tokens) / tile.keys + 1) > 0x7FFFFFFFLL) return -103;
+    PlanArgs a;
+    a.ctx_lens = static_cast<const int*>(p.ctx_lens);
+    a.new_lens = static_cast<const int*>(p.new_lens);
+    a.table = static_cast<int*>(p.block_table);
+    a.table_stride = p.table_stride;
+    a.free_list = static_cast<int*>(p.free_list);
+    a.free_count = static_cast<const int*>(p.free_count);
+    a.free_count_out = static_cast<int*>(p.free_count_out);
+    a.cu_new = static_cast<int*>(p.cu_new);
+    a.kv_lens = static_cast<int*>(p.kv_lens);
+    a.positions = static_cast<int*>(p.positions);
+    a.slots = static_cast<long long*>(p.slots);
+    a.info = static_cast<int*>(p.info);
+    a.schedule = static_cast<int*>(p.schedule);
+    a.requests = p.requests;
+    a.max_pages = p.max_pages;
+    a.n_pages = p.n_pages;
+    a.page_shift = shift;
+    a.max_tokens = p.max_tokens;
+    a.max_new = p.max_new;
+    a.tile_tokens = tile.tokens;
+    a.tile_keys = tile.keys;
+    a.item_cap = items;
+    const size_t smem = (size_t)3 * (p.requests + 1) * 4;
+    static bool attr_done[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    if (dev < 0 || dev >= 64) return -100;
+    if (!attr_done[dev]) {
+        err = cudaFuncSetAttribute((const void*)khq_paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (PLAN_MAX_REQUESTS + 1) * 4);
+        if (err != cudaSuccess) return static_cast<int>(err);
+        attr_done[dev] = true;
+    }
+    err = khq::launch_pdl(khq_paged_plan_kernel, (unsigned)PLAN_CTAS, 0, smem, stream, (unsigned)PLAN_THREADS, a);
+    return static_cast<int>(err);
+}
+
+extern "C" int launch_khq_paged_prestep_fp16(const khq_paged_prestep_args* args, khq_stream_t stream) {
+    return khq_paged::launch_prestep(args, false, stream);
+}
+
+extern "C" int launch_khq_paged_prestep_bf16(const khq_paged_prestep_args* args, khq_stream_t stream) {
+    return khq_paged::launch_prestep(args, true, stream);
+}

@@ -1,0 +1,305 @@
+// khq_paged_attn.cu -- attention of a step's new tokens over a raw paged K/V cache: the kernels' common part, the joining of shared
+// segments and the host side.  The kernels: khq_paged_decode.cuh (few rows a request).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "khq_b200.h"
+#include "khq_common.cuh"
+#include "khq_launch.cuh"
+#include "khq_paged.cuh"
+#include "khq_tc5.cuh"
+
+namespace khq_paged {
+
+using khq::smem_u32;
+using namespace khq_tc5;
+
+__device__ int g_paged_status = 0;
+
+struct Params {
+    const uint16_t *q, *gate;
+    uint16_t* out;
+    float* lse;
+    long long q_ts, q_hs, g_ts, g_hs, o_ts, o_hs, table_stride;
+    const int *table, *cu_new, *kv_lens, *schedule;
+    const Item* items;
+    const int* cum;
+    float* records;
+    int4* meta;  // by CTA: CTAs that share the segment which begins in it and goes on (0: none), item, kv head
+    int tokens, max_pages, n_pages, page_shift, page_mask, H_q, H_kv, n_rep;
+    float scale_log2e;
+};
+
+// An item of one kv head, and how far its key blocks have been walked.
+struct Segment {
+    int item, h, b, n_blocks, blk, ntok, kv, row0, pos0;  // row0: its first row in the ragged tensors, pos0: that row's position
+};
+__device__ __forceinline__ void load_segment(const Params& p, Segment& s) {
+    const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + s.item);
+    s.b = it.x;
+    s.ntok = it.z;
+    s.n_blocks = it.w;
+    const int first = __ldg(p.cu_new + it.x);
+    s.kv = __ldg(p.kv_lens + it.x);
+    s.row0 = first + it.y;
+    s.pos0 = s.kv - (__ldg(p.cu_new + it.x + 1) - first) + it.y;
+}
+// Block w of the row of all blocks.  A warp bisects by 32.
+__device__ __forceinline__ void find_segment(const Params& p, int n_items, long long per_head, long long w, Segment& s) {
+    const int lane = threadIdx.x & 31;
+    s.h = (int)(w / per_head);
+    const int r = (int)(w % per_head);
+    int lo = 0, n = n_items;  // the last item of [lo, lo + n) with cum <= r
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lo + lane * step;
+        const unsigned below = __ballot_sync(0xFFFFFFFFu, lane * step < n && __ldg(p.cum + (lane * step < n ? at : lo)) <= r);
+        const int last = 31 - __clz((int)(below | 1u));
+        lo += last * step;
+        n = min(step, n - last * step);
+    }
+    s.item = lo;
+    load_segment(p, s);
+    s.blk = r - __ldg(p.cum + lo);
+}
+// Every item has a key block at least (its own tokens).
+__device__ __forceinline__ void next_segment(const Params& p, int n_items, Segment& s) {
+    if (++s.item == n_items) {
+        s.item = 0;
+        ++s.h;
+    }
+    s.blk = 0;
+    load_segment(p, s);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store_out(const Params& p, int row, int head, int c, float4 acc, float inv) {
+    acc.x *= inv;
+    acc.y *= inv;
+    acc.z *= inv;
+    acc.w *= inv;
+    if (p.gate) {
+        const uint2 g = __ldg(reinterpret_cast<const uint2*>(p.gate + row * p.g_ts + head * p.g_hs + c));
+        const float2 g0 = unpack2<BF16>(g.x), g1 = unpack2<BF16>(g.y);
+        acc.x *= sigmoid(g0.x);
+        acc.y *= sigmoid(g0.y);
+        acc.z *= sigmoid(g1.x);
+        acc.w *= sigmoid(g1.y);
+    }
+    *reinterpret_cast<uint2*>(p.out + row * p.o_ts + head * p.o_hs + c) = make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
+}
+
+// Joins the records of the segment that begins in CTA blockIdx.x of the attention and goes on in the next ones; rows blockIdx.y, + gridDim.y, ..
+// A CTA's record 1 is of the segment that begins in it, record 0 of one that it took over.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128) khq_paged_merge_kernel(const Params p, int rows, int record_floats, int ctas) {
+    khq::pdl_wait();
+    khq::pdl_trigger();
+    const int4 meta = p.meta[blockIdx.x];
+    if (meta.x == 0) return;
+    const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + meta.y);
+    const int R = it.z * p.n_rep, row0 = __ldg(p.cu_new + it.x) + it.y;
+    constexpr int PER_ROW = D / 4;  // threads a row
+    const int c = (threadIdx.x % PER_ROW) * 4;
+    const long long total = (long long)p.schedule[1] * p.H_kv;
+    const auto empty = [&](int cta) { return cta * total / ctas == (cta + 1) * total / ctas; };
+    for (int r = blockIdx.y * (128 / PER_ROW) + threadIdx.x / PER_ROW; r < R; r += gridDim.y * (128 / PER_ROW)) {
+        float M = -INFINITY;
+        for (int i = 0; i < meta.x; ++i) {
+            const int cta = blockIdx.x + i;
+            if (empty(cta)) continue;
+            M = fmaxf(M, p.records[(2LL * cta + (i == 0)) * record_floats + rows * D + 2 * r]);
+        }
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float L = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < meta.x; ++i) {
+            const int cta = blockIdx.x + i;
+            if (empty(cta)) continue;
+            const float* rec = p.records + (2LL * cta + (i == 0)) * record_floats;
+            const float2 ml = *reinterpret_cast<const float2*>(rec + rows * D + 2 * r);
+            const float4 a = *reinterpret_cast<const float4*>(rec + r * D + c);
+            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+            L += ml.y * f;
+            acc.x += a.x * f;
+            acc.y += a.y * f;
+            acc.z += a.z * f;
+            acc.w += a.w * f;
+        }
+        const int row = row0 + r / p.n_rep, head = meta.z * p.n_rep + r % p.n_rep;
+        if (row >= p.tokens) continue;
+        store_out<BF16>(p, row, head, c, acc, L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L);
+        if (p.lse && c == 0) p.lse[(long long)row * p.H_q + head] = (M + log2f(L)) * 0.6931471805599453f;
+    }
+}
+
+}  // namespace khq_paged
+
+#include "khq_paged_decode.cuh"
+
+// ---- host side -----------------------------------------------------------------------------------
+namespace {
+
+using namespace khq_paged;
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static bool tried = false;
+    if (!tried) {
+        void* q = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(q);
+        tried = true;
+    }
+    return fn;
+}
+
+// A cache (n_pages, page_size, heads, d) as {64 values, token of a page, 64-column group, head, page}; a box is `box_tokens` tokens
+// x `box_groups` groups.
+int cache_map(CUtensorMap* map, const void* base, const int64_t (&stride)[3], int page_size, int heads, int d, int n_pages, int box_tokens, int box_groups,
+              bool bf16) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return -107;
+    const cuuint64_t dims[5] = {64, (cuuint64_t)page_size, (cuuint64_t)(d / 64), (cuuint64_t)heads, (cuuint64_t)n_pages};
+    // a dimension of one has any stride
+    const auto bytes = [](int64_t s, int n) { return n == 1 ? (cuuint64_t)16 : (cuuint64_t)s * 2; };
+    const cuuint64_t strides[4] = {(cuuint64_t)stride[1] * 2, 128, bytes(stride[2], heads), bytes(stride[0], n_pages)};
+    const cuuint32_t box[5] = {64, (cuuint32_t)box_tokens, (cuuint32_t)box_groups, 1, 1};
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : -108;
+}
+
+// Bytes of the workspace: two records per CTA and one line of `meta`.
+struct Work {
+    int ctas, record_floats;
+    size_t bytes;
+};
+Work work_of(const Tile& tile, int d) {
+    Work w;
+    (void)tile;
+    w.ctas = khq::sm_count();
+    w.record_floats = d == 256 ? decode::Shape<256>::RECORD : decode::Shape<128>::RECORD;
+    w.bytes = (size_t)w.ctas * 16 + (size_t)2 * w.ctas * w.record_floats * 4;
+    return w;
+}
+
+template <int D, bool BF16>
+int launch_decode(const khq_paged_attn_args& a, const Params& p, const Work& w, cudaStream_t stream) {
+    using S = decode::Shape<D>;
+    static bool attr_done[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    if (dev < 0 || dev >= 64) return -100;
+    if (!attr_done[dev]) {
+        err = cudaFuncSetAttribute((const void*)decode::khq_paged_decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (err != cudaSuccess) return static_cast<int>(err);
+        attr_done[dev] = true;
+    }
+    CUtensorMap mk, mv;
+    int rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
+    if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
+    if (rc != 0) return rc;
+    err = khq::launch_pdl(decode::khq_paged_decode_kernel<D, BF16>, (unsigned)w.ctas, 0, (size_t)S::SMEM, stream, (unsigned)(decode::WARPS * 32), mk, mv, p);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)w.ctas, 4, 1);
+    cfg.blockDim = dim3(128, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, khq_paged_merge_kernel<D, BF16>, p, DECODE_ROWS, w.record_floats, w.ctas));
+}
+
+bool heads_ok(int H_q, int H_kv) { return H_q > 0 && H_kv > 0 && H_q % H_kv == 0 && H_q / H_kv <= MAX_REP; }
+
+int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream) {
+    if (!args) return -100;
+    const khq_paged_attn_args& a = *args;
+    if (a.tokens <= 0 || a.max_tokens <= 0 || a.max_new <= 0 || a.requests <= 0 || a.max_pages <= 0 || a.n_pages <= 0 || a.H_q <= 0 || a.H_kv <= 0 || !a.q ||
+        !a.k_cache || !a.v_cache || !a.block_table || !a.cu_new || !a.kv_lens || !a.schedule || !a.out || !a.workspace)
+        return -100;
+    if (!(a.scale > 0.0f) || !(a.scale <= 3.0e38f)) return -100;
+    const int shift = a.page_size == 16 ? 4 : a.page_size == 32 ? 5 : a.page_size == 64 ? 6 : a.page_size == 128 ? 7 : -1;
+    if (shift < 0 || (a.d != 128 && a.d != 256) || !heads_ok(a.H_q, a.H_kv) || a.table_stride < a.max_pages) return -103;
+    const void* ptrs[] = {a.q, a.gate, a.k_cache, a.v_cache, a.out, a.schedule};
+    for (const void* x : ptrs)
+        if ((reinterpret_cast<uintptr_t>(x) & 15) != 0) return -104;
+    const void* ints[] = {a.block_table, a.cu_new, a.kv_lens, a.lse};
+    for (const void* x : ints)
+        if ((reinterpret_cast<uintptr_t>(x) & 3) != 0) return -104;
+    if ((reinterpret_cast<uintptr_t>(a.workspace) & 255) != 0) return -104;
+    for (int i = 0; i < 2; ++i)
+        if (((a.q_stride[i] | (a.gate ? a.gate_stride[i] : 0) | a.out_stride[i]) & 7) != 0) return -104;
+    for (int i = 0; i < 3; ++i)
+        if (((a.k_cache_stride[i] | a.v_cache_stride[i]) & 7) != 0 || a.k_cache_stride[i] < 0 || a.v_cache_stride[i] < 0) return -104;
+    const Tile tile = tile_of(a.H_q, a.H_kv, a.max_new);
+    const long long items = max_items(a.requests, a.max_tokens, tile.tokens);
+    const Work w = work_of(tile, a.d);
+    if (a.schedule_bytes < (size_t)schedule_ints(items) * 4 || a.workspace_bytes < w.bytes) return -105;
+    Params p;
+    p.q = static_cast<const uint16_t*>(a.q);
+    p.gate = static_cast<const uint16_t*>(a.gate);
+    p.out = static_cast<uint16_t*>(a.out);
+    p.lse = static_cast<float*>(a.lse);
+    p.q_ts = a.q_stride[0];
+    p.q_hs = a.q_stride[1];
+    p.g_ts = a.gate_stride[0];
+    p.g_hs = a.gate_stride[1];
+    p.o_ts = a.out_stride[0];
+    p.o_hs = a.out_stride[1];
+    p.table_stride = a.table_stride;
+    p.table = static_cast<const int*>(a.block_table);
+    p.cu_new = static_cast<const int*>(a.cu_new);
+    p.kv_lens = static_cast<const int*>(a.kv_lens);
+    p.schedule = static_cast<const int*>(a.schedule);
+    p.items = reinterpret_cast<const Item*>(p.schedule + SCHED_HEADER);
+    p.cum = p.schedule + SCHED_HEADER + 4 * items;
+    p.meta = static_cast<int4*>(a.workspace);
+    p.records = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + (size_t)w.ctas * 16);
+    p.tokens = a.tokens;
+    p.max_pages = a.max_pages;
+    p.n_pages = a.n_pages;
+    p.page_shift = shift;
+    p.page_mask = a.page_size - 1;
+    p.H_q = a.H_q;
+    p.H_kv = a.H_kv;
+    p.n_rep = a.H_q / a.H_kv;
+    p.scale_log2e = a.scale * 1.4426950408889634f;
+    if (a.d == 256) return bf16 ? launch_decode<256, true>(a, p, w, stream) : launch_decode<256, false>(a, p, w, stream);
+    return bf16 ? launch_decode<128, true>(a, p, w, stream) : launch_decode<128, false>(a, p, w, stream);
+}
+
+}  // namespace
+
+extern "C" size_t khq_b200_paged_workspace_bytes(int max_new, int H_q, int H_kv, int d) {
+    if (max_new <= 0 || !heads_ok(H_q, H_kv) || (d != 128 && d != 256)) return 0;
+    return (work_of(tile_of(H_q, H_kv, max_new), d).bytes + 255) / 256 * 256;
+}
+
+extern "C" int launch_khq_paged_attn_fp16(const khq_paged_attn_args* args, khq_stream_t stream) { return launch_attn(args, false, stream); }
+
+extern "C" int launch_khq_paged_attn_bf16(const khq_paged_attn_args* args, khq_stream_t stream) { return launch_attn(args, true, stream); }
+
+extern "C" int khq_b200_paged_status(void) {
+    int st = 0;
+    if (cudaMemcpyFromSymbol(&st, khq_paged::g_paged_status, sizeof(int)) != cudaSuccess) return -1;
+    if (st != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(khq_paged::g_paged_status, &zero, sizeof(int));
+    }
+    return st;
+}

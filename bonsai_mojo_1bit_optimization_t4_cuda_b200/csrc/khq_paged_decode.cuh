@@ -1,0 +1,320 @@
+// khq_paged_decode.cuh -- attention over the paged cache for tiles of up to 16 query rows (a decode step: one or a few new tokens a
+// request).  Included by khq_paged_attn.cu.
+//
+// Every K and V byte is used by 16 rows at most, so the cache's bytes bound it.  The key blocks (64 keys) of all (kv head,
+// item) pairs stand in one row, and each CTA takes an equal stretch of it (one CTA per SM): any mix of lengths is even, and a CTA ends up with at most two
+// segments that it shares with others.  Those leave records (unnormalised rows, maximum, sum) that khq_paged_merge_kernel joins
+// in a fixed order; the others are finished here.
+//
+// A warp takes 16 keys of each block and runs alone: its first lane brings the 16 rows of K and V in by TMA (pages of 16 tokens and more hold
+// them in one piece) some units ahead, into a ring that no other warp touches; S = Q K^T and O += P V are mma.sync m16n8k16 with the query rows
+// as M and all of O in registers.  Only at a segment's end the four warps join their maxima, sums and rows through shared memory.
+#pragma once
+
+namespace khq_paged {
+namespace decode {
+
+constexpr int WARPS = 4, UNIT = 16;  // keys a warp takes at a time
+static_assert(WARPS * UNIT == DECODE_KEYS, "a block is a unit per warp");
+template <int D> struct Shape {
+    static constexpr int UNIT_BYTES = UNIT * D * 2, STAGE_BYTES = 2 * UNIT_BYTES, STAGES = 3 * 256 / D;
+    static constexpr int ROW = D + 8;  // floats of a row in the join buffer: rows 8 banks apart
+    static constexpr int OFF_JOIN = WARPS * STAGES * STAGE_BYTES, OFF_ML = OFF_JOIN + WARPS * 8 * ROW * 4;
+    static constexpr int OFF_BARS = OFF_ML + WARPS * DECODE_ROWS * 8, SMEM = OFF_BARS + WARPS * STAGES * 8;
+    static constexpr int RECORD = DECODE_ROWS * D + 2 * DECODE_ROWS;  // floats
+};
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t at, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t at, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(WARPS * 32, 1)
+khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
+    using S = Shape<D>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BARS);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int* const status = &g_paged_status;
+    if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled layout needs a 1024-byte aligned base
+        if (tid == 0) atomicExch(status, 2);
+        return;
+    }
+    if (lane == 0) {
+        for (int s = 0; s < S::STAGES; ++s) khq::mbar_init(&bars[warp * S::STAGES + s], 1);
+        khq::fence_barrier_init();
+    }
+    __syncthreads();
+    khq::pdl_wait();
+    khq::pdl_trigger();
+
+    // ---- this CTA's stretch of the key blocks ------------------------------------------------------
+    const int n_items = p.schedule[0];
+    const long long per_head = p.schedule[1], total = per_head * p.H_kv;
+    const long long lo = blockIdx.x * total / gridDim.x, hi = (blockIdx.x + 1) * total / gridDim.x;
+    if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);  // overwritten below if a segment goes on in the next CTA
+    if (lo >= hi) return;
+    Segment in, cur;  // where the loads and where the products are
+    find_segment(p, n_items, per_head, lo, in);
+    cur = in;
+    uint64_t* const bar = bars + warp * S::STAGES;
+    const uint32_t ring = smem_u32(smem) + warp * S::STAGES * S::STAGE_BYTES;
+
+    // ---- loads ---------------------------------------------------------------------------------------
+    // Lane i of `pages` has the page of the unit i blocks behind `pages_at`, the next 32 are on their way; n_pages: none (the copy then fills in
+    // zeros, and the unit is skipped).
+    int pages = 0, pages_next = 0, pages_at = -1;
+    long long w_in = lo;
+    int s_in = 0;
+    uint32_t missing = 0;  // by stage: the unit has no page
+    bool ok = true;        // no wait has run out
+    int issued = 0;        // units, by lane 0
+    const auto fetch_pages = [&](int blk) {
+        const int key = (blk + lane) * DECODE_KEYS + warp * UNIT, col = key >> p.page_shift;
+        int pg = p.n_pages;
+        if (key < in.kv && col < p.max_pages) {
+            pg = __ldg(p.table + in.b * p.table_stride + col);
+            if ((unsigned)pg >= (unsigned)p.n_pages) pg = p.n_pages;
+        }
+        return pg;
+    };
+    const auto issue = [&]() {
+        if (w_in >= hi) return;
+        if (pages_at < 0 || in.blk - pages_at >= 32) {
+            pages = pages_at < 0 ? fetch_pages(in.blk) : pages_next;
+            pages_at = in.blk;
+            pages_next = fetch_pages(in.blk + 32);
+        }
+        const int page = __shfl_sync(0xFFFFFFFFu, pages, in.blk - pages_at);
+        const int key = in.blk * DECODE_KEYS + warp * UNIT;
+        missing = (missing & ~(1u << s_in)) | ((uint32_t)(page == p.n_pages) << s_in);
+        if (ok && lane == 0) {
+            ++issued;
+            const uint32_t dst = ring + s_in * S::STAGE_BYTES;
+            khq::mbar_arrive_expect_tx(&bar[s_in], S::STAGE_BYTES);
+            tma_load_5d(dst, &tm_k, &bar[s_in], key & p.page_mask, 0, in.h, page);
+            tma_load_5d(dst + S::UNIT_BYTES, &tm_v, &bar[s_in], key & p.page_mask, 0, in.h, page);
+        }
+        s_in = s_in + 1 == S::STAGES ? 0 : s_in + 1;
+        ++w_in;
+        if (++in.blk == in.n_blocks && w_in < hi) {
+            next_segment(p, n_items, in);
+            pages_at = -1;
+        }
+    };
+#pragma unroll 1
+    for (int s = 0; s < S::STAGES; ++s) issue();
+
+    // ---- products ------------------------------------------------------------------------------------
+    const int g = lane >> 2, t2 = (lane & 3) * 2;  // rows g and g + 8, columns t2 and t2 + 1 of a fragment
+    uint32_t qf[D / 16][4];
+    float o[D / 8][4], m[2], l[2];
+    // addresses of this lane's rows for ldmatrix; chunk c of key k is at (c ^ (k & 7)) << 4
+    const int k_key = (lane & 7) + ((lane >> 4) & 1) * 8, k_chunk = (lane >> 3) & 1;
+    const int v_key = (lane & 7) + ((lane >> 3) & 1) * 8, v_chunk = lane >> 4;
+    const uint32_t k_row = k_key * 128, v_row = S::UNIT_BYTES + v_key * 128, sw = (lane & 7);
+    int s = 0;
+    uint32_t phase = 0;
+    bool fresh = true;
+    const int R_max = DECODE_ROWS;
+#pragma unroll 1
+    for (long long w = lo; w < hi; ++w) {
+        const int R = cur.ntok * p.n_rep;
+        if (fresh) {
+            fresh = false;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = g + 8 * half, row = cur.row0 + r / p.n_rep;
+                const bool live = r < R && row < p.tokens;
+                const uint16_t* q = p.q + (live ? row * p.q_ts + (long long)(cur.h * p.n_rep + r % p.n_rep) * p.q_hs : 0) + t2;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    qf[kk][half] = live ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16)) : 0u;
+                    qf[kk][2 + half] = live ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16 + 8)) : 0u;
+                }
+                m[half] = -INFINITY;
+                l[half] = 0.0f;
+            }
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        }
+        // (after a wait that ran out the warp goes on without data, so that the others are not left at a barrier; the status word tells)
+        ok = ok && __all_sync(0xFFFFFFFFu, khq::mbar_wait_bounded(&bar[s], phase, status));
+        const int key0 = cur.blk * DECODE_KEYS + warp * UNIT;
+        if (ok && !((missing >> s) & 1u)) {
+            const uint32_t base = ring + s * S::STAGE_BYTES;
+            float x[2][4] = {}, y[2][4] = {};  // two chains each
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                uint32_t b[4];
+                ldsm4(base + (kk >> 2) * (UNIT * 128) + k_row + (((uint32_t)((kk & 3) * 2 + k_chunk) ^ sw) << 4), b);
+                if (kk & 1) {
+                    mma16816<BF16>(y[0], qf[kk], b[0], b[1]);
+                    mma16816<BF16>(y[1], qf[kk], b[2], b[3]);
+                } else {
+                    mma16816<BF16>(x[0], qf[kk], b[0], b[1]);
+                    mma16816<BF16>(x[1], qf[kk], b[2], b[3]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][e] = (x[n][e] + y[n][e]) * p.scale_log2e;
+            const bool tail = key0 + UNIT > cur.kv;
+            if (key0 + UNIT - 1 > cur.pos0) {  // some row's position lies in front of the unit's last key
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int at = cur.pos0 + (g + 8 * half) / p.n_rep;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (key0 + n * 8 + t2 + e > at) x[n][half * 2 + e] = -INFINITY;
+                }
+            }
+            float factor[2];
+            bool grow = false;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float mx = fmaxf(fmaxf(x[0][half * 2], x[0][half * 2 + 1]), fmaxf(x[1][half * 2], x[1][half * 2 + 1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+                factor[half] = 1.0f;
+                // the reference follows the maximum only when that has grown by more than 2^8: fewer passes over O, and nothing leaves fp32's or
+                // the 16-bit weights' range
+                if (mx > m[half] + 8.0f) {
+                    factor[half] = exp2f(m[half] - mx);
+                    m[half] = mx;
+                    grow = true;
+                }
+            }
+            uint32_t pf[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float ref = m[half] == -INFINITY ? 0.0f : m[half];
+                const float p0 = ex2_approx(x[0][half * 2] - ref), p1 = ex2_approx(x[0][half * 2 + 1] - ref);
+                const float p2 = ex2_approx(x[1][half * 2] - ref), p3 = ex2_approx(x[1][half * 2 + 1] - ref);
+                l[half] = l[half] * factor[half] + ((p0 + p1) + (p2 + p3));
+                pf[half] = pack2<BF16>(p0, p1);
+                pf[2 + half] = pack2<BF16>(p2, p3);
+            }
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) {
+                    o[n][0] *= factor[0];
+                    o[n][1] *= factor[0];
+                    o[n][2] *= factor[1];
+                    o[n][3] *= factor[1];
+                }
+            }
+            // rows of V behind the request's last token may hold anything: a weight of 0 does not undo that
+            uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
+            if (tail) {
+                const int n = cur.kv - key0;  // keys that exist; this lane's are t2, t2 + 1 and those 8 further
+                keep0 = (t2 < n ? 0x0000FFFFu : 0u) | (t2 + 1 < n ? 0xFFFF0000u : 0u);
+                keep1 = (t2 + 8 < n ? 0x0000FFFFu : 0u) | (t2 + 9 < n ? 0xFFFF0000u : 0u);
+            }
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                uint32_t b[4];
+                ldsm4_trans(base + (n >> 2) * (UNIT * 128) + v_row + (((uint32_t)((n & 3) * 2 + v_chunk) ^ sw) << 4), b);
+                mma16816<BF16>(o[2 * n], pf, b[0] & keep0, b[1] & keep1);
+                mma16816<BF16>(o[2 * n + 1], pf, b[2] & keep0, b[3] & keep1);
+            }
+        }
+        __syncwarp();  // all lanes have read the stage
+        s = s + 1 == S::STAGES ? 0 : s + 1;
+        phase ^= (uint32_t)(s == 0);
+        issue();
+        const bool ends = cur.blk + 1 == cur.n_blocks;
+        if (ends || w + 1 == hi) {
+            // ---- join the warps ----------------------------------------------------------------------
+            const long long seg_lo = w - cur.blk, seg_hi = seg_lo + cur.n_blocks;
+            const bool whole = seg_lo >= lo && seg_hi <= hi;
+            float* const join = reinterpret_cast<float*>(smem + S::OFF_JOIN);
+            float2* const ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 1);
+                l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 2);
+                if ((lane & 3) == 0) ml[warp * R_max + g + 8 * half] = make_float2(m[half], l[half]);
+            }
+            __syncthreads();
+            const auto top = [&](int r) {
+                float M = ml[r].x;
+#pragma unroll
+                for (int v = 1; v < WARPS; ++v) M = fmaxf(M, ml[v * R_max + r].x);
+                return M;
+            };
+            float* const rec = p.records + (2LL * blockIdx.x + (seg_lo >= lo ? 1 : 0)) * S::RECORD;
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                if (half * 8 >= R) break;
+                const float M = top(g + 8 * half), f = m[half] == -INFINITY ? 0.0f : exp2f(m[half] - M);
+                float* const mine = join + (warp * 8 + g) * S::ROW + t2;
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)
+                    *reinterpret_cast<float2*>(mine + n * 8) = half == 0 ? make_float2(o[n][0] * f, o[n][1] * f) : make_float2(o[n][2] * f, o[n][3] * f);
+                __syncthreads();
+                const int rr = tid >> 4, r = rr + 8 * half;  // 16 threads a row
+                if (r < R) {
+                    const float Mr = top(r);
+                    float L = 0.0f;
+#pragma unroll
+                    for (int v = 0; v < WARPS; ++v) {
+                        const float2 a = ml[v * R_max + r];
+                        L += a.x == -INFINITY ? 0.0f : a.y * exp2f(a.x - Mr);
+                    }
+                    const int row = cur.row0 + r / p.n_rep, head = cur.h * p.n_rep + r % p.n_rep;
+                    const bool live = row < p.tokens;
+                    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;  // a NaN stays one
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) {
+                        const int c = j * 64 + (tid & 15) * 4;
+                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                        for (int v = 0; v < WARPS; ++v) {
+                            const float4 a = *reinterpret_cast<const float4*>(join + (v * 8 + rr) * S::ROW + c);
+                            acc.x += a.x;
+                            acc.y += a.y;
+                            acc.z += a.z;
+                            acc.w += a.w;
+                        }
+                        if (!whole) *reinterpret_cast<float4*>(rec + r * D + c) = acc;
+                        else if (live) store_out<BF16>(p, row, head, c, acc, inv);
+                    }
+                    if ((tid & 15) == 0) {
+                        if (!whole) *reinterpret_cast<float2*>(rec + DECODE_ROWS * D + 2 * r) = make_float2(Mr, L);
+                        else if (live && p.lse) p.lse[(long long)row * p.H_q + head] = (Mr + log2f(L)) * 0.6931471805599453f;
+                    }
+                }
+                __syncthreads();
+            }
+            if (tid == 0 && seg_lo >= lo && seg_hi > hi)
+                p.meta[blockIdx.x] = make_int4((int)((seg_hi * gridDim.x - 1) / total) - (int)blockIdx.x + 1, cur.item, cur.h, 0);
+            fresh = true;
+        }
+        ++cur.blk;
+        if (ends && w + 1 < hi) next_segment(p, n_items, cur);
+    }
+    // nothing this warp started may still be in flight when the CTA leaves
+    if (!ok && lane == 0)
+        for (int i = max(0, issued - S::STAGES); i < issued; ++i) khq::mbar_wait_bounded(&bar[i % S::STAGES], (uint32_t)((i / S::STAGES) & 1), status);
+}
+
+}  // namespace decode
+}  // namespace khq_paged

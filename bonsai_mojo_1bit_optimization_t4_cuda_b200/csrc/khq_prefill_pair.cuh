@@ -41,88 +41,6 @@ constexpr int SMEM = OFF_SLOT + 16;
 static_assert(2 * STG_BYTES <= Q_BYTES && SMEM <= 227 * 1024, "shared memory");
 __host__ __device__ constexpr int off_piece(int c) { return c < 2 ? OFF_STG + c * STG_BYTES : OFF_Q + (c - 2) * STG_BYTES; }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-// (d0, d1) = (a0, a1) m + c and (s0, s1) += (a0, a1), one packed instruction each
-__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float m, float c) {
-    asm("{.reg .b64 a, m, c, d; mov.b64 a, {%2, %3}; mov.b64 m, {%4, %4}; mov.b64 c, {%5, %5}; fma.rn.f32x2 d, a, m, c; mov.b64 {%0, %1}, d;}"
-        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(m), "f"(c));
-}
-__device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
-    asm("{.reg .b64 a, s; mov.b64 a, {%2, %3}; mov.b64 s, {%0, %1}; add.rn.f32x2 s, s, a; mov.b64 {%0, %1}, s;}" : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]),
-                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-                 "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-                 : "memory");
-}
-// The MMA warp stays together and one lane issues (`one`): its descriptors are then values of the whole warp, kept and stepped in uniform
-// registers.  With one lane alone inside a branch each instruction's operands had to be moved there one by one, which took about as
-// long as the pipe takes for the instruction, or longer by the luck of the code's placement (4 x 8192: 2.42 ms, 2.49 to 2.95).
-template <int ACC>
-__device__ __forceinline__ void umma2_ss(uint32_t one, uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc) {
-    asm volatile(
-        "{\n\t.reg .b64 da, db;\n\t.reg .pred p, q;\n\t"
-        "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
-        "setp.ne.u32 p, %6, 0;\n\tsetp.ne.u32 q, %7, 0;\n\t"
-        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ACC), "r"(one)
-        : "memory");
-}
-__device__ __forceinline__ void umma2_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                         uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .b64 db;\n\t.reg .pred p, q;\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "setp.ne.u32 p, %5, 0;\n\tsetp.ne.u32 q, %6, 0;\n\t"
-        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(one)
-        : "memory");
-}
-// Arrives at this barrier of both CTAs once the instructions issued so far have completed.
-__device__ __forceinline__ void umma2_commit(uint32_t one, uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
-        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
-        "h"((uint16_t)3), "r"(one)
-        : "memory");
-}
-// The address of `bar` in the pair's first CTA.
-__device__ __forceinline__ uint32_t in_leader(uint64_t* bar) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
-    return r;
-}
-__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
-}
-// A load into this CTA's shared memory whose bytes count at a barrier of the pair's first CTA.
-__device__ __forceinline__ void load_for_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c1, int c2, int c3, int c4) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, "
-        "%6, %7}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
-        : "memory");
-}
-// Of the MMA warp's barriers too: the other CTA's arrivals announce tensor-memory contents and asynchronous copies, which the tcgen05
-// fences and the copies' byte counts order, not ordinary memory.  Acquiring at cluster scope cost 4 to 8 %.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-
 // Item of a pair: (batch, kv head) groups one after the other, the heaviest row blocks first inside a group: what is in flight then
 // streams the K and V rows of one or two groups, which stay in L2, and the hardware's scheduler evens out the triangle.
 // q_gate (B, T, H_q, 2D), out (B, T, H_q, D) through their tensor maps; grid = 2 x row blocks x H_q / 2 x B.

@@ -71,6 +71,14 @@ SIGNATURES = {
     "launch_khq_compress_batched_fp16": (
         c_int, [_P, c_int, c_int] + [_P] * 9 + [c_int, c_float, c_float, c_int, c_longlong, _P]),
     "launch_khq_update_descs": (c_int, [_P, _P, c_int, c_int, _P]),
+    "khq_b200_paged_schedule_bytes": (c_size_t, [c_int] * 5),
+    "launch_khq_paged_plan": (c_int, [_P, _P]),
+    "launch_khq_paged_prestep_fp16": (c_int, [_P, _P]),
+    "launch_khq_paged_prestep_bf16": (c_int, [_P, _P]),
+    "khq_b200_paged_workspace_bytes": (c_size_t, [c_int] * 4),
+    "launch_khq_paged_attn_fp16": (c_int, [_P, _P]),
+    "launch_khq_paged_attn_bf16": (c_int, [_P, _P]),
+    "khq_b200_paged_status": (c_int, []),
     "launch_khq_cal_kstatic_fp32": (c_int, [_P, c_int, _P, _P, _P, _P]),
     "khq_b200_version": (c_char_p, []),
     "khq_b200_device_status": (c_int, []),

@@ -355,6 +355,80 @@ int khq_b200_engine_destroy(khq_engine* engine);
 int khq_b200_engine_wait_control(khq_engine* engine, int parity);
 int launch_khq_engine_step(khq_engine* engine, const khq_engine_layer* layers, const khq_engine_step* step, khq_stream_t stream);
 
+/* ---- Prompts in chunks: a raw paged K/V cache (no counterpart in the reference, whose chunks of a prompt go into one dense
+ * cache, main.mojo:1651-1734) -----------------------------------------------------------------------------------------------
+ * The exact attention of a chunk needs the raw K and V of the chunks before it.  They stand in pages of 16, 32, 64 or 128 tokens,
+ * shared by all requests of a server, until the prompt is complete and its pages are compressed
+ * (launch_khq_compress_batched_fp16 takes a page of a token-major cache as a run).  A step is: one plan for all layers, then per
+ * layer the pre-step and the attention.  Shapes: d 128 or 256, H_q a multiple of H_kv, at most 16 query heads per kv head.
+ *
+ * The plan.  ctx_lens (requests): tokens that a request has in the cache; new_lens (requests): tokens that the step adds, -1: the
+ * request has ended (its pages go back), both int32.  block_table (requests, table_stride) int32: page numbers, max_pages of a row in
+ * use.  free_list (n_pages) int32, free_count (1) int32: the free pages are the first free_count entries and are taken from the
+ * end, for requests in row order; pages that come back stand behind the others, in row order, before any is taken, and are
+ * written to free_list; free_count_out may be free_count.  free_list == NULL: the table has the new tokens' pages already.  Written: the
+ * table entries of taken pages; cu_new (requests + 1) int32, the first row of each request in the step's ragged tensors; kv_lens
+ * (requests) int32, its tokens behind the step (0: ended); positions (max_tokens) int32 and slots (max_tokens) int64 of the rows,
+ * slot = page * page_size + position % page_size, -1 behind the last row; info (8) int32: rows, pages taken, pages given back, pages
+ * missing, rows dropped, pages free; schedule: what the attention runs from, schedule_bytes >= khq_b200_paged_schedule_bytes(...)
+ * at 16 bytes.  A row gets at most max_new tokens and all together max_tokens, the rest is dropped.  When pages run out, the table
+ * gets -1 and so do the slots: such tokens are not stored and not attended.  Returns -100 (arguments), -103 (a page size, head counts, more than
+ * 16384 requests, 2^20 tokens or 2^30 tokens of a table row), -104 (alignment), -105 (schedule too small). */
+typedef struct khq_paged_plan_args {
+    const void *ctx_lens, *new_lens;
+    void *block_table, *free_list;
+    const void* free_count;
+    void *free_count_out, *cu_new, *kv_lens, *positions, *slots, *info, *schedule;
+    size_t schedule_bytes;
+    long long table_stride;
+    int32_t requests, max_pages, n_pages, page_size, max_tokens, max_new, H_q, H_kv;
+} khq_paged_plan_args;
+size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, int H_q, int H_kv); /* 0: bad arguments */
+int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream_t stream);
+
+/* The pre-step of `tokens` rows: head RMS norms of q and k (fp32 weights of d, or NULL), rotation of the pairs (i, i + rotary_dim / 2) of the first
+ * rotary_dim dims (a multiple of 16, 0: none) at the rows' positions, q to q_out (which may be q), K rotated, V and, unless
+ * u_cache is NULL, K not rotated into the slots of the caches.  fp32 inside, each stored value rounded once.  Rows with position < 0 are
+ * left alone, rows whose slot is not in the cache get their q only.  q (tokens, H_q, d), k and v (tokens, H_kv, d), caches (n_pages, page_size,
+ * H_kv, d): strides in elements (multiples of 8), the last dim contiguous; pointers at 16 bytes.  Returns -100, -103, -104. */
+typedef struct khq_paged_prestep_args {
+    const void *q, *k, *v, *q_norm_w, *k_norm_w;
+    void *q_out, *k_cache, *v_cache, *u_cache;
+    const void *positions, *slots;
+    int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2];          /* token, head */
+    int64_t k_cache_stride[3], v_cache_stride[3], u_cache_stride[3];         /* page, token, head */
+    int32_t tokens, n_pages, page_size, H_q, H_kv, d, rotary_dim;
+    float rope_theta, rms_eps;
+} khq_paged_prestep_args;
+int launch_khq_paged_prestep_fp16(const khq_paged_prestep_args* args, khq_stream_t stream);
+int launch_khq_paged_prestep_bf16(const khq_paged_prestep_args* args, khq_stream_t stream);
+
+/* Attention of a step's rows over the cache: row t of request b attends the positions 0..positions[t] of b,
+ *   out[t,h,:] = softmax_u(q[t,h] . K[u,h / n_rep] * scale) V[u,h / n_rep] * sigmoid(gate[t,h,:])      (gate NULL: without)
+ * and, unless lse is NULL, lse[t,h] = log sum_u exp(q . K * scale) (tokens, H_q) fp32.  Softmax statistics, weights' sums and outputs in fp32;
+ * the weights enter the product with V as 16-bit values.  A row that attends nothing (no page of it could be had) gets out 0 and lse
+ * -inf.  Stale cache rows behind a request's last token are not attended, whatever they hold, NaN included.  cu_new, kv_lens and
+ * schedule are a plan's, max_tokens, max_new, requests, page_size and the head counts the same as there; `tokens` rows of q, gate,
+ * out and lse exist (the plan must not have more).  Page numbers outside 0..n_pages-1 are not attended.  Rows behind the plan's last are left alone.
+ * scale > 0.  workspace: khq_b200_paged_workspace_bytes(...) at 256 bytes; calls that may run at the same time need their own.  Returns -100, -103,
+ * -104, -105, -107 / -108 (no tensor map). */
+typedef struct khq_paged_attn_args {
+    const void *q, *gate, *k_cache, *v_cache, *block_table, *cu_new, *kv_lens, *schedule;
+    void *out, *lse, *workspace;
+    size_t schedule_bytes, workspace_bytes;
+    int64_t q_stride[2], gate_stride[2], out_stride[2];                      /* token, head */
+    int64_t k_cache_stride[3], v_cache_stride[3];                            /* page, token, head */
+    long long table_stride;
+    int32_t tokens, max_tokens, max_new, requests, max_pages, n_pages, page_size, H_q, H_kv, d;
+    float scale;
+} khq_paged_attn_args;
+size_t khq_b200_paged_workspace_bytes(int max_new, int H_q, int H_kv, int d); /* of the current device; 0: bad arguments */
+int launch_khq_paged_attn_fp16(const khq_paged_attn_args* args, khq_stream_t stream);
+int launch_khq_paged_attn_bf16(const khq_paged_attn_args* args, khq_stream_t stream);
+/* Reads and clears the status word of the paged attention on the current device (synchronises): 0 clean, 1 a bounded wait ran out, 2
+ * misaligned shared memory. */
+int khq_b200_paged_status(void);
+
 /* ---- Prefill: causal GQA attention + sigmoid gate over a whole prompt --------------------
  * The math of the reference's fp16-KV attention kernel (gqa_attention_sm75_gpu,
  * src/kernels/elementwise_sm75.mojo:1091-1231), which the reference launches once per prompt
