@@ -167,16 +167,19 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         if (tid == 0) taken[B] = items;
         __syncthreads();
         Item* const list = reinterpret_cast<Item*>(a.schedule + SCHED_HEADER);
-        int* const cum = a.schedule + SCHED_HEADER + 4 * a.item_cap;
+        int* const cum = a.schedule + SCHED_HEADER + ITEM_INTS * a.item_cap;
         int blocks = 0;
         for (int i0 = 0; i0 < items; i0 += PLAN_THREADS) {
             const int i = i0 + tid;
-            Item it = {0, 0, 0, 0};
+            Item it = {};
             if (i < items) {
                 it.b = find(taken, B, i);
-                it.q0 = (i - taken[it.b]) * a.tile_tokens;
-                it.ntok = min(a.tile_tokens, cu[it.b + 1] - cu[it.b] - it.q0);
-                it.n_blocks = (ctx_of(it.b) + it.q0 + it.ntok + a.tile_keys - 1) / a.tile_keys;
+                const int q0 = (i - taken[it.b]) * a.tile_tokens, kept = cu[it.b + 1] - cu[it.b], ctx = ctx_of(it.b);
+                it.ntok = min(a.tile_tokens, kept - q0);
+                it.n_blocks = (ctx + q0 + it.ntok + a.tile_keys - 1) / a.tile_keys;
+                it.kv = ctx + kept;
+                it.row0 = cu[it.b] + q0;
+                it.pos0 = ctx + q0;
             }
             int n = it.n_blocks, z = 0, total;
             block_scan2(n, z, part, total, u);

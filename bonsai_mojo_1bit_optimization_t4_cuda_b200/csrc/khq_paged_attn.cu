@@ -1,5 +1,5 @@
 // khq_paged_attn.cu -- attention of a step's new tokens over a raw paged K/V cache: the kernels' common part, the joining of shared
-// segments and the host side.  The kernels: khq_paged_decode.cuh (few rows a request).
+// segments and the host side.  The kernels: khq_paged_decode.cuh (few rows a request), khq_paged_tile.cuh (chunks).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -20,12 +20,37 @@ using namespace khq_tc5;
 
 __device__ int g_paged_status = 0;
 
+// Waits give up after two seconds, record that in the status word and return false.  (A count of polls says little: a poll may
+// park the thread for a while.)  `any` joins the lanes that wait together: their tests and their clocks have to agree.
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+template <class Test, class Any>
+__device__ __forceinline__ bool bounded(Test test, Any any, int* status) {
+    unsigned long long begin = 0;
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i)
+            if (any(test())) return true;
+        const unsigned long long now = now_ns();
+        if (begin == 0) begin = now;
+        if (any(now - begin > 2000000000ull)) break;
+    }
+    atomicExch(status, 1);
+    return false;
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* status) {
+    return bounded([&] { return khq::mbar_try_wait(bar, parity); }, [](bool x) { return x; }, status);
+}
+
 struct Params {
     const uint16_t *q, *gate;
     uint16_t* out;
     float* lse;
     long long q_ts, q_hs, g_ts, g_hs, o_ts, o_hs, table_stride;
-    const int *table, *cu_new, *kv_lens, *schedule;
+    const int *table, *schedule;
     const Item* items;
     const int* cum;
     float* records;
@@ -39,14 +64,14 @@ struct Segment {
     int item, h, b, n_blocks, blk, ntok, kv, row0, pos0;  // row0: its first row in the ragged tensors, pos0: that row's position
 };
 __device__ __forceinline__ void load_segment(const Params& p, Segment& s) {
-    const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + s.item);
-    s.b = it.x;
-    s.ntok = it.z;
-    s.n_blocks = it.w;
-    const int first = __ldg(p.cu_new + it.x);
-    s.kv = __ldg(p.kv_lens + it.x);
-    s.row0 = first + it.y;
-    s.pos0 = s.kv - (__ldg(p.cu_new + it.x + 1) - first) + it.y;
+    const int4* it = reinterpret_cast<const int4*>(p.items + s.item);
+    const int4 x = __ldg(it), y = __ldg(it + 1);
+    s.b = x.x;
+    s.n_blocks = x.y;
+    s.ntok = x.z;
+    s.kv = x.w;
+    s.row0 = y.x;
+    s.pos0 = y.y;
 }
 // Block w of the row of all blocks.  A warp bisects by 32.
 __device__ __forceinline__ void find_segment(const Params& p, int n_items, long long per_head, long long w, Segment& s) {
@@ -100,8 +125,10 @@ __global__ void __launch_bounds__(128) khq_paged_merge_kernel(const Params p, in
     khq::pdl_trigger();
     const int4 meta = p.meta[blockIdx.x];
     if (meta.x == 0) return;
-    const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + meta.y);
-    const int R = it.z * p.n_rep, row0 = __ldg(p.cu_new + it.x) + it.y;
+    Segment seg;
+    seg.item = meta.y;
+    load_segment(p, seg);
+    const int R = seg.ntok * p.n_rep, row0 = seg.row0;
     constexpr int PER_ROW = D / 4;  // threads a row
     const int c = (threadIdx.x % PER_ROW) * 4;
     const long long total = (long long)p.schedule[1] * p.H_kv;
@@ -139,6 +166,7 @@ __global__ void __launch_bounds__(128) khq_paged_merge_kernel(const Params p, in
 }  // namespace khq_paged
 
 #include "khq_paged_decode.cuh"
+#include "khq_paged_tile.cuh"
 
 // ---- host side -----------------------------------------------------------------------------------
 namespace {
@@ -179,18 +207,47 @@ int cache_map(CUtensorMap* map, const void* base, const int64_t (&stride)[3], in
     return r == CUDA_SUCCESS ? 0 : -108;
 }
 
-// Bytes of the workspace: two records per CTA and one line of `meta`.
+// Queries (tokens, heads, d) as {64 values, head, token, column group}; a box is a column group of one kv head's heads of `box_tokens` tokens.
+int query_map(CUtensorMap* map, const void* base, const int64_t (&stride)[2], int tokens, int heads, int d, int box_heads, int box_tokens, bool bf16) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return -107;
+    const cuuint64_t dims[4] = {64, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)(d / 64)};
+    const auto bytes = [](int64_t s, int n) { return n == 1 ? (cuuint64_t)16 : (cuuint64_t)s * 2; };
+    const cuuint64_t strides[3] = {bytes(stride[1], heads), bytes(stride[0], tokens), 128};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : -108;
+}
+
+// The workspace: a line of `meta` and two records per CTA.
 struct Work {
     int ctas, record_floats;
     size_t bytes;
 };
 Work work_of(const Tile& tile, int d) {
     Work w;
-    (void)tile;
-    w.ctas = khq::sm_count();
-    w.record_floats = d == 256 ? decode::Shape<256>::RECORD : decode::Shape<128>::RECORD;
+    w.ctas = tile.decode ? khq::sm_count() : khq::sm_count() / 2 * 2;  // one per SM
+    w.record_floats = tile.decode ? (d == 256 ? decode::Shape<256>::RECORD : decode::Shape<128>::RECORD)
+                                  : (d == 256 ? tile::Shape<256>::RECORD : tile::Shape<128>::RECORD);
     w.bytes = (size_t)w.ctas * 16 + (size_t)2 * w.ctas * w.record_floats * 4;
     return w;
+}
+
+template <typename... Params_>
+cudaError_t launch_merge(void (*kernel)(Params_...), dim3 grid, cudaStream_t stream, Params_... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(128, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <int D, bool BF16>
@@ -212,16 +269,31 @@ int launch_decode(const khq_paged_attn_args& a, const Params& p, const Work& w, 
     if (rc != 0) return rc;
     err = khq::launch_pdl(decode::khq_paged_decode_kernel<D, BF16>, (unsigned)w.ctas, 0, (size_t)S::SMEM, stream, (unsigned)(decode::WARPS * 32), mk, mv, p);
     if (err != cudaSuccess) return static_cast<int>(err);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)w.ctas, 4, 1);
-    cfg.blockDim = dim3(128, 1, 1);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, khq_paged_merge_kernel<D, BF16>, p, DECODE_ROWS, w.record_floats, w.ctas));
+    return static_cast<int>(launch_merge(khq_paged_merge_kernel<D, BF16>, dim3((unsigned)w.ctas, 4, 1), stream, p, DECODE_ROWS, w.record_floats, w.ctas));
+}
+
+template <int D, bool BF16>
+int launch_tile(const khq_paged_attn_args& a, const Params& p, const Work& w, cudaStream_t stream) {
+    using S = tile::Shape<D>;
+    static bool attr_done[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    if (dev < 0 || dev >= 64) return -100;
+    if (!attr_done[dev]) {
+        err = cudaFuncSetAttribute((const void*)tile::khq_paged_tile_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (err != cudaSuccess) return static_cast<int>(err);
+        attr_done[dev] = true;
+    }
+    CUtensorMap mq, mk, mv;
+    int rc = query_map(&mq, a.q, a.q_stride, a.tokens, a.H_q, D, p.n_rep, tile::BR / p.n_rep, BF16);
+    if (rc == 0) rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, a.page_size < 64 ? a.page_size : 64, a.page_size < 64 ? 1 : S::G, BF16);
+    if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, a.page_size, a.page_size < 128 ? 1 : S::G / 2, BF16);
+    if (rc != 0) return rc;
+    err = khq::launch_pdl(tile::khq_paged_tile_kernel<D, BF16>, (unsigned)w.ctas, 2u, (size_t)S::SMEM, stream, (unsigned)tile::NTHREADS, mq, mk, mv, p);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    constexpr int parts = 16;
+    return static_cast<int>(launch_merge(tile::khq_paged_tile_merge_kernel<D, BF16>, dim3((unsigned)w.ctas / 2, 2 * parts, 1), stream, p, w.ctas / 2, parts));
 }
 
 bool heads_ok(int H_q, int H_kv) { return H_q > 0 && H_kv > 0 && H_q % H_kv == 0 && H_q / H_kv <= MAX_REP; }
@@ -230,7 +302,7 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     if (!args) return -100;
     const khq_paged_attn_args& a = *args;
     if (a.tokens <= 0 || a.max_tokens <= 0 || a.max_new <= 0 || a.requests <= 0 || a.max_pages <= 0 || a.n_pages <= 0 || a.H_q <= 0 || a.H_kv <= 0 || !a.q ||
-        !a.k_cache || !a.v_cache || !a.block_table || !a.cu_new || !a.kv_lens || !a.schedule || !a.out || !a.workspace)
+        !a.k_cache || !a.v_cache || !a.block_table || !a.schedule || !a.out || !a.workspace)
         return -100;
     if (!(a.scale > 0.0f) || !(a.scale <= 3.0e38f)) return -100;
     const int shift = a.page_size == 16 ? 4 : a.page_size == 32 ? 5 : a.page_size == 64 ? 6 : a.page_size == 128 ? 7 : -1;
@@ -238,7 +310,7 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     const void* ptrs[] = {a.q, a.gate, a.k_cache, a.v_cache, a.out, a.schedule};
     for (const void* x : ptrs)
         if ((reinterpret_cast<uintptr_t>(x) & 15) != 0) return -104;
-    const void* ints[] = {a.block_table, a.cu_new, a.kv_lens, a.lse};
+    const void* ints[] = {a.block_table, a.lse};
     for (const void* x : ints)
         if ((reinterpret_cast<uintptr_t>(x) & 3) != 0) return -104;
     if ((reinterpret_cast<uintptr_t>(a.workspace) & 255) != 0) return -104;
@@ -263,11 +335,9 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     p.o_hs = a.out_stride[1];
     p.table_stride = a.table_stride;
     p.table = static_cast<const int*>(a.block_table);
-    p.cu_new = static_cast<const int*>(a.cu_new);
-    p.kv_lens = static_cast<const int*>(a.kv_lens);
     p.schedule = static_cast<const int*>(a.schedule);
     p.items = reinterpret_cast<const Item*>(p.schedule + SCHED_HEADER);
-    p.cum = p.schedule + SCHED_HEADER + 4 * items;
+    p.cum = p.schedule + SCHED_HEADER + ITEM_INTS * items;
     p.meta = static_cast<int4*>(a.workspace);
     p.records = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + (size_t)w.ctas * 16);
     p.tokens = a.tokens;
@@ -279,8 +349,12 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     p.H_kv = a.H_kv;
     p.n_rep = a.H_q / a.H_kv;
     p.scale_log2e = a.scale * 1.4426950408889634f;
-    if (a.d == 256) return bf16 ? launch_decode<256, true>(a, p, w, stream) : launch_decode<256, false>(a, p, w, stream);
-    return bf16 ? launch_decode<128, true>(a, p, w, stream) : launch_decode<128, false>(a, p, w, stream);
+    if (tile.decode) {
+        if (a.d == 256) return bf16 ? launch_decode<256, true>(a, p, w, stream) : launch_decode<256, false>(a, p, w, stream);
+        return bf16 ? launch_decode<128, true>(a, p, w, stream) : launch_decode<128, false>(a, p, w, stream);
+    }
+    if (a.d == 256) return bf16 ? launch_tile<256, true>(a, p, w, stream) : launch_tile<256, false>(a, p, w, stream);
+    return bf16 ? launch_tile<128, true>(a, p, w, stream) : launch_tile<128, false>(a, p, w, stream);
 }
 
 }  // namespace

@@ -153,7 +153,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
         }
         // (after a wait that ran out the warp goes on without data, so that the others are not left at a barrier; the status word tells)
-        ok = ok && __all_sync(0xFFFFFFFFu, khq::mbar_wait_bounded(&bar[s], phase, status));
+        ok = ok && __all_sync(0xFFFFFFFFu, wait_for(&bar[s], phase, status));
         const int key0 = cur.blk * DECODE_KEYS + warp * UNIT;
         if (ok && !((missing >> s) & 1u)) {
             const uint32_t base = ring + s * S::STAGE_BYTES;
@@ -313,7 +313,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     }
     // nothing this warp started may still be in flight when the CTA leaves
     if (!ok && lane == 0)
-        for (int i = max(0, issued - S::STAGES); i < issued; ++i) khq::mbar_wait_bounded(&bar[i % S::STAGES], (uint32_t)((i / S::STAGES) & 1), status);
+        for (int i = max(0, issued - S::STAGES); i < issued; ++i) wait_for(&bar[i % S::STAGES], (uint32_t)((i / S::STAGES) & 1), status);
 }
 
 }  // namespace decode

@@ -28,7 +28,7 @@ from .lib import KhqLaunchError, check
 # the structs of include/khq_b200.h, field by field ("@": native alignment)
 _PLAN_ARGS = struct.Struct("@12PNq8i0q")
 _PRESTEP_ARGS = struct.Struct("@11P17q7i2f0q")
-_ATTN_ARGS = struct.Struct("@11P2N12qq10if0q")
+_ATTN_ARGS = struct.Struct("@9P2N12qq10if0q")
 _TYPES = {torch.float16: "fp16", torch.bfloat16: "bf16"}
 
 
@@ -215,7 +215,7 @@ def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scal
     if workspace is None:
         workspace = plan.workspace
     ws = _ints(workspace, "workspace", None, dev, torch.uint8)
-    packed = _ATTN_ARGS.pack(qp, gp, kc, vc, block_table.data_ptr(), plan._own[0], plan._own[1], plan._own[5], op, lp, ws, plan.schedule.numel(),
+    packed = _ATTN_ARGS.pack(qp, gp, kc, vc, block_table.data_ptr(), plan._own[5], op, lp, ws, plan.schedule.numel(),
                              workspace.numel(), q0, q1, g0, g1, o0, o1, kc0, kc1, kc2, vc0, vc1, vc2,
                              block_table.stride(0) if plan.requests > 1 else plan.max_pages, T, plan.max_tokens, plan.max_new, plan.requests, plan.max_pages,
                              n_pages, P, H_q, H_kv, d, float(scale))

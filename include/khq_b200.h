@@ -360,7 +360,7 @@ int launch_khq_engine_step(khq_engine* engine, const khq_engine_layer* layers, c
  * The exact attention of a chunk needs the raw K and V of the chunks before it.  They stand in pages of 16, 32, 64 or 128 tokens,
  * shared by all requests of a server, until the prompt is complete and its pages are compressed
  * (launch_khq_compress_batched_fp16 takes a page of a token-major cache as a run).  A step is: one plan for all layers, then per
- * layer the pre-step and the attention.  Shapes: d 128 or 256, H_q a multiple of H_kv, at most 16 query heads per kv head.
+ * layer the pre-step and the attention.  Shapes: d 128 or 256, H_q a multiple of H_kv, at most 128 query heads per kv head.
  *
  * The plan.  ctx_lens (requests): tokens that a request has in the cache; new_lens (requests): tokens that the step adds, -1: the
  * request has ended (its pages go back), both int32.  block_table (requests, table_stride) int32: page numbers, max_pages of a row in
@@ -407,13 +407,13 @@ int launch_khq_paged_prestep_bf16(const khq_paged_prestep_args* args, khq_stream
  *   out[t,h,:] = softmax_u(q[t,h] . K[u,h / n_rep] * scale) V[u,h / n_rep] * sigmoid(gate[t,h,:])      (gate NULL: without)
  * and, unless lse is NULL, lse[t,h] = log sum_u exp(q . K * scale) (tokens, H_q) fp32.  Softmax statistics, weights' sums and outputs in fp32;
  * the weights enter the product with V as 16-bit values.  A row that attends nothing (no page of it could be had) gets out 0 and lse
- * -inf.  Stale cache rows behind a request's last token are not attended, whatever they hold, NaN included.  cu_new, kv_lens and
- * schedule are a plan's, max_tokens, max_new, requests, page_size and the head counts the same as there; `tokens` rows of q, gate,
+ * -inf.  Stale cache rows behind a request's last token are not attended, whatever they hold, NaN included.  schedule is
+ * a plan's, max_tokens, max_new, requests, page_size and the head counts the same as there; `tokens` rows of q, gate,
  * out and lse exist (the plan must not have more).  Page numbers outside 0..n_pages-1 are not attended.  Rows behind the plan's last are left alone.
  * scale > 0.  workspace: khq_b200_paged_workspace_bytes(...) at 256 bytes; calls that may run at the same time need their own.  Returns -100, -103,
  * -104, -105, -107 / -108 (no tensor map). */
 typedef struct khq_paged_attn_args {
-    const void *q, *gate, *k_cache, *v_cache, *block_table, *cu_new, *kv_lens, *schedule;
+    const void *q, *gate, *k_cache, *v_cache, *block_table, *schedule;
     void *out, *lse, *workspace;
     size_t schedule_bytes, workspace_bytes;
     int64_t q_stride[2], gate_stride[2], out_stride[2];                      /* token, head */

@@ -23,7 +23,7 @@ PLAN = [("ctx_lens", P), ("new_lens", P), ("block_table", P), ("free_list", P), 
 PRESTEP = ([(n, P) for n in ("q", "k", "v", "q_norm_w", "k_norm_w", "q_out", "k_cache", "v_cache", "u_cache", "positions", "slots")]
            + [(n, 256) for n in ("q0", "q1", "k0", "k1", "v0", "v1", "o0", "o1", "kc0", "kc1", "kc2", "vc0", "vc1", "vc2", "uc0", "uc1", "uc2")]
            + [("tokens", 5), ("n_pages", 4), ("page_size", 16), ("H_q", 24), ("H_kv", 4), ("d", 256), ("rotary_dim", 64), ("rope_theta", 1e7), ("rms_eps", 1e-6)])
-ATTN = ([(n, P) for n in ("q", "gate", "k_cache", "v_cache", "block_table", "cu_new", "kv_lens", "schedule", "out", "lse", "workspace")]
+ATTN = ([(n, P) for n in ("q", "gate", "k_cache", "v_cache", "block_table", "schedule", "out", "lse", "workspace")]
         + [("schedule_bytes", 1 << 40), ("workspace_bytes", 1 << 40)]
         + [(n, 256) for n in ("q0", "q1", "g0", "g1", "o0", "o1", "kc0", "kc1", "kc2", "vc0", "vc1", "vc2")]
         + [("table_stride", 9), ("tokens", 5), ("max_tokens", 64), ("max_new", 64), ("requests", 3), ("max_pages", 9), ("n_pages", 40), ("page_size", 16),
