@@ -28,8 +28,8 @@ struct PlanArgs {
     int *free_count_out, *cu_new, *kv_lens, *positions;
     long long* slots;
     int *info, *schedule;
-    int requests, max_pages, n_pages, page_shift, max_tokens, max_new, tile_tokens, tile_keys;
-    long long item_cap;
+    int requests, max_pages, n_pages, page_shift, max_tokens, max_new;
+    Schedule sched;
 };
 
 // Inclusive sums of two ints over the block.  `part`: 2 x 32 ints.
@@ -141,24 +141,32 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         const int i = stack - 1 - j;
         return i < 0 ? -1 : i < count ? a.free_list[i] : given_back(i - count);
     };
-    if (rank == 0) {
-        // ---- sums, and the items of the attention --------------------------------------------------
-        int drop = dropped, unused = 0, total_drop, u;
-        block_scan2(drop, unused, part, total_drop, u);
-        if (tid == 0) {
-            a.cu_new[B] = sum_tok;
-            a.info[0] = sum_tok;
-            a.info[1] = min(sum_taken, stack);
-            a.info[2] = sum_back;
-            a.info[3] = max(sum_taken - stack, 0);
-            a.info[4] = total_drop;
+    if (rank < 2) {
+        // ---- the items of the attention: the first CTA the chunks', the second the decodes'; and the sums ----
+        const bool decodes = rank == 1;
+        const int tile_tokens = decodes ? a.sched.decode_tokens : a.sched.tile_tokens, tile_keys = decodes ? DECODE_KEYS : TILE_KEYS;
+        int u;
+        if (rank == 0) {
+            int drop = dropped, unused = 0, total_drop;
+            block_scan2(drop, unused, part, total_drop, u);
+            if (tid == 0) {
+                a.cu_new[B] = sum_tok;
+                a.info[0] = sum_tok;
+                a.info[1] = min(sum_taken, stack);
+                a.info[2] = sum_back;
+                a.info[3] = max(sum_taken - stack, 0);
+                a.info[4] = total_drop;
+            }
         }
-        // the first sums are not needed any more once all threads are here: items per request
+        // the pages' sums are not needed here: in their place the items'
         int items = 0;
         for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
             const int b = b0 + tid;
             int n = 0, z = 0, total;
-            if (b < B) n = (cu[b + 1] - cu[b] + a.tile_tokens - 1) / a.tile_tokens;
+            if (b < B) {
+                const int kept = cu[b + 1] - cu[b];
+                if (kept > 0 && (kept <= a.sched.decode_tokens) == decodes) n = (kept + tile_tokens - 1) / tile_tokens;
+            }
             const int mine = n;
             block_scan2(n, z, part, total, u);
             if (b < B) taken[b] = items + n - mine;
@@ -166,17 +174,17 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         }
         if (tid == 0) taken[B] = items;
         __syncthreads();
-        Item* const list = reinterpret_cast<Item*>(a.schedule + SCHED_HEADER);
-        int* const cum = a.schedule + SCHED_HEADER + ITEM_INTS * a.item_cap;
+        Item* const list = reinterpret_cast<Item*>(a.schedule + (decodes ? a.sched.decode_items : a.sched.chunk_items));
+        int* const cum = a.schedule + (decodes ? a.sched.decode_cum : a.sched.chunk_cum);
         int blocks = 0;
         for (int i0 = 0; i0 < items; i0 += PLAN_THREADS) {
             const int i = i0 + tid;
             Item it = {};
             if (i < items) {
                 it.b = find(taken, B, i);
-                const int q0 = (i - taken[it.b]) * a.tile_tokens, kept = cu[it.b + 1] - cu[it.b], ctx = ctx_of(it.b);
-                it.ntok = min(a.tile_tokens, kept - q0);
-                it.n_blocks = (ctx + q0 + it.ntok + a.tile_keys - 1) / a.tile_keys;
+                const int q0 = (i - taken[it.b]) * tile_tokens, kept = cu[it.b + 1] - cu[it.b], ctx = ctx_of(it.b);
+                it.ntok = min(tile_tokens, kept - q0);
+                it.n_blocks = (ctx + q0 + it.ntok + tile_keys - 1) / tile_keys;
                 it.kv = ctx + kept;
                 it.row0 = cu[it.b] + q0;
                 it.pos0 = ctx + q0;
@@ -191,12 +199,12 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         }
         if (tid == 0) {
             cum[items] = blocks;
-            a.schedule[0] = items;
-            a.schedule[1] = blocks;
+            a.schedule[2 * rank] = items;
+            a.schedule[2 * rank + 1] = blocks;
         }
     } else {
         // ---- table entries, the free list, positions and slots --------------------------------------
-        const int at = (rank - 1) * PLAN_THREADS + tid, step = (PLAN_CTAS - 1) * PLAN_THREADS;
+        const int at = (rank - 2) * PLAN_THREADS + tid, step = (PLAN_CTAS - 2) * PLAN_THREADS;
         for (int j = at; j < sum_taken; j += step) {
             const int b = find(taken, B, j);
             a.table[b * a.table_stride + pages(ctx_of(b)) + (j - taken[b])] = nth_taken(j);
@@ -377,7 +385,7 @@ int launch_prestep(const khq_paged_prestep_args* args, bool bf16, cudaStream_t s
 extern "C" size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, int H_q, int H_kv) {
     using namespace khq_paged;
     if (requests <= 0 || max_tokens <= 0 || max_new <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || H_q / H_kv > MAX_REP) return 0;
-    return (size_t)schedule_ints(max_items(requests, max_tokens, tile_of(H_q, H_kv, max_new).tokens)) * 4;
+    return (size_t)schedule_of(requests, max_tokens, max_new, H_q, H_kv).ints * 4;
 }
 
 extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream_t stream) {
@@ -396,11 +404,11 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
     for (const void* q : ptrs)
         if ((reinterpret_cast<uintptr_t>(q) & 3) != 0) return -104;
     if ((reinterpret_cast<uintptr_t>(p.slots) & 7) != 0 || (reinterpret_cast<uintptr_t>(p.schedule) & 15) != 0) return -104;
-    const Tile tile = tile_of(p.H_q, p.H_kv, p.max_new);
-    const long long items = max_items(p.requests, p.max_tokens, tile.tokens);
-    if (p.schedule_bytes < (size_t)schedule_ints(items) * 4) return -105;
+    const Schedule sched = schedule_of(p.requests, p.max_tokens, p.max_new, p.H_q, p.H_kv);
+    if (p.schedule_bytes < (size_t)sched.ints * 4) return -105;
     // the key blocks of all items are counted in 32 bits
-    if (items * ((((long long)p.max_pages << shift) + p.max_tokens) / tile.keys + 1) > 0x7FFFFFFFLL) return -103;
+    const long long row = ((long long)p.max_pages << shift) + p.max_tokens;
+    if (sched.chunk_cap * (row / TILE_KEYS + 1) > 0x7FFFFFFFLL || sched.decode_cap * (row / DECODE_KEYS + 1) > 0x7FFFFFFFLL) return -103;
     PlanArgs a;
     a.ctx_lens = static_cast<const int*>(p.ctx_lens);
     a.new_lens = static_cast<const int*>(p.new_lens);
@@ -421,9 +429,7 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
     a.page_shift = shift;
     a.max_tokens = p.max_tokens;
     a.max_new = p.max_new;
-    a.tile_tokens = tile.tokens;
-    a.tile_keys = tile.keys;
-    a.item_cap = items;
+    a.sched = sched;
     const size_t smem = (size_t)3 * (p.requests + 1) * 4;
     static bool attr_done[64] = {};
     int dev = 0;

@@ -4,30 +4,42 @@
 
 namespace khq_paged {
 
-// The schedule in device memory: a header of 16 ints, the items (one per request and query tile, request by request), and the
-// items' first key blocks counted through (cum[n_items] = the total).  The attention runs over H_kv copies of that list, one kv
-// head after the other.
-constexpr int SCHED_HEADER = 16;  // ints: [0] items, [1] key blocks of one kv head
+// The schedule in device memory: a header of 16 ints, then for the chunk kernel and for the decode kernel a list of items (in the order
+// of the requests) and the items' first key blocks counted through (cum[n_items] = the total).  Each kernel runs over H_kv copies of its
+// list, one kv head after the other.
+constexpr int SCHED_HEADER = 16;  // ints: [0] items, [1] key blocks of one kv head, for the chunk kernel; [2], [3] for the decode kernel
 struct alignas(16) Item {
     int b, n_blocks, ntok, kv;  // request; key blocks (causal: up to the tile's last token); new tokens of the tile; the request's tokens
     int row0, pos0, pad[2];     // the tile's first row in the ragged tensors, that row's position
 };
 constexpr int ITEM_INTS = sizeof(Item) / 4;
 
-// Query rows are (new token, query head of the kv head) pairs, token-major.  Up to 16 rows a request: the decode kernel, whose tile is
-// a request's rows.  Above: tiles of 2 x 128 rows on a CTA pair.
+// Query rows are (new token, query head of the kv head) pairs, token-major.  A request with up to 16 rows goes to the decode kernel, whose
+// tile is the request's rows (the cache's bytes bound those, and a pair's 256 rows would be all but empty); one with more is cut
+// into tiles of 2 x 128 rows, each for a CTA pair.
 constexpr int MAX_REP = 128;  // query heads of a kv head
 constexpr int DECODE_ROWS = 16, DECODE_KEYS = 64, TILE_ROWS = 128, TILE_KEYS = 128;
-struct Tile {
-    int tokens, keys;  // new tokens of a query tile, keys of a block
-    bool decode;
+struct Schedule {
+    bool chunks, decodes;             // the lists that the step can have
+    int tile_tokens, decode_tokens;   // new tokens of a tile; the most of a request for the decode kernel (0: none)
+    long long chunk_cap, decode_cap;  // items at most
+    long long chunk_items, chunk_cum, decode_items, decode_cum, ints;  // offsets in ints
 };
-inline Tile tile_of(int H_q, int H_kv, int max_new) {
+inline Schedule schedule_of(int requests, int max_tokens, int max_new, int H_q, int H_kv) {
     const int n_rep = H_q / H_kv;
-    if ((long long)max_new * n_rep <= DECODE_ROWS) return Tile{DECODE_ROWS / n_rep, DECODE_KEYS, true};
-    return Tile{2 * (TILE_ROWS / n_rep), TILE_KEYS, false};
+    Schedule s;
+    s.tile_tokens = 2 * (TILE_ROWS / n_rep);
+    s.decode_tokens = DECODE_ROWS / n_rep;
+    s.chunks = max_new > s.decode_tokens;
+    s.decodes = s.decode_tokens > 0;
+    s.chunk_cap = s.chunks ? (long long)max_tokens / s.tile_tokens + requests : 0;
+    s.decode_cap = s.decodes ? requests : 0;
+    s.chunk_items = SCHED_HEADER;
+    s.decode_items = s.chunk_items + ITEM_INTS * s.chunk_cap;
+    s.chunk_cum = s.decode_items + ITEM_INTS * s.decode_cap;
+    s.decode_cum = s.chunk_cum + s.chunk_cap + 1;
+    s.ints = s.decode_cum + s.decode_cap + 1;
+    return s;
 }
-inline long long max_items(int requests, int max_tokens, int tile_tokens) { return (long long)max_tokens / tile_tokens + requests; }
-inline long long schedule_ints(long long items) { return SCHED_HEADER + ITEM_INTS * items + items + 1; }
 
 }  // namespace khq_paged

@@ -54,8 +54,8 @@ struct Params {
     const Item* items;
     const int* cum;
     float* records;
-    int4* meta;  // by CTA: CTAs that share the segment which begins in it and goes on (0: none), item, kv head
-    int tokens, max_pages, n_pages, page_shift, page_mask, H_q, H_kv, n_rep;
+    int4* meta;  // by worker (CTA or pair): records of the segment which begins in it and goes on (0: none), item, kv head, first block
+    int tokens, max_pages, n_pages, page_shift, page_mask, H_q, H_kv, n_rep, rep_mul;  // x / n_rep = x * rep_mul >> 16 for x < 128
     float scale_log2e;
 };
 
@@ -117,10 +117,27 @@ __device__ __forceinline__ void store_out(const Params& p, int row, int head, in
     *reinterpret_cast<uint2*>(p.out + row * p.o_ts + head * p.o_hs + c) = make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
 }
 
-// Joins the records of the segment that begins in CTA blockIdx.x of the attention and goes on in the next ones; rows blockIdx.y, + gridDim.y, ..
-// A CTA's record 1 is of the segment that begins in it, record 0 of one that it took over.
+// Who shares a segment of blocks [seg_lo, seg_hi) that begins with worker `first`: the workers whose stretch has blocks of it.  (With fewer blocks than workers some
+// have none.)
+__device__ __forceinline__ int4 shared_segment(long long seg_lo, long long seg_hi, long long total, int first, int workers, int item, int h) {
+    const int last = (int)((seg_hi * workers - 1) / total);
+    return make_int4(total >= workers ? last - first + 1 : (int)(seg_hi - seg_lo), item, h, total >= workers ? -1 : (int)seg_lo);
+}
+// The worker of the segment's i-th record.
+__device__ __forceinline__ int record_worker(const int4& meta, int first, int i, long long total, int workers) {
+    return meta.w < 0 ? first + i : (int)(((meta.w + i + 1LL) * workers - 1) / total);
+}
+
+// Joins the records of the segment that begins in CTA blockIdx.x of the decode kernel and goes on in the next ones; rows blockIdx.y, + gridDim.y, ..
+// A CTA's record 1 is of the segment that begins in it, record 0 of one that it took over.  Groups of D / 4 threads take the records in
+// turn, 4 columns a thread.
+constexpr int MERGE_THREADS = 256, MAX_WORKERS = 256;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) khq_paged_merge_kernel(const Params p, int rows, int record_floats, int ctas) {
+__global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Params p, int record_floats, int workers) {
+    constexpr int PER_ROW = D / 4, GROUPS = MERGE_THREADS / PER_ROW;
+    __shared__ float factor[MAX_WORKERS];
+    __shared__ int base[MAX_WORKERS];
+    __shared__ float4 sums[GROUPS][PER_ROW];
     khq::pdl_wait();
     khq::pdl_trigger();
     const int4 meta = p.meta[blockIdx.x];
@@ -128,38 +145,58 @@ __global__ void __launch_bounds__(128) khq_paged_merge_kernel(const Params p, in
     Segment seg;
     seg.item = meta.y;
     load_segment(p, seg);
-    const int R = seg.ntok * p.n_rep, row0 = seg.row0;
-    constexpr int PER_ROW = D / 4;  // threads a row
-    const int c = (threadIdx.x % PER_ROW) * 4;
-    const long long total = (long long)p.schedule[1] * p.H_kv;
-    const auto empty = [&](int cta) { return cta * total / ctas == (cta + 1) * total / ctas; };
-    for (int r = blockIdx.y * (128 / PER_ROW) + threadIdx.x / PER_ROW; r < R; r += gridDim.y * (128 / PER_ROW)) {
-        float M = -INFINITY;
-        for (int i = 0; i < meta.x; ++i) {
-            const int cta = blockIdx.x + i;
-            if (empty(cta)) continue;
-            M = fmaxf(M, p.records[(2LL * cta + (i == 0)) * record_floats + rows * D + 2 * r]);
+    const int R = seg.ntok * p.n_rep, n = meta.x, tid = threadIdx.x, lane = tid & 31;
+    const long long total = (long long)p.schedule[3] * p.H_kv;
+    for (int i = tid; i < n; i += MERGE_THREADS) base[i] = 2 * record_worker(meta, blockIdx.x, i, total, workers) + (i == 0);
+    const int col = tid % PER_ROW, group = tid / PER_ROW;
+    for (int r = blockIdx.y; r < R; r += gridDim.y) {
+        __syncthreads();
+        // every warp for itself: the row's maximum, its sum, and each record's factor
+        float2 ml[MAX_WORKERS / 32];
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < MAX_WORKERS / 32; ++k) {
+            const int i = k * 32 + lane;
+            ml[k] = make_float2(-INFINITY, 0.0f);
+            if (i < n) ml[k] = *reinterpret_cast<const float2*>(p.records + (long long)base[i] * record_floats + DECODE_ROWS * D + 2 * r);
+            M = fmaxf(M, ml[k].x);
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+#pragma unroll
+        for (int k = 0; k < MAX_WORKERS / 32; ++k) {
+            const int i = k * 32 + lane;
+            const float f = ml[k].x == -INFINITY ? 0.0f : exp2f(ml[k].x - M);
+            L += ml[k].y * f;
+            if (tid < 32 && i < n) factor[i] = f;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
+        __syncthreads();
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float L = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < meta.x; ++i) {
-            const int cta = blockIdx.x + i;
-            if (empty(cta)) continue;
-            const float* rec = p.records + (2LL * cta + (i == 0)) * record_floats;
-            const float2 ml = *reinterpret_cast<const float2*>(rec + rows * D + 2 * r);
-            const float4 a = *reinterpret_cast<const float4*>(rec + r * D + c);
-            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-            L += ml.y * f;
+#pragma unroll 8
+        for (int i = group; i < n; i += GROUPS) {
+            const float4 a = *reinterpret_cast<const float4*>(p.records + (long long)base[i] * record_floats + r * D + col * 4);
+            const float f = factor[i];
             acc.x += a.x * f;
             acc.y += a.y * f;
             acc.z += a.z * f;
             acc.w += a.w * f;
         }
-        const int row = row0 + r / p.n_rep, head = meta.z * p.n_rep + r % p.n_rep;
-        if (row >= p.tokens) continue;
-        store_out<BF16>(p, row, head, c, acc, L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L);
-        if (p.lse && c == 0) p.lse[(long long)row * p.H_q + head] = (M + log2f(L)) * 0.6931471805599453f;
+        sums[group][col] = acc;
+        __syncthreads();
+        const int row = seg.row0 + r / p.n_rep, head = meta.z * p.n_rep + r % p.n_rep;
+        if (group != 0 || row >= p.tokens) continue;
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g) {
+            const float4 a = sums[g][col];
+            acc.x += a.x;
+            acc.y += a.y;
+            acc.z += a.z;
+            acc.w += a.w;
+        }
+        store_out<BF16>(p, row, head, col * 4, acc, L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L);
+        if (p.lse && col == 0) p.lse[(long long)row * p.H_q + head] = (M + log2f(L)) * 0.6931471805599453f;
     }
 }
 
@@ -222,25 +259,28 @@ int query_map(CUtensorMap* map, const void* base, const int64_t (&stride)[2], in
     return r == CUDA_SUCCESS ? 0 : -108;
 }
 
-// The workspace: a line of `meta` and two records per CTA.
+// The workspace: for each kernel that the step can have a line of `meta` and two records per CTA.
 struct Work {
-    int ctas, record_floats;
-    size_t bytes;
+    int ctas, pairs;
+    size_t decode_meta, decode_records, chunk_meta, chunk_records, bytes;
 };
-Work work_of(const Tile& tile, int d) {
+Work work_of(const Schedule& sched, int d) {
     Work w;
-    w.ctas = tile.decode ? khq::sm_count() : khq::sm_count() / 2 * 2;  // one per SM
-    w.record_floats = tile.decode ? (d == 256 ? decode::Shape<256>::RECORD : decode::Shape<128>::RECORD)
-                                  : (d == 256 ? tile::Shape<256>::RECORD : tile::Shape<128>::RECORD);
-    w.bytes = (size_t)w.ctas * 16 + (size_t)2 * w.ctas * w.record_floats * 4;
+    w.ctas = khq::sm_count() < MAX_WORKERS ? khq::sm_count() : MAX_WORKERS;  // one per SM
+    w.pairs = w.ctas / 2;
+    w.decode_meta = 0;
+    w.decode_records = w.decode_meta + (size_t)w.ctas * 16;
+    w.chunk_meta = w.decode_records + (sched.decodes ? (size_t)2 * w.ctas * (d == 256 ? decode::Shape<256>::RECORD : decode::Shape<128>::RECORD) * 4 : 0);
+    w.chunk_records = w.chunk_meta + (sched.chunks ? (size_t)w.pairs * 16 : 0);
+    w.bytes = w.chunk_records + (sched.chunks ? (size_t)4 * w.pairs * (d == 256 ? tile::Shape<256>::RECORD : tile::Shape<128>::RECORD) * 4 : 0);
     return w;
 }
 
 template <typename... Params_>
-cudaError_t launch_merge(void (*kernel)(Params_...), dim3 grid, cudaStream_t stream, Params_... args) {
+cudaError_t launch_merge(void (*kernel)(Params_...), dim3 grid, unsigned threads, cudaStream_t stream, Params_... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(128, 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -250,50 +290,67 @@ cudaError_t launch_merge(void (*kernel)(Params_...), dim3 grid, cudaStream_t str
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Both kernels' shared memory, once per device.
 template <int D, bool BF16>
-int launch_decode(const khq_paged_attn_args& a, const Params& p, const Work& w, cudaStream_t stream) {
-    using S = decode::Shape<D>;
+int prepare_kernels() {
     static bool attr_done[64] = {};
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return static_cast<int>(err);
     if (dev < 0 || dev >= 64) return -100;
-    if (!attr_done[dev]) {
-        err = cudaFuncSetAttribute((const void*)decode::khq_paged_decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-        if (err != cudaSuccess) return static_cast<int>(err);
-        attr_done[dev] = true;
-    }
-    CUtensorMap mk, mv;
-    int rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
-    if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
-    if (rc != 0) return rc;
-    err = khq::launch_pdl(decode::khq_paged_decode_kernel<D, BF16>, (unsigned)w.ctas, 0, (size_t)S::SMEM, stream, (unsigned)(decode::WARPS * 32), mk, mv, p);
+    if (attr_done[dev]) return 0;
+    err = cudaFuncSetAttribute((const void*)decode::khq_paged_decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, decode::Shape<D>::SMEM);
+    if (err == cudaSuccess)
+        err = cudaFuncSetAttribute((const void*)tile::khq_paged_tile_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile::Shape<D>::SMEM);
     if (err != cudaSuccess) return static_cast<int>(err);
-    return static_cast<int>(launch_merge(khq_paged_merge_kernel<D, BF16>, dim3((unsigned)w.ctas, 4, 1), stream, p, DECODE_ROWS, w.record_floats, w.ctas));
+    attr_done[dev] = true;
+    return 0;
 }
 
 template <int D, bool BF16>
-int launch_tile(const khq_paged_attn_args& a, const Params& p, const Work& w, cudaStream_t stream) {
-    using S = tile::Shape<D>;
-    static bool attr_done[64] = {};
-    int dev = 0;
-    cudaError_t err = cudaGetDevice(&dev);
-    if (err != cudaSuccess) return static_cast<int>(err);
-    if (dev < 0 || dev >= 64) return -100;
-    if (!attr_done[dev]) {
-        err = cudaFuncSetAttribute((const void*)tile::khq_paged_tile_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+int launch_kernels(const khq_paged_attn_args& a, Params p, const Schedule& sched, const Work& w, cudaStream_t stream) {
+    int rc = prepare_kernels<D, BF16>();
+    unsigned char* const ws = static_cast<unsigned char*>(a.workspace);
+    const auto of_kernel = [&](long long items, long long cum, size_t meta, size_t records) {
+        p.items = reinterpret_cast<const Item*>(p.schedule + items);
+        p.cum = p.schedule + cum;
+        p.meta = reinterpret_cast<int4*>(ws + meta);
+        p.records = reinterpret_cast<float*>(ws + records);
+    };
+    cudaError_t err;
+    if (sched.chunks) {
+        using S = tile::Shape<D>;
+        of_kernel(sched.chunk_items, sched.chunk_cum, w.chunk_meta, w.chunk_records);
+        CUtensorMap mq, mk, mv;
+        if (rc == 0) rc = query_map(&mq, a.q, a.q_stride, a.tokens, a.H_q, D, p.n_rep, tile::BR / p.n_rep, BF16);
+        if (rc == 0)
+            rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, a.page_size < 64 ? a.page_size : 64, a.page_size < 64 ? 1 : S::G, BF16);
+        if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, a.page_size, a.page_size < 128 ? 1 : S::G / 2, BF16);
+        if (rc != 0) return rc;
+        err = khq::launch_pdl(tile::khq_paged_tile_kernel<D, BF16>, (unsigned)(2 * w.pairs), 2u, (size_t)S::SMEM, stream, (unsigned)tile::NTHREADS, mq, mk, mv, p);
         if (err != cudaSuccess) return static_cast<int>(err);
-        attr_done[dev] = true;
     }
-    CUtensorMap mq, mk, mv;
-    int rc = query_map(&mq, a.q, a.q_stride, a.tokens, a.H_q, D, p.n_rep, tile::BR / p.n_rep, BF16);
-    if (rc == 0) rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, a.page_size < 64 ? a.page_size : 64, a.page_size < 64 ? 1 : S::G, BF16);
-    if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, a.page_size, a.page_size < 128 ? 1 : S::G / 2, BF16);
-    if (rc != 0) return rc;
-    err = khq::launch_pdl(tile::khq_paged_tile_kernel<D, BF16>, (unsigned)w.ctas, 2u, (size_t)S::SMEM, stream, (unsigned)tile::NTHREADS, mq, mk, mv, p);
-    if (err != cudaSuccess) return static_cast<int>(err);
-    constexpr int parts = 16;
-    return static_cast<int>(launch_merge(tile::khq_paged_tile_merge_kernel<D, BF16>, dim3((unsigned)w.ctas / 2, 2 * parts, 1), stream, p, w.ctas / 2, parts));
+    const Params chunk = p;
+    if (sched.decodes) {
+        of_kernel(sched.decode_items, sched.decode_cum, w.decode_meta, w.decode_records);
+        CUtensorMap mk, mv;
+        if (rc == 0) rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
+        if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
+        if (rc != 0) return rc;
+        err = khq::launch_pdl(decode::khq_paged_decode_kernel<D, BF16>, (unsigned)w.ctas, 0, (size_t)decode::Shape<D>::SMEM, stream,
+                              (unsigned)(decode::WARPS * 32), mk, mv, p, (int)sched.chunks);
+        if (err != cudaSuccess) return static_cast<int>(err);
+    }
+    if (sched.chunks) {
+        constexpr int parts = 16;
+        err = launch_merge(tile::khq_paged_tile_merge_kernel<D, BF16>, dim3((unsigned)w.pairs, 2 * parts, 1), tile::BR, stream, chunk, w.pairs, parts);
+        if (err != cudaSuccess) return static_cast<int>(err);
+    }
+    if (sched.decodes) {
+        err = launch_merge(khq_paged_merge_kernel<D, BF16>, dim3((unsigned)w.ctas, 4, 1), MERGE_THREADS, stream, p, (int)decode::Shape<D>::RECORD, w.ctas);
+        if (err != cudaSuccess) return static_cast<int>(err);
+    }
+    return 0;
 }
 
 bool heads_ok(int H_q, int H_kv) { return H_q > 0 && H_kv > 0 && H_q % H_kv == 0 && H_q / H_kv <= MAX_REP; }
@@ -318,10 +375,9 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
         if (((a.q_stride[i] | (a.gate ? a.gate_stride[i] : 0) | a.out_stride[i]) & 7) != 0) return -104;
     for (int i = 0; i < 3; ++i)
         if (((a.k_cache_stride[i] | a.v_cache_stride[i]) & 7) != 0 || a.k_cache_stride[i] < 0 || a.v_cache_stride[i] < 0) return -104;
-    const Tile tile = tile_of(a.H_q, a.H_kv, a.max_new);
-    const long long items = max_items(a.requests, a.max_tokens, tile.tokens);
-    const Work w = work_of(tile, a.d);
-    if (a.schedule_bytes < (size_t)schedule_ints(items) * 4 || a.workspace_bytes < w.bytes) return -105;
+    const Schedule sched = schedule_of(a.requests, a.max_tokens, a.max_new, a.H_q, a.H_kv);
+    const Work w = work_of(sched, a.d);
+    if (a.schedule_bytes < (size_t)sched.ints * 4 || a.workspace_bytes < w.bytes) return -105;
     Params p;
     p.q = static_cast<const uint16_t*>(a.q);
     p.gate = static_cast<const uint16_t*>(a.gate);
@@ -336,10 +392,6 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     p.table_stride = a.table_stride;
     p.table = static_cast<const int*>(a.block_table);
     p.schedule = static_cast<const int*>(a.schedule);
-    p.items = reinterpret_cast<const Item*>(p.schedule + SCHED_HEADER);
-    p.cum = p.schedule + SCHED_HEADER + ITEM_INTS * items;
-    p.meta = static_cast<int4*>(a.workspace);
-    p.records = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + (size_t)w.ctas * 16);
     p.tokens = a.tokens;
     p.max_pages = a.max_pages;
     p.n_pages = a.n_pages;
@@ -348,20 +400,17 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     p.H_q = a.H_q;
     p.H_kv = a.H_kv;
     p.n_rep = a.H_q / a.H_kv;
+    p.rep_mul = 65536 / p.n_rep + 1;
     p.scale_log2e = a.scale * 1.4426950408889634f;
-    if (tile.decode) {
-        if (a.d == 256) return bf16 ? launch_decode<256, true>(a, p, w, stream) : launch_decode<256, false>(a, p, w, stream);
-        return bf16 ? launch_decode<128, true>(a, p, w, stream) : launch_decode<128, false>(a, p, w, stream);
-    }
-    if (a.d == 256) return bf16 ? launch_tile<256, true>(a, p, w, stream) : launch_tile<256, false>(a, p, w, stream);
-    return bf16 ? launch_tile<128, true>(a, p, w, stream) : launch_tile<128, false>(a, p, w, stream);
+    if (a.d == 256) return bf16 ? launch_kernels<256, true>(a, p, sched, w, stream) : launch_kernels<256, false>(a, p, sched, w, stream);
+    return bf16 ? launch_kernels<128, true>(a, p, sched, w, stream) : launch_kernels<128, false>(a, p, sched, w, stream);
 }
 
 }  // namespace
 
 extern "C" size_t khq_b200_paged_workspace_bytes(int max_new, int H_q, int H_kv, int d) {
     if (max_new <= 0 || !heads_ok(H_q, H_kv) || (d != 128 && d != 256)) return 0;
-    return (work_of(tile_of(H_q, H_kv, max_new), d).bytes + 255) / 256 * 256;
+    return (work_of(schedule_of(1, 1, max_new, H_q, H_kv), d).bytes + 255) / 256 * 256;
 }
 
 extern "C" int launch_khq_paged_attn_fp16(const khq_paged_attn_args* args, khq_stream_t stream) { return launch_attn(args, false, stream); }

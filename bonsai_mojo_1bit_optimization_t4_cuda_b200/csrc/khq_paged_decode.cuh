@@ -44,7 +44,7 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t at, uint32_t (&r)[4]) {
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(WARPS * 32, 1)
-khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
+khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p, int beside) {
     using S = Shape<D>;
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BARS);
@@ -52,6 +52,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     int* const status = &g_paged_status;
     if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled layout needs a 1024-byte aligned base
         if (tid == 0) atomicExch(status, 2);
+        khq::pdl_wait();
         return;
     }
     if (lane == 0) {
@@ -59,15 +60,21 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         khq::fence_barrier_init();
     }
     __syncthreads();
-    khq::pdl_wait();
+    // Behind the chunk kernel of the same step (`beside`) there is nothing to wait for: that one lets this one start once everything before
+    // both is complete, and they share no row.  So these CTAs come in as the pairs run out of work.  The end waits instead, or the
+    // kernel behind could start before the chunk kernel is complete.
+    if (!beside) khq::pdl_wait();
     khq::pdl_trigger();
 
     // ---- this CTA's stretch of the key blocks ------------------------------------------------------
-    const int n_items = p.schedule[0];
-    const long long per_head = p.schedule[1], total = per_head * p.H_kv;
+    const int n_items = p.schedule[2];
+    const long long per_head = p.schedule[3], total = per_head * p.H_kv;
     const long long lo = blockIdx.x * total / gridDim.x, hi = (blockIdx.x + 1) * total / gridDim.x;
     if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);  // overwritten below if a segment goes on in the next CTA
-    if (lo >= hi) return;
+    if (lo >= hi) {
+        if (beside) khq::pdl_wait();
+        return;
+    }
     Segment in, cur;  // where the loads and where the products are
     find_segment(p, n_items, per_head, lo, in);
     cur = in;
@@ -305,7 +312,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 __syncthreads();
             }
             if (tid == 0 && seg_lo >= lo && seg_hi > hi)
-                p.meta[blockIdx.x] = make_int4((int)((seg_hi * gridDim.x - 1) / total) - (int)blockIdx.x + 1, cur.item, cur.h, 0);
+                p.meta[blockIdx.x] = shared_segment(seg_lo, seg_hi, total, blockIdx.x, gridDim.x, cur.item, cur.h);
             fresh = true;
         }
         ++cur.blk;
@@ -314,6 +321,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     // nothing this warp started may still be in flight when the CTA leaves
     if (!ok && lane == 0)
         for (int i = max(0, issued - S::STAGES); i < issued; ++i) wait_for(&bar[i % S::STAGES], (uint32_t)((i / S::STAGES) & 1), status);
+    if (beside) khq::pdl_wait();
 }
 
 }  // namespace decode

@@ -26,18 +26,21 @@ constexpr int NSOFT = 256, NTHREADS = NSOFT + 96;
 constexpr uint32_t TM_COLS = 512, TM_S = 256;  // O from column 0
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr int STG_BYTES = 32 * 64;           // per softmax warp: 32 rows x 32 columns
-enum Bar {  // K, V, S and P V by block parity
-    B_KFULL = 0, B_VFULL = 2, B_SFULL = 4, B_PVDONE = 6, B_PREADY = 8 /* [parity][half of the keys] */, B_QFULL = 12, B_QFREE = 13, B_PEER = 14,
-    B_MREF = 15 /* [group][lane quarter] */, B_LSUM = 23 /* [lane quarter] */, B_OFREE = 27, B_VLAND = 28, B_COUNT = 29
+constexpr int MAX_STAGES = 4;
+enum Bar {  // K and V by stage, S and P V by block parity
+    B_KFULL = 0, B_KFREE = 4, B_VFULL = 8, B_VFREE = 12, B_SFULL = 16, B_PVDONE = 18, B_PREADY = 20 /* [parity][half of the keys] */, B_QFULL = 24, B_QFREE = 25,
+    B_PEER = 26, B_MREF = 27 /* [group][lane quarter] */, B_LSUM = 35 /* [lane quarter] */, B_OFREE = 39, B_VLAND = 40, B_COUNT = 41
 };
 template <int D> struct Shape {
     static constexpr int G = D / 64;               // column groups
+    // K and V blocks in flight: what fits.  Few query rows leave the cache's latency and bytes as the bound.
+    static constexpr int STAGES = D == 256 ? 2 : 4;
     static constexpr int Q_BYTES = BR * D * 2, TILE_BYTES = 64 * D * 2;  // a CTA's rows; its share of a K or V block
-    static constexpr int OFF_Q = 0, OFF_K = OFF_Q + Q_BYTES, OFF_V = OFF_K + 2 * TILE_BYTES, OFF_STG = OFF_V + 2 * TILE_BYTES;
+    static constexpr int OFF_Q = 0, OFF_K = OFF_Q + Q_BYTES, OFF_V = OFF_K + STAGES * TILE_BYTES, OFF_STG = OFF_V + STAGES * TILE_BYTES;
     static constexpr int OFF_MREF = OFF_STG + 8 * STG_BYTES;  // float [2 groups][128 rows]: the reference behind the group's last block
     static constexpr int OFF_LSUM = OFF_MREF + 2 * 128 * 4;   // float [segment parity][2 groups][128 rows]
     static constexpr int OFF_BARS = OFF_LSUM + 4 * 128 * 4, OFF_SLOT = OFF_BARS + B_COUNT * 8, SMEM = OFF_SLOT + 16;
-    static_assert(SMEM <= 227 * 1024, "shared memory");
+    static_assert(STAGES <= MAX_STAGES && SMEM <= 227 * 1024, "shared memory");
     // A CTA's record: its rows [4 columns][128 rows][4 floats], so that a thread per row writes whole lines, then (maximum, sum) by row.
     static constexpr int RECORD = BR * D + 2 * BR;
 };
@@ -127,9 +130,13 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     }
     const int tok = BR / p.n_rep, rows = tok * p.n_rep;  // new tokens and query rows of a CTA
     if (tid == 0) {
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < S::STAGES; ++s) {
             khq::mbar_init(&bars[B_KFULL + s], 1);
+            khq::mbar_init(&bars[B_KFREE + s], 1);
             khq::mbar_init(&bars[B_VFULL + s], 2);  // the V producers of both CTAs
+            khq::mbar_init(&bars[B_VFREE + s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
             khq::mbar_init(&bars[B_SFULL + s], 1);
             khq::mbar_init(&bars[B_PVDONE + s], 1);
         }
@@ -198,12 +205,12 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             }
             pages.begin(p, walk.s, walk.s.blk, log_per);
             for (int j = 0; j < walk.n; ++j, ++g) {
-                const int s = g & 1, blk = walk.s.blk + j;
+                const int s = g % S::STAGES, blk = walk.s.blk + j;
                 const int at = pages.seek(p, walk.s, blk, log_per);
                 // the page of this lane's box: keys rank * 64 + (lane / groups) pages further
                 const int mine = p.page_shift >= 6 ? at + ((rank * 64) >> p.page_shift) : at + rank * per_half + lane / S::G;
                 const int page = __shfl_sync(0xFFFFFFFFu, pages.now, mine & 31);
-                if (g >= 2 && !(ok = tile::warp_wait(&bars[B_SFULL + s], (uint32_t)(((g >> 1) - 1) & 1), status))) break;
+                if (g >= S::STAGES && !(ok = tile::warp_wait(&bars[B_KFREE + s], (uint32_t)((g / S::STAGES - 1) & 1), status))) break;
                 if (rank == 0 && lane == 0) khq::mbar_arrive_expect_tx(&bars[B_KFULL + s], 2 * S::TILE_BYTES);
                 __syncwarp();
                 if (lane < boxes) {
@@ -216,7 +223,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         }
         // nothing may still be in flight when the pair leaves: the first CTA waits for the loads of both
         if (!ok && rank == 0 && lane == 0)
-            for (int k = max(0, g - 2); k < g; ++k) wait_for(&bars[B_KFULL + (k & 1)], (uint32_t)((k >> 1) & 1), status);
+            for (int k = max(0, g - S::STAGES); k < g; ++k) wait_for(&bars[B_KFULL + k % S::STAGES], (uint32_t)((k / S::STAGES) & 1), status);
     } else if (warp == 10) {
         // ================================ producer of V: the CTA's d / 2 head dims as [group][128 keys][128 B] ======================
         constexpr int VG = S::G / 2;
@@ -227,10 +234,10 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         for (bool more = walk.begin(p, n_items, per_head); ok && more; more = walk.step(p, n_items)) {
             pages.begin(p, walk.s, walk.s.blk, log_per);
             for (int j = 0; j < walk.n; ++j, ++g) {
-                const int s = g & 1, blk = walk.s.blk + j, key0 = blk * BC;
+                const int s = g % S::STAGES, blk = walk.s.blk + j, key0 = blk * BC;
                 const int at = pages.seek(p, walk.s, blk, log_per);
                 const int page = __shfl_sync(0xFFFFFFFFu, pages.now, (log_per == 0 ? at : at + lane / VG) & 31);
-                if (g >= 2 && !(ok = tile::warp_wait(&bars[B_PVDONE + s], (uint32_t)(((g >> 1) - 1) & 1), status))) break;
+                if (g >= S::STAGES && !(ok = tile::warp_wait(&bars[B_VFREE + s], (uint32_t)((g / S::STAGES - 1) & 1), status))) break;
                 const bool tail = key0 + BC > walk.s.kv && (walk.s.kv & p.page_mask) != 0;
                 if (lane == 0) {
                     if (tail) khq::mbar_arrive_expect_tx(&bars[B_VLAND], S::TILE_BYTES);
@@ -280,10 +287,11 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             // S[g & 1] = Q K^T of block g; the tests are of block g - 1's weights and V
             const auto issue_qk = [&](int g, bool test) {
                 const uint32_t s_tmem = tmem + TM_S + (uint32_t)(g & 1) * BC;
-                need(k_of == g ? k_there : 0u, &bars[B_KFULL + (g & 1)], (uint32_t)((g >> 1) & 1));
+                const int ks_at = g % S::STAGES;
+                need(k_of == g ? k_there : 0u, &bars[B_KFULL + ks_at], (uint32_t)((g / S::STAGES) & 1));
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t k_at = k_lo + (uint32_t)(g & 1) * (S::TILE_BYTES >> 4);
+                const uint32_t k_at = k_lo + (uint32_t)ks_at * (S::TILE_BYTES >> 4);
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     // byte offsets / 16: next 64-dim group = rows * 128 bytes, next K step = 32 bytes
@@ -293,10 +301,11 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     else umma2_ss<1>(one, s_tmem, q_lo + oa, HI, k_at + ob, HI, IDESC_S);
                     if (ks == D / 16 - 5 && test) {
                         p_there = mbar_test(&bars[B_PREADY + 2 * ((g - 1) & 1)], (uint32_t)(((g - 1) >> 1) & 1));
-                        v_there = mbar_test(&bars[B_VFULL + ((g - 1) & 1)], (uint32_t)(((g - 1) >> 1) & 1));
+                        v_there = mbar_test(&bars[B_VFULL + (g - 1) % S::STAGES], (uint32_t)(((g - 1) / S::STAGES) & 1));
                     }
                 }
                 umma2_commit(one, &bars[B_SFULL + (g & 1)]);
+                umma2_commit(one, &bars[B_KFREE + ks_at]);
             };
             int g = 0, i = 0;
             bool more = walk.begin(p, n_items, per_head);
@@ -308,8 +317,8 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 if (!ok) break;
                 if (walk.n == 1) umma2_commit(one, &bars[B_QFREE]);
                 for (int j = 0; j < walk.n; ++j, ++g) {
-                    const int s = g & 1;
-                    const uint32_t par = (uint32_t)((g >> 1) & 1);
+                    const int s = g & 1, vs = g % S::STAGES;
+                    const uint32_t par = (uint32_t)((g >> 1) & 1), v_par = (uint32_t)((g / S::STAGES) & 1);
                     p_there = v_there = 0;
                     if (j + 1 < walk.n) {
                         issue_qk(g + 1, true);
@@ -319,15 +328,15 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     need(p_there, &bars[B_PREADY + 2 * s], par);
                     if ((walk.s.blk + j + 1) * BC > walk.s.kv) {
                         // zeros that the other CTA's V producer may have stored
-                        if (ok) ok = warp_wait_cluster(&bars[B_VFULL + s], par, status);
+                        if (ok) ok = warp_wait_cluster(&bars[B_VFULL + vs], v_par, status);
                     } else {
-                        need(v_there, &bars[B_VFULL + s], par);
+                        need(v_there, &bars[B_VFULL + vs], v_par);
                     }
                     // the first P V of a segment overwrites O: the one before has been read
                     if (j == 0 && i > 0 && ok) ok = tile::warp_wait(&bars[B_OFREE], (uint32_t)((i - 1) & 1), status);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t v_at = v_lo + (uint32_t)s * (S::TILE_BYTES >> 4), p_tmem = tmem + TM_S + (uint32_t)s * BC;
+                    const uint32_t v_at = v_lo + (uint32_t)vs * (S::TILE_BYTES >> 4), p_tmem = tmem + TM_S + (uint32_t)s * BC;
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
                         if (kk == 4) {  // the other half of the keys: its weights come while the first half is multiplied
@@ -338,12 +347,13 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                         umma2_ts(one, tmem, p_tmem + kk * 8, v_at + ((uint32_t)(kk * 2048) >> 4), HI, IDESC_O, kk > 0 ? 1u : (uint32_t)(j > 0));  // 16 keys = 2048 bytes
                         if (kk == 1) p_there = mbar_test(&bars[B_PREADY + 2 * s + 1], par);
                         if (kk == 5) {
-                            k_there = mbar_test(&bars[B_KFULL + s], (uint32_t)(((g + 2) >> 1) & 1));
+                            k_there = mbar_test(&bars[B_KFULL + (g + 2) % S::STAGES], (uint32_t)(((g + 2) / S::STAGES) & 1));
                             k_of = g + 2;
                         }
                     }
                     if (!ok) break;
                     umma2_commit(one, &bars[B_PVDONE + s]);
+                    umma2_commit(one, &bars[B_VFREE + vs]);
                 }
             }
         }
@@ -353,12 +363,12 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         // half the columns of O in the epilogue).  The groups' reference maxima follow one another through shared memory, warp by
         // warp: the two warps of a lane quarter have the same rows.
         const uint32_t tmem = *tmem_slot;
-        const int grp = warp >> 2, quarter = warp & 3, r = tid & 127, t_row = r / p.n_rep;
+        const int grp = warp >> 2, quarter = warp & 3, r = tid & 127, t_row = (r * p.rep_mul) >> 16;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
         unsigned char* const stage = smem + S::OFF_STG + warp * STG_BYTES;
         bool ok = true;
         int g0 = 0, i = 0;  // running index of the segment's first block; segments
-        if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);  // overwritten below if a segment goes on in the next pair
+        if (tid == 0 && rank == 0) p.meta[blockIdx.x >> 1] = make_int4(0, 0, 0, 0);  // overwritten below if a segment goes on in the next pair
         for (bool more = walk.begin(p, n_items, per_head); ok && more; more = walk.step(p, n_items), ++i) {
             const Segment& sg = walk.s;
             const int pos = min(sg.pos0 + rank * tok + t_row, sg.kv - 1);  // keys 0..pos
@@ -460,6 +470,22 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             if (!ok) break;
             // ---- epilogue of the segment ----------------------------------------------------------------
             const bool whole = sg.blk == 0 && walk.n == sg.n_blocks;
+            const int n_tok = min(sg.ntok - rank * tok, tok);  // of this CTA, may be 0 or less
+            const int row0 = sg.row0 + rank * tok;
+            // Gates and outputs, 32 columns at a time, pass through the warp's own piece of shared memory: a thread owns a row, so its global
+            // accesses would take a line each; this way four lanes take a row's 64 bytes.  All gates are on their way before the last waits.
+            constexpr int PIECES = D / 64;  // of a group's half of the columns
+            uint4 gates[PIECES][4];
+            if (whole && p.gate) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int R = quarter * 32 + e * 8 + (lane >> 2), t = (R * p.rep_mul) >> 16;
+                    const bool live = t < n_tok && row0 + t < p.tokens;
+                    const uint16_t* from = p.gate + (live ? (row0 + t) * p.g_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.g_hs : 0) + grp * (D / 2) + (lane & 3) * 8;
+#pragma unroll
+                    for (int c = 0; c < PIECES; ++c) gates[c][e] = live ? __ldg(reinterpret_cast<const uint4*>(from + c * 32)) : make_uint4(0, 0, 0, 0);
+                }
+            }
             // the last block's reference, then both groups' sums against it
             if (grp != (last & 1))
                 ok = wait_for(&bars[B_MREF + 4 * (last & 1) + quarter], (uint32_t)((last >> 1) & 1), status);
@@ -476,29 +502,24 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             tc_fence_after();
-            const int n_tok = min(sg.ntok - rank * tok, tok);  // of this CTA, may be 0 or less
-            const int row0 = sg.row0 + rank * tok;
             if (whole) {
-                // 32 columns at a time through the warp's own piece of shared memory: a thread owns a row, so its global accesses would take a
-                // line each; this way four lanes take a row's 64 bytes
                 const float inv = l_run > 0.0f ? 1.0f / l_run : l_run == 0.0f ? 0.0f : l_run;  // a NaN stays one
                 const auto spot = [&](int row, int chunk) { return reinterpret_cast<uint4*>(stage + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); };
-#pragma unroll 1
-                for (int c0 = grp * (D / 2); c0 < (grp + 1) * (D / 2); c0 += 32) {
+#pragma unroll
+                for (int c = 0; c < PIECES; ++c) {
                     uint32_t o[32];
-                    tmem_ld32(lane_base + c0, o);
+                    tmem_ld32(lane_base + grp * (D / 2) + c * 32, o);
                     if (p.gate) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int rr = e * 8 + (lane >> 2), R = quarter * 32 + rr, t = R / p.n_rep;
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (t < n_tok && row0 + t < p.tokens)
-                                v = __ldg(reinterpret_cast<const uint4*>(p.gate + (row0 + t) * p.g_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.g_hs + c0 + (lane & 3) * 8));
-                            *spot(rr, lane & 3) = v;
-                        }
+                        for (int e = 0; e < 4; ++e) *spot(e * 8 + (lane >> 2), lane & 3) = gates[c][e];
                         __syncwarp();
                     }
                     tmem_ld_wait();
+                    if (c == PIECES - 1) {  // O has been read: the next segment's first P V may overwrite it
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive_leader(&bars[B_OFREE]);
+                    }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         uint4* const at = spot(lane, q);
@@ -520,9 +541,10 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     __syncwarp();
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int rr = e * 8 + (lane >> 2), R = quarter * 32 + rr, t = R / p.n_rep;
+                        const int rr = e * 8 + (lane >> 2), R = quarter * 32 + rr, t = (R * p.rep_mul) >> 16;
                         if (t < n_tok && row0 + t < p.tokens)
-                            *reinterpret_cast<uint4*>(p.out + (row0 + t) * p.o_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.o_hs + c0 + (lane & 3) * 8) = *spot(rr, lane & 3);
+                            *reinterpret_cast<uint4*>(p.out + (row0 + t) * p.o_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.o_hs + grp * (D / 2) + c * 32 + (lane & 3) * 8) =
+                                *spot(rr, lane & 3);
                     }
                     __syncwarp();
                 }
@@ -544,15 +566,12 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     __syncwarp();
                 }
                 if (grp == 0 && t_row < n_tok) *reinterpret_cast<float2*>(rec + BR * D + 2 * r) = make_float2(m_end, l_run);
-                if (tid == 0 && sg.blk == 0) {  // it goes on in the next pairs
-                    const long long total = per_head * p.H_kv, seg_hi = walk.w + sg.n_blocks, pairs = gridDim.x >> 1;
-                    p.meta[blockIdx.x] = make_int4((int)((seg_hi * pairs - 1) / total) - (int)(blockIdx.x >> 1) + 1, sg.item, sg.h, 0);
-                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&bars[B_OFREE]);
+                if (tid == 0 && rank == 0 && sg.blk == 0)  // it goes on in the next pairs
+                    p.meta[blockIdx.x >> 1] = shared_segment(walk.w, walk.w + sg.n_blocks, per_head * p.H_kv, (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1), sg.item, sg.h);
             }
-            // O has been read: the next segment's first P V may overwrite it
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_leader(&bars[B_OFREE]);
             g0 = last + 1;
         }
     }
@@ -564,46 +583,57 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "n"(TM_COLS) : "memory");
 }
 
-// Joins the records of the segment that begins in pair blockIdx.x of the attention and goes on in the next ones.  A thread takes 4 columns of
-// a row; blockIdx.y: the CTA of the pair and a part of its columns.
+// Joins the records of the segment that begins in pair blockIdx.x of the chunk kernel and goes on in the next ones.  A thread takes a row;
+// blockIdx.y: the CTA of the pair and a part of its columns.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(BR) khq_paged_tile_merge_kernel(const Params p, int pairs, int parts) {
     using S = Shape<D>;
+    __shared__ int base[MAX_WORKERS];
     khq::pdl_wait();
     khq::pdl_trigger();
-    const int rank = blockIdx.y / parts, part = blockIdx.y % parts, r = threadIdx.x;
-    const int4 meta = p.meta[2 * blockIdx.x];  // the first CTA's; both have the same segments
+    const int4 meta = p.meta[blockIdx.x];
     if (meta.x == 0) return;
+    const int rank = blockIdx.y / parts, part = blockIdx.y % parts, r = threadIdx.x, n = meta.x;
     Segment s;
     s.item = meta.y;
     load_segment(p, s);
-    const int tok = BR / p.n_rep, t = r / p.n_rep, n_tok = min(s.ntok - rank * tok, tok), row = s.row0 + rank * tok + t;
-    if (t >= n_tok || row >= p.tokens) return;
+    const int tok = BR / p.n_rep, t = (r * p.rep_mul) >> 16, n_tok = min(s.ntok - rank * tok, tok), row = s.row0 + rank * tok + t;
+    if (n_tok <= 0) return;
     const long long total = (long long)p.schedule[1] * p.H_kv;
-    const auto empty = [&](int pair) { return pair * total / pairs == (pair + 1) * total / pairs; };
-    const auto record = [&](int i) { return p.records + (2LL * (2 * (blockIdx.x + i) + rank) + (i == 0)) * S::RECORD; };
+    // record 1 is of the segment that begins in a pair, record 0 of one that it took over
+    for (int i = r; i < n; i += BR) base[i] = 2 * (2 * record_worker(meta, blockIdx.x, i, total, pairs) + rank) + (i == 0);
+    __syncthreads();
+    if (t >= n_tok || row >= p.tokens) return;
     float M = -INFINITY;
-    for (int i = 0; i < meta.x; ++i)
-        if (!empty(blockIdx.x + i)) M = fmaxf(M, record(i)[BR * D + 2 * r]);
-    const int head = meta.z * p.n_rep + (r - t * p.n_rep);
-    for (int c4 = part * (D / 4 / parts); c4 < (part + 1) * (D / 4 / parts); ++c4) {
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float L = 0.0f;
-        for (int i = 0; i < meta.x; ++i) {
-            if (empty(blockIdx.x + i)) continue;
-            const float* rec = record(i);
-            const float2 ml = *reinterpret_cast<const float2*>(rec + BR * D + 2 * r);
-            const float4 a = reinterpret_cast<const float4*>(rec)[c4 * BR + r];
-            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-            L += ml.y * f;
-            acc.x += a.x * f;
-            acc.y += a.y * f;
-            acc.z += a.z * f;
-            acc.w += a.w * f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) M = fmaxf(M, p.records[(long long)base[i] * S::RECORD + BR * D + 2 * r]);
+    constexpr int COLS = D / 4 / 16;  // groups of 4 columns per part
+    float4 acc[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float L = 0.0f;
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
+        const float* rec = p.records + (long long)base[i] * S::RECORD;
+        const float2 ml = *reinterpret_cast<const float2*>(rec + BR * D + 2 * r);
+        float4 a[COLS];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) a[c] = reinterpret_cast<const float4*>(rec)[(part * COLS + c) * BR + r];
+        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+        L += ml.y * f;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            acc[c].x += a[c].x * f;
+            acc[c].y += a[c].y * f;
+            acc[c].z += a[c].z * f;
+            acc[c].w += a[c].w * f;
         }
-        store_out<BF16>(p, row, head, c4 * 4, acc, L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L);
-        if (p.lse && c4 == 0) p.lse[(long long)row * p.H_q + head] = (M + log2f(L)) * 0.6931471805599453f;
     }
+    const int head = meta.z * p.n_rep + (r - t * p.n_rep);
+    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) store_out<BF16>(p, row, head, (part * COLS + c) * 4, acc[c], inv);
+    if (p.lse && part == 0) p.lse[(long long)row * p.H_q + head] = (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace tile

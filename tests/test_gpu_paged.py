@@ -270,6 +270,28 @@ def test_attention_chunks(cuda_ops, dtype, ctx, new, H_q, H_kv, d, page):
     attend(dtype, H_q, H_kv, d, page, ctx, new, seed=len(ctx) + sum(new))
 
 
+@pytest.mark.parametrize("H_q,H_kv,d,page", [(32, 1, 128, 16), (128, 1, 128, 64), (48, 1, 256, 128), (100, 1, 256, 32), (34, 2, 128, 128)])
+@pytest.mark.parametrize("ctx,new", [([0, 200, 5], [1, 1, 1]), ([64, 0, 700], [9, 130, 2])])
+def test_attention_many_heads_of_a_kv_head(cuda_ops, H_q, H_kv, d, page, ctx, new):
+    attend("fp16", H_q, H_kv, d, page, ctx, new, seed=H_q)
+
+
+@pytest.mark.parametrize("H_q,H_kv,d,page", [(24, 4, 256, 64), (20, 4, 128, 16)])
+def test_attention_chunks_between_decodes(cuda_ops, H_q, H_kv, d, page):
+    """Both kernels in one call, either of them with little, much or nothing to do."""
+    rng = random.Random(3)
+    for ctx, new in (([500, 20, 3000, 0, 77], [1, 300, 1, 90, 2]), ([0, 64, 65], [1, 1, 200]), ([4000, 4000], [17, 1]), ([300] * 5, [2, 1, 2, 1, 1]),
+                     ([rng.randint(0, 900) for _ in range(120)], [rng.choice([0, 1, 1, 1, 2, 40]) for _ in range(120)])):
+        attend("bf16", H_q, H_kv, d, page, ctx, new, max_new=300, seed=len(ctx))
+
+
+def test_attention_long_contexts_shared(cuda_ops):
+    """Few requests over long contexts: every segment is shared by many CTAs."""
+    attend("fp16", 24, 4, 256, 128, [40000], [30], seed=1)
+    attend("bf16", 8, 1, 256, 16, [30011], [1], seed=2)
+    attend("fp16", 4, 1, 128, 16, [60000, 3], [50, 1], seed=3)
+
+
 def test_attention_many_requests(cuda_ops):
     rng = random.Random(8)
     ctx = [rng.choice([0, 1, 15, 16, 17, 100, 400]) for _ in range(400)]
