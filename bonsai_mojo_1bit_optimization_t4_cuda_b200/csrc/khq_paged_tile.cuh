@@ -22,7 +22,7 @@ namespace khq_paged {
 namespace tile {
 
 constexpr int BR = 128, BC = 128;            // query rows of a CTA, keys of a block
-constexpr int NSOFT = 256, NTHREADS = NSOFT + 96;
+constexpr int NSOFT = 256, NTHREADS = NSOFT + 128;  // warp 11 has no work: registers are split by groups of four warps
 constexpr uint32_t TM_COLS = 512, TM_S = 256;  // O from column 0
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr int STG_BYTES = 32 * 64;           // per softmax warp: 32 rows x 32 columns
@@ -104,11 +104,16 @@ struct Walk {
         return true;
     }
     __device__ __forceinline__ bool step(const Params& p, int n_items) {
-        w += n;
-        if (w >= hi) return false;
-        next_segment(p, n_items, s);
-        n = (int)min((long long)s.n_blocks, hi - w);
+        if (w + n >= hi) return false;
+        Segment next = s;
+        next_segment(p, n_items, next);
+        step_to(next);
         return true;
+    }
+    __device__ __forceinline__ void step_to(const Segment& next) {
+        w += n;
+        s = next;
+        n = (int)min((long long)s.n_blocks, hi - w);
     }
 };
 
@@ -175,7 +180,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     }
     tc_fence_before();
     // tensor memory is there; the loads do not wait for that
-    if (warp == 8 || warp == 10) asm volatile("bar.arrive 1, %0;" ::"n"(NTHREADS) : "memory");
+    if (warp == 8 || warp >= 10) asm volatile("bar.arrive 1, %0;" ::"n"(NTHREADS) : "memory");
     else asm volatile("bar.sync 1, %0;" ::"n"(NTHREADS) : "memory");
     tc_fence_after();
 
@@ -183,6 +188,10 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const long long per_head = p.schedule[1];
     const int log_per = 7 - p.page_shift;  // pages of a block
     Walk walk;
+    // 384 threads start with 168 registers each; the softmax threads, who hold 128 scores, take 208 and leave the others 88: together
+    // the same 64512.  (Behind a point where both come together the compiler counts on the smaller number.)
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8) {
         // ================================ producer of Q and K: the CTA's 64 keys of a block as [group][64 keys][128 B] =============
         // boxes: 64 keys x all groups, or page x one group
@@ -357,7 +366,9 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 }
             }
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ================================ softmax + epilogue ======================================
         // Group 0 (warps 0-3) has the even blocks, group 1 (warps 4-7) the odd ones; a thread owns a row (all 128 keys of its blocks, and
         // half the columns of O in the epilogue).  The groups' reference maxima follow one another through shared memory, warp by
@@ -369,24 +380,25 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         bool ok = true;
         int g0 = 0, i = 0;  // running index of the segment's first block; segments
         if (tid == 0 && rank == 0) p.meta[blockIdx.x >> 1] = make_int4(0, 0, 0, 0);  // overwritten below if a segment goes on in the next pair
-        for (bool more = walk.begin(p, n_items, per_head); ok && more; more = walk.step(p, n_items), ++i) {
+        // pages that are not there, of block `blk` of a segment: bit by page
+        const auto fetch_holes = [&](const Segment& sg, int blk) {
+            const int col = (blk << log_per) + lane;
+            int hole = 0;
+            if (lane < (1 << log_per) && (long long)col << p.page_shift < sg.kv)
+                hole = col >= p.max_pages || (unsigned)__ldg(p.table + sg.b * p.table_stride + (col < p.max_pages ? col : 0)) >= (unsigned)p.n_pages;
+            return hole;
+        };
+        bool more = walk.begin(p, n_items, per_head);
+        int hole_next = more && walk.n > grp ? fetch_holes(walk.s, walk.s.blk + grp) : 0;
+        for (; ok && more; ++i) {
             const Segment& sg = walk.s;
             const int pos = min(sg.pos0 + rank * tok + t_row, sg.kv - 1);  // keys 0..pos
             const int pos_min = sg.pos0 + rank * tok + (quarter * 32) / p.n_rep;
             const int last = g0 + walk.n - 1;
-            // pages that are not there, of this group's next block: bit by page
-            const auto fetch_holes = [&](int g) {
-                const int col = ((sg.blk + g - g0) << log_per) + lane;
-                int hole = 0;
-                if (lane < (1 << log_per) && g <= last && (long long)col << p.page_shift < sg.kv)
-                    hole = col >= p.max_pages || (unsigned)__ldg(p.table + sg.b * p.table_stride + (col < p.max_pages ? col : 0)) >= (unsigned)p.n_pages;
-                return hole;
-            };
             float m_l = -INFINITY, l_run = 0.0f;  // the sum of this group's blocks and the reference that it is against
-            int hole_next = fetch_holes(g0 + ((g0 ^ grp) & 1));
             for (int g = g0 + ((g0 ^ grp) & 1); g <= last; g += 2) {
                 const uint32_t holes = __ballot_sync(0xFFFFFFFFu, hole_next);
-                hole_next = fetch_holes(g + 2);
+                if (g + 2 <= last) hole_next = fetch_holes(sg, sg.blk + g + 2 - g0);
                 // the reference behind the block before, mostly there by now: ahead of the scores
                 float before = 0.0f;
                 if (g > g0) {
@@ -472,19 +484,22 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             const bool whole = sg.blk == 0 && walk.n == sg.n_blocks;
             const int n_tok = min(sg.ntok - rank * tok, tok);  // of this CTA, may be 0 or less
             const int row0 = sg.row0 + rank * tok;
+            // the next segment is on its way meanwhile
+            more = walk.w + walk.n < walk.hi;
+            Segment next = sg;
+            if (more) next_segment(p, n_items, next);
             // Gates and outputs, 32 columns at a time, pass through the warp's own piece of shared memory: a thread owns a row, so its global
-            // accesses would take a line each; this way four lanes take a row's 64 bytes.  All gates are on their way before the last waits.
-            constexpr int PIECES = D / 64;  // of a group's half of the columns
-            uint4 gates[PIECES][4];
-            if (whole && p.gate) {
+            // accesses would take a line each; this way four lanes take a row's 64 bytes.
+            const auto gate_at = [&](int e, int c) {
+                const int R = quarter * 32 + e * 8 + (lane >> 2), t = (R * p.rep_mul) >> 16;
+                if (t >= n_tok || row0 + t >= p.tokens) return make_uint4(0, 0, 0, 0);
+                return __ldg(reinterpret_cast<const uint4*>(p.gate + (row0 + t) * p.g_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.g_hs + grp * (D / 2) + c * 32 + (lane & 3) * 8));
+            };
+            const bool gated = whole && p.gate;
+            uint4 gates[4];
+            if (gated) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int R = quarter * 32 + e * 8 + (lane >> 2), t = (R * p.rep_mul) >> 16;
-                    const bool live = t < n_tok && row0 + t < p.tokens;
-                    const uint16_t* from = p.gate + (live ? (row0 + t) * p.g_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.g_hs : 0) + grp * (D / 2) + (lane & 3) * 8;
-#pragma unroll
-                    for (int c = 0; c < PIECES; ++c) gates[c][e] = live ? __ldg(reinterpret_cast<const uint4*>(from + c * 32)) : make_uint4(0, 0, 0, 0);
-                }
+                for (int e = 0; e < 4; ++e) gates[e] = gate_at(e, 0);
             }
             // the last block's reference, then both groups' sums against it
             if (grp != (last & 1))
@@ -505,17 +520,21 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             if (whole) {
                 const float inv = l_run > 0.0f ? 1.0f / l_run : l_run == 0.0f ? 0.0f : l_run;  // a NaN stays one
                 const auto spot = [&](int row, int chunk) { return reinterpret_cast<uint4*>(stage + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); };
-#pragma unroll
-                for (int c = 0; c < PIECES; ++c) {
+                // one copy of this code: the instructions come from far, once a segment
+#pragma unroll 1
+                for (int c = 0; c < D / 64; ++c) {
                     uint32_t o[32];
                     tmem_ld32(lane_base + grp * (D / 2) + c * 32, o);
-                    if (p.gate) {
+                    if (gated) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) *spot(e * 8 + (lane >> 2), lane & 3) = gates[c][e];
+                        for (int e = 0; e < 4; ++e) {
+                            *spot(e * 8 + (lane >> 2), lane & 3) = gates[e];
+                            if (c + 1 < D / 64) gates[e] = gate_at(e, c + 1);
+                        }
                         __syncwarp();
                     }
                     tmem_ld_wait();
-                    if (c == PIECES - 1) {  // O has been read: the next segment's first P V may overwrite it
+                    if (c == D / 64 - 1) {  // O has been read: the next segment's first P V may overwrite it
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) arrive_leader(&bars[B_OFREE]);
@@ -524,7 +543,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     for (int q = 0; q < 4; ++q) {
                         uint4* const at = spot(lane, q);
                         uint32_t w[4];
-                        if (p.gate) {
+                        if (gated) {
                             const uint4 gv = *at;
                             const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
 #pragma unroll
@@ -573,6 +592,11 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     p.meta[blockIdx.x >> 1] = shared_segment(walk.w, walk.w + sg.n_blocks, per_head * p.H_kv, (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1), sg.item, sg.h);
             }
             g0 = last + 1;
+            if (more) {
+                walk.step_to(next);
+                const int first = (g0 ^ grp) & 1;
+                if (walk.n > first) hole_next = fetch_holes(walk.s, walk.s.blk + first);
+            }
         }
     }
     // ---- teardown: every thread arrives here, with or without a failed wait ----------------------
