@@ -408,7 +408,7 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
     if (p.schedule_bytes < (size_t)sched.ints * 4) return -105;
     // the key blocks of all items are counted in 32 bits
     const long long row = ((long long)p.max_pages << shift) + p.max_tokens;
-    if (sched.chunk_cap * (row / TILE_KEYS + 1) > 0x7FFFFFFFLL || sched.decode_cap * (row / DECODE_KEYS + 1) > 0x7FFFFFFFLL) return -103;
+    if (sched.chunk_cap * (row / TILE_KEYS + 1 + CHUNK_OVER) > 0x7FFFFFFFLL || sched.decode_cap * (row / DECODE_KEYS + 1) > 0x7FFFFFFFLL) return -103;
     PlanArgs a;
     a.ctx_lens = static_cast<const int*>(p.ctx_lens);
     a.new_lens = static_cast<const int*>(p.new_lens);

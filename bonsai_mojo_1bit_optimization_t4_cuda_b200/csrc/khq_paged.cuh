@@ -19,6 +19,8 @@ constexpr int ITEM_INTS = sizeof(Item) / 4;
 // into tiles of 2 x 128 rows, each for a CTA pair.
 constexpr int MAX_REP = 128;  // query heads of a kv head
 constexpr int DECODE_ROWS = 16, DECODE_KEYS = 64, TILE_ROWS = 128, TILE_KEYS = 128;
+// What a tile costs beside its key blocks, in blocks: its queries, gates and outputs, and the pipe's run-in.
+constexpr int CHUNK_OVER = 3;
 struct Schedule {
     bool chunks, decodes;             // the lists that the step can have
     int tile_tokens, decode_tokens;   // new tokens of a tile; the most of a request for the decode kernel (0: none)

@@ -73,22 +73,25 @@ __device__ __forceinline__ void load_segment(const Params& p, Segment& s) {
     s.row0 = y.x;
     s.pos0 = y.y;
 }
-// Block w of the row of all blocks.  A warp bisects by 32.
-__device__ __forceinline__ void find_segment(const Params& p, int n_items, long long per_head, long long w, Segment& s) {
+// Block w of the row of all blocks, in which each item stands with `over` blocks in front of its own that stand for its fixed cost.  Returns
+// where the item begins in that row; s.blk: the block, 0 for those in front.  A warp bisects by 32.
+__device__ __forceinline__ long long find_segment(const Params& p, int n_items, long long per_head, int over, long long w, Segment& s) {
     const int lane = threadIdx.x & 31;
     s.h = (int)(w / per_head);
     const int r = (int)(w % per_head);
-    int lo = 0, n = n_items;  // the last item of [lo, lo + n) with cum <= r
+    int lo = 0, n = n_items;  // the last item of [lo, lo + n) that begins at r or in front
     while (n > 1) {
-        const int step = (n + 31) / 32, at = lo + lane * step;
-        const unsigned below = __ballot_sync(0xFFFFFFFFu, lane * step < n && __ldg(p.cum + (lane * step < n ? at : lo)) <= r);
+        const int step = (n + 31) / 32, at = lane * step < n ? lo + lane * step : lo;
+        const unsigned below = __ballot_sync(0xFFFFFFFFu, lane * step < n && __ldg(p.cum + at) + at * over <= r);
         const int last = 31 - __clz((int)(below | 1u));
         lo += last * step;
         n = min(step, n - last * step);
     }
     s.item = lo;
     load_segment(p, s);
-    s.blk = r - __ldg(p.cum + lo);
+    const int off = r - __ldg(p.cum + lo) - lo * over;
+    s.blk = max(off - over, 0);
+    return w - off;
 }
 // Every item has a key block at least (its own tokens).
 __device__ __forceinline__ void next_segment(const Params& p, int n_items, Segment& s) {

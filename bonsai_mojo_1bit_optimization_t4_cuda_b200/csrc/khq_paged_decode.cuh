@@ -76,7 +76,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         return;
     }
     Segment in, cur;  // where the loads and where the products are
-    find_segment(p, n_items, per_head, lo, in);
+    find_segment(p, n_items, per_head, 0, lo, in);
     cur = in;
     uint64_t* const bar = bars + warp * S::STAGES;
     const uint32_t ring = smem_u32(smem) + warp * S::STAGES * S::STAGE_BYTES;

@@ -89,31 +89,32 @@ struct Pages {
     }
 };
 
-// The pair's segments one after the other, as every role walks them.
+// The pair's segments one after the other, as every role walks them.  Positions count the CHUNK_OVER blocks in front of every item.
 struct Walk {
-    long long w, hi;  // the segment's first block, the stretch's end
-    int n;            // its blocks in this stretch
+    long long begins, hi;  // where the segment's item begins, the stretch's end
+    int n;                 // its blocks in this stretch
     Segment s;
     __device__ __forceinline__ bool begin(const Params& p, int n_items, long long per_head) {
-        const long long total = per_head * p.H_kv, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-        w = pair * total / pairs;
+        const long long total = per_head * p.H_kv, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, w = pair * total / pairs;
         hi = (pair + 1) * total / pairs;
         if (w >= hi) return false;
-        find_segment(p, n_items, per_head, w, s);
-        n = (int)min((long long)(s.n_blocks - s.blk), hi - w);
-        return true;
+        begins = find_segment(p, n_items, per_head, CHUNK_OVER, w, s);
+        count();
+        return n > 0;
+    }
+    __device__ __forceinline__ void count() { n = (int)min((long long)s.n_blocks, hi - begins - CHUNK_OVER) - s.blk; }
+    __device__ __forceinline__ bool more() const { return begins + s.n_blocks + 2 * CHUNK_OVER < hi; }
+    __device__ __forceinline__ void step_to(const Segment& next) {
+        begins += s.n_blocks + CHUNK_OVER;
+        s = next;
+        count();
     }
     __device__ __forceinline__ bool step(const Params& p, int n_items) {
-        if (w + n >= hi) return false;
+        if (!more()) return false;
         Segment next = s;
         next_segment(p, n_items, next);
         step_to(next);
         return true;
-    }
-    __device__ __forceinline__ void step_to(const Segment& next) {
-        w += n;
-        s = next;
-        n = (int)min((long long)s.n_blocks, hi - w);
     }
 };
 
@@ -185,7 +186,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     tc_fence_after();
 
     const int n_items = p.schedule[0];
-    const long long per_head = p.schedule[1];
+    const long long per_head = p.schedule[1] + (long long)n_items * CHUNK_OVER;
     const int log_per = 7 - p.page_shift;  // pages of a block
     Walk walk;
     // 384 threads start with 168 registers each; the softmax threads, who hold 128 scores, take 208 and leave the others 88: together
@@ -213,7 +214,14 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                         : "memory");
             }
             pages.begin(p, walk.s, walk.s.blk, log_per);
+            const bool ahead = walk.more();  // the next segment's queries to L2: their load waits for this one's last Q K^T
+            Segment next = walk.s;
+            if (ahead) next_segment(p, n_items, next);
             for (int j = 0; j < walk.n; ++j, ++g) {
+                if (j == 0 && ahead && lane < S::G)
+                    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(0),
+                                 "r"(next.h * p.n_rep), "r"(next.row0 + rank * tok), "r"(lane)
+                                 : "memory");
                 const int s = g % S::STAGES, blk = walk.s.blk + j;
                 const int at = pages.seek(p, walk.s, blk, log_per);
                 // the page of this lane's box: keys rank * 64 + (lane / groups) pages further
@@ -395,6 +403,14 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             const int pos = min(sg.pos0 + rank * tok + t_row, sg.kv - 1);  // keys 0..pos
             const int pos_min = sg.pos0 + rank * tok + (quarter * 32) / p.n_rep;
             const int last = g0 + walk.n - 1;
+            const bool whole = sg.blk == 0 && walk.n == sg.n_blocks, gated = whole && p.gate;
+            const int n_tok = min(sg.ntok - rank * tok, tok);  // of this CTA, may be 0 or less
+            const int row0 = sg.row0 + rank * tok;
+            if (gated && t_row < n_tok && row0 + t_row < p.tokens) {  // this row's gates to L2, until the epilogue
+                const uint16_t* at = p.gate + (row0 + t_row) * p.g_ts + (sg.h * p.n_rep + r - t_row * p.n_rep) * p.g_hs + grp * (D / 2);
+#pragma unroll
+                for (int c = 0; c < D / 2; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + c));
+            }
             float m_l = -INFINITY, l_run = 0.0f;  // the sum of this group's blocks and the reference that it is against
             for (int g = g0 + ((g0 ^ grp) & 1); g <= last; g += 2) {
                 const uint32_t holes = __ballot_sync(0xFFFFFFFFu, hole_next);
@@ -481,26 +497,27 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             }
             if (!ok) break;
             // ---- epilogue of the segment ----------------------------------------------------------------
-            const bool whole = sg.blk == 0 && walk.n == sg.n_blocks;
-            const int n_tok = min(sg.ntok - rank * tok, tok);  // of this CTA, may be 0 or less
-            const int row0 = sg.row0 + rank * tok;
             // the next segment is on its way meanwhile
-            more = walk.w + walk.n < walk.hi;
+            more = walk.more();
             Segment next = sg;
             if (more) next_segment(p, n_items, next);
             // Gates and outputs, 32 columns at a time, pass through the warp's own piece of shared memory: a thread owns a row, so its global
             // accesses would take a line each; this way four lanes take a row's 64 bytes.
-            const auto gate_at = [&](int e, int c) {
-                const int R = quarter * 32 + e * 8 + (lane >> 2), t = (R * p.rep_mul) >> 16;
-                if (t >= n_tok || row0 + t >= p.tokens) return make_uint4(0, 0, 0, 0);
-                return __ldg(reinterpret_cast<const uint4*>(p.gate + (row0 + t) * p.g_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.g_hs + grp * (D / 2) + c * 32 + (lane & 3) * 8));
-            };
-            const bool gated = whole && p.gate;
-            uint4 gates[4];
-            if (gated) {
+            long long q_row[4];  // of the four rows that this lane moves: offset of its 8 columns of the first piece in the gates, -1: none
+            long long o_row[4];  // and in the outputs
 #pragma unroll
-                for (int e = 0; e < 4; ++e) gates[e] = gate_at(e, 0);
+            for (int e = 0; e < 4; ++e) {
+                const int R = quarter * 32 + e * 8 + (lane >> 2), t = (R * p.rep_mul) >> 16, head = sg.h * p.n_rep + R - t * p.n_rep, c = grp * (D / 2) + (lane & 3) * 8;
+                const bool live = whole && t < n_tok && row0 + t < p.tokens;
+                q_row[e] = live && gated ? (row0 + t) * p.g_ts + head * p.g_hs + c : -1;
+                o_row[e] = live ? (row0 + t) * p.o_ts + head * p.o_hs + c : -1;
             }
+            const auto gate_at = [&](int e, int c) {
+                return q_row[e] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(p.gate + q_row[e] + c * 32));
+            };
+            uint4 gates[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) gates[e] = gate_at(e, 0);
             // the last block's reference, then both groups' sums against it
             if (grp != (last & 1))
                 ok = wait_for(&bars[B_MREF + 4 * (last & 1) + quarter], (uint32_t)((last >> 1) & 1), status);
@@ -517,6 +534,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             tc_fence_after();
+            if (more) hole_next = fetch_holes(next, ((last + 1) ^ grp) & 1);  // (a block past the segment's end: no key, no hole)
             if (whole) {
                 const float inv = l_run > 0.0f ? 1.0f / l_run : l_run == 0.0f ? 0.0f : l_run;  // a NaN stays one
                 const auto spot = [&](int row, int chunk) { return reinterpret_cast<uint4*>(stage + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); };
@@ -560,10 +578,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     __syncwarp();
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int rr = e * 8 + (lane >> 2), R = quarter * 32 + rr, t = (R * p.rep_mul) >> 16;
-                        if (t < n_tok && row0 + t < p.tokens)
-                            *reinterpret_cast<uint4*>(p.out + (row0 + t) * p.o_ts + (sg.h * p.n_rep + R - t * p.n_rep) * p.o_hs + grp * (D / 2) + c * 32 + (lane & 3) * 8) =
-                                *spot(rr, lane & 3);
+                        if (o_row[e] >= 0) *reinterpret_cast<uint4*>(p.out + o_row[e] + c * 32) = *spot(e * 8 + (lane >> 2), lane & 3);
                     }
                     __syncwarp();
                 }
@@ -589,14 +604,11 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 __syncwarp();
                 if (lane == 0) arrive_leader(&bars[B_OFREE]);
                 if (tid == 0 && rank == 0 && sg.blk == 0)  // it goes on in the next pairs
-                    p.meta[blockIdx.x >> 1] = shared_segment(walk.w, walk.w + sg.n_blocks, per_head * p.H_kv, (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1), sg.item, sg.h);
+                    p.meta[blockIdx.x >> 1] = shared_segment(walk.begins + CHUNK_OVER, walk.begins + CHUNK_OVER + sg.n_blocks, per_head * p.H_kv, (int)(blockIdx.x >> 1),
+                                                             (int)(gridDim.x >> 1), sg.item, sg.h);
             }
             g0 = last + 1;
-            if (more) {
-                walk.step_to(next);
-                const int first = (g0 ^ grp) & 1;
-                if (walk.n > first) hole_next = fetch_holes(walk.s, walk.s.blk + first);
-            }
+            if (more) walk.step_to(next);
         }
     }
     // ---- teardown: every thread arrives here, with or without a failed wait ----------------------
@@ -623,7 +635,7 @@ __global__ void __launch_bounds__(BR) khq_paged_tile_merge_kernel(const Params p
     load_segment(p, s);
     const int tok = BR / p.n_rep, t = (r * p.rep_mul) >> 16, n_tok = min(s.ntok - rank * tok, tok), row = s.row0 + rank * tok + t;
     if (n_tok <= 0) return;
-    const long long total = (long long)p.schedule[1] * p.H_kv;
+    const long long total = (p.schedule[1] + (long long)p.schedule[0] * CHUNK_OVER) * p.H_kv;
     // record 1 is of the segment that begins in a pair, record 0 of one that it took over
     for (int i = r; i < n; i += BR) base[i] = 2 * (2 * record_worker(meta, blockIdx.x, i, total, pairs) + rank) + (i == 0);
     __syncthreads();
