@@ -14,9 +14,11 @@ namespace khq_paged {
 
 // ---- the plan of a step --------------------------------------------------------------------------
 // One cluster.  Every CTA sums up the lengths of all requests for itself (8 bytes a request) and keeps three running sums in shared
-// memory: tokens, pages taken, pages given back.  From those any token and any moved page is found by bisection, so the CTAs need nothing from each
-// other: the pages of ended requests are read where they stand in their table rows, on top of the free ones.  Only the new
-// number of free pages waits (free_count_out may be free_count).
+// memory: tokens, pages taken, pages given back.  From those any moved page is found by bisection: the pages of ended requests are
+// read where they stand in their table rows, on top of the free ones.  Behind one barrier (the table is complete, the number of free pages has
+// been read and may be overwritten) two CTAs cut the step into the attention's items and its workers' stretches, and the others write
+// positions and slots.  Latency bounds it: a chain of some ten loads, scans and bisections (a bisection step in shared memory is 30 cycles,
+// in global memory some 500).
 constexpr int PLAN_THREADS = 1024, PLAN_CTAS = 8, PLAN_MAX_REQUESTS = 16384, PLAN_MAX_TOKENS = 1 << 20;
 
 struct PlanArgs {
@@ -28,7 +30,7 @@ struct PlanArgs {
     int *free_count_out, *cu_new, *kv_lens, *positions;
     long long* slots;
     int *info, *schedule;
-    int requests, max_pages, n_pages, page_shift, max_tokens, max_new;
+    int requests, max_pages, n_pages, page_shift, max_tokens, max_new, H_kv, workers, cum_in_smem;
     Schedule sched;
 };
 
@@ -141,25 +143,43 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         const int i = stack - 1 - j;
         return i < 0 ? -1 : i < count ? a.free_list[i] : given_back(i - count);
     };
-    if (rank < 2) {
-        // ---- the items of the attention: the first CTA the chunks', the second the decodes'; and the sums ----
-        const bool decodes = rank == 1;
-        const int tile_tokens = decodes ? a.sched.decode_tokens : a.sched.tile_tokens, tile_keys = decodes ? DECODE_KEYS : TILE_KEYS;
-        int u;
-        if (rank == 0) {
-            int drop = dropped, unused = 0, total_drop;
-            block_scan2(drop, unused, part, total_drop, u);
-            if (tid == 0) {
-                a.cu_new[B] = sum_tok;
-                a.info[0] = sum_tok;
-                a.info[1] = min(sum_taken, stack);
-                a.info[2] = sum_back;
-                a.info[3] = max(sum_taken - stack, 0);
-                a.info[4] = total_drop;
-            }
+    {
+        // ---- table entries and the free list ------------------------------------------------------------
+        const int at = rank * PLAN_THREADS + tid, step = PLAN_CTAS * PLAN_THREADS;
+        for (int j = at; j < sum_taken; j += step) {
+            const int b = find(taken, B, j);
+            a.table[b * a.table_stride + pages(ctx_of(b)) + (j - taken[b])] = nth_taken(j);
         }
-        // the pages' sums are not needed here: in their place the items'
-        int items = 0;
+        for (int r = at; r < sum_back; r += step)
+            if (count + r < a.n_pages) a.free_list[count + r] = given_back(r);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (rank == 0) {
+        int drop = dropped, unused = 0, total_drop, u;
+        block_scan2(drop, unused, part, total_drop, u);
+        if (tid == 0) {
+            a.cu_new[B] = sum_tok;
+            a.info[0] = sum_tok;
+            a.info[1] = min(sum_taken, stack);
+            a.info[2] = sum_back;
+            a.info[3] = max(sum_taken - stack, 0);
+            a.info[4] = total_drop;
+        }
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // the pages' sums have done their work: in their place the requests' lengths, and the items' sums
+    int *const ctx_lens = back, *const first_item = taken;
+    for (int b = tid; b < B; b += PLAN_THREADS) ctx_lens[b] = ctx_of(b);
+    if (rank < 2) {
+        // ---- the items of the attention: the first CTA the chunks', the second the decodes' ----------------
+        if (rank == 0 && tid == 0 && pool) {
+            const int left = max(stack - sum_taken, 0);
+            a.info[5] = left;
+            *a.free_count_out = left;
+        }
+        const bool decodes = rank == 1;
+        const int tile_tokens = decodes ? a.sched.decode_tokens : a.sched.tile_tokens, tile_keys = decodes ? a.sched.decode_keys : TILE_KEYS;
+        int items = 0, u;
         for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
             const int b = b0 + tid;
             int n = 0, z = 0, total;
@@ -169,20 +189,20 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
             }
             const int mine = n;
             block_scan2(n, z, part, total, u);
-            if (b < B) taken[b] = items + n - mine;
+            if (b < B) first_item[b] = items + n - mine;
             items += total;
         }
-        if (tid == 0) taken[B] = items;
+        if (tid == 0) first_item[B] = items;
         __syncthreads();
         Item* const list = reinterpret_cast<Item*>(a.schedule + (decodes ? a.sched.decode_items : a.sched.chunk_items));
-        int* const cum = a.schedule + (decodes ? a.sched.decode_cum : a.sched.chunk_cum);
+        int* const cum = a.cum_in_smem ? back + B + 1 : a.schedule + (decodes ? a.sched.decode_cum : a.sched.chunk_cum);
         int blocks = 0;
         for (int i0 = 0; i0 < items; i0 += PLAN_THREADS) {
             const int i = i0 + tid;
             Item it = {};
             if (i < items) {
-                it.b = find(taken, B, i);
-                const int q0 = (i - taken[it.b]) * tile_tokens, kept = cu[it.b + 1] - cu[it.b], ctx = ctx_of(it.b);
+                it.b = find(first_item, B, i);
+                const int q0 = (i - first_item[it.b]) * tile_tokens, kept = cu[it.b + 1] - cu[it.b], ctx = ctx_lens[it.b];
                 it.ntok = min(tile_tokens, kept - q0);
                 it.n_blocks = (ctx + q0 + it.ntok + tile_keys - 1) / tile_keys;
                 it.kv = ctx + kept;
@@ -198,41 +218,58 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
             blocks += total;
         }
         if (tid == 0) {
-            cum[items] = blocks;
             a.schedule[2 * rank] = items;
             a.schedule[2 * rank + 1] = blocks;
         }
-    } else {
-        // ---- table entries, the free list, positions and slots --------------------------------------
-        const int at = (rank - 2) * PLAN_THREADS + tid, step = (PLAN_CTAS - 2) * PLAN_THREADS;
-        for (int j = at; j < sum_taken; j += step) {
-            const int b = find(taken, B, j);
-            a.table[b * a.table_stride + pages(ctx_of(b)) + (j - taken[b])] = nth_taken(j);
-        }
-        for (int r = at; r < sum_back; r += step)
-            if (count + r < a.n_pages) a.free_list[count + r] = given_back(r);
-        for (int t = at; t < a.max_tokens; t += step) {
-            int pos = -1;
-            long long slot = -1;
-            if (t < sum_tok) {
-                const int b = find(cu, B, t), ctx = ctx_of(b);
-                pos = ctx + (t - cu[b]);
-                const int col = pos >> a.page_shift, held = pages(ctx);
-                if (col < a.max_pages) {
-                    const int p = pool && col >= held ? nth_taken(taken[b] + col - held) : a.table[b * a.table_stride + col];
-                    if (p >= 0) slot = ((long long)p << a.page_shift) + (pos & (page - 1));
+        __syncthreads();
+        // each worker's stretch of the blocks of all kv heads
+        const int over = decodes ? 0 : CHUNK_OVER, workers = decodes ? a.workers : a.workers / 2;
+        const long long per_head = blocks + (long long)items * over, total = per_head * a.H_kv;
+        Start* const starts = reinterpret_cast<Start*>(a.schedule + (decodes ? a.sched.decode_starts : a.sched.chunk_starts));
+        if (tid < workers) {
+            Start st = {};
+            const long long w = tid * total / workers, hi = (tid + 1) * total / workers;
+            if (w < hi) {
+                st.h = (int)(w / per_head);
+                const int r = (int)(w % per_head);
+                int lo = 0, up = items;  // the last item that begins at r or in front
+                while (up - lo > 1) {
+                    const int mid = (lo + up) >> 1;
+                    if (cum[mid] + mid * over <= r) lo = mid;
+                    else up = mid;
                 }
+                const int off = r - cum[lo] - lo * over;
+                st.it = list[lo];
+                st.item = lo;
+                st.blk = max(off - over, 0);
+                st.n_items = items;
+                st.begins = w - off;
+                st.hi = hi;
             }
-            a.positions[t] = pos;
-            a.slots[t] = slot;
+            starts[tid] = st;
         }
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0 && tid == 0 && pool) {
-        const int left = max(stack - sum_taken, 0);
-        a.info[5] = left;
-        *a.free_count_out = left;
+    } else {
+        // ---- positions and slots: four tokens a thread, one bisection, and four table entries on their way at once ----
+        __syncthreads();
+        const int at = (rank - 2) * PLAN_THREADS + tid, step = (PLAN_CTAS - 2) * PLAN_THREADS;
+        for (int t0 = 4 * at; t0 < a.max_tokens; t0 += 4 * step) {
+            int b = t0 < sum_tok ? find(cu, B, t0) : B - 1;
+            int pos[4], page_of[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = t0 + i;
+                while (t < sum_tok && cu[b + 1] <= t) ++b;
+                pos[i] = t < sum_tok ? ctx_lens[b] + (t - cu[b]) : -1;
+                const int col = pos[i] >> a.page_shift;
+                page_of[i] = t < sum_tok && col < a.max_pages ? a.table[b * a.table_stride + col] : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (t0 + i >= a.max_tokens) break;
+                a.positions[t0 + i] = pos[i];
+                a.slots[t0 + i] = page_of[i] >= 0 ? ((long long)page_of[i] << a.page_shift) + (pos[i] & (page - 1)) : -1;
+            }
+        }
     }
 }
 
@@ -266,42 +303,62 @@ struct PrestepArgs {
     int page_shift;
 };
 
-// A CTA takes a token: its cosines and sines once, then a warp per head, 8 values (16 bytes) a lane; d == 128: a head per half warp.
-template <int D, bool BF16>
+// A CTA takes a token, or a part of its heads; the heads of q, then of k, then of v, 8 values (16 bytes) a lane, so d / 8 lanes a head.  The
+// token's bytes bound it: all of a warp's HEADS heads are on their way while the first threads form the cosines and sines.
+template <int D, bool BF16, int HEADS>
 __global__ void __launch_bounds__(PRE_WARPS * 32) khq_paged_prestep_kernel(const __grid_constant__ PrestepArgs p) {
-    constexpr int LANES = D / 8;
+    constexpr int LANES = D / 8, PER = PRE_WARPS * 32 / LANES;
     __shared__ float2 turn[MAX_PAIRS];
     const khq_paged_prestep_args& a = p.a;
-    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, heads = PRE_WARPS * 32 / LANES;
-    const int t = blockIdx.x, n_pairs = a.rotary_dim / 2, half_lanes = a.rotary_dim / 16;
+    const int lane = threadIdx.x % LANES, first = blockIdx.y * (PER * HEADS) + threadIdx.x / LANES, heads = a.H_q + 2 * a.H_kv;
+    const long long t = blockIdx.x;
+    const int n_pairs = a.rotary_dim / 2, half_lanes = a.rotary_dim / 16;
     khq::pdl_wait();
     khq::pdl_trigger();
     const int pos = static_cast<const int*>(a.positions)[t];
-    if (pos < 0) return;  // behind the last token
     long long slot = static_cast<const long long*>(a.slots)[t];
+    uint4 raw[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const int h = first + i * PER, hk = h - a.H_q, hv = hk - a.H_kv;
+        const uint16_t* src = h < a.H_q ? static_cast<const uint16_t*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1]
+                              : hk < a.H_kv ? static_cast<const uint16_t*>(a.k) + t * a.k_stride[0] + hk * a.k_stride[1]
+                                            : static_cast<const uint16_t*>(a.v) + t * a.v_stride[0] + hv * a.v_stride[1];
+        raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src + lane * 8) : make_uint4(0, 0, 0, 0);
+    }
+    if (pos < 0) return;  // behind the last token
     if (slot >= (long long)a.n_pages << p.page_shift) slot = -1;
-    for (int i = threadIdx.x; i < n_pairs; i += PRE_WARPS * 32) {
-        double turns = (double)pos * p.freq[i];
+    if (threadIdx.x < n_pairs) {
+        double turns = (double)pos * p.freq[threadIdx.x];
         turns -= rint(turns);
         float s, c;
         sincospif((float)(2.0 * turns), &s, &c);
-        turn[i] = make_float2(c, s);
+        turn[threadIdx.x] = make_float2(c, s);
     }
     __syncthreads();
+    // the rotary pair of value e of lane l is value e of lane l +- half_lanes; x cos + y sin with the sign on the lower lane's sine, and cosine 1,
+    // sine 0 where nothing is rotated
+    const bool low = lane < half_lanes, turned = lane < 2 * half_lanes;
+    const int partner = low ? lane + half_lanes : turned ? lane - half_lanes : lane;
+    float cs[8], sn[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float2 f = turned ? turn[(low ? lane : partner) * 8 + e] : make_float2(1.0f, 0.0f);
+        cs[e] = f.x;
+        sn[e] = low ? -f.y : f.y;
+    }
     const long long pg = slot >> p.page_shift, at = slot & (a.page_size - 1);
-    for (int h0 = 0; h0 < a.H_q + a.H_kv; h0 += heads) {  // whole warps stay together
-        const int h = min(h0 + sub, a.H_q + a.H_kv - 1);
-        const bool is_q = h < a.H_q, mine = h == h0 + sub;
-        const int hk = h - a.H_q;
-        const uint16_t* src = is_q ? static_cast<const uint16_t*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1]
-                                   : static_cast<const uint16_t*>(a.k) + t * a.k_stride[0] + hk * a.k_stride[1];
-        const uint4 raw = *reinterpret_cast<const uint4*>(src + lane * 8);
-        uint4 vv = make_uint4(0, 0, 0, 0);
-        if (!is_q && slot >= 0) vv = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.v) + t * a.v_stride[0] + hk * a.v_stride[1] + lane * 8);
-        const float* w = static_cast<const float*>(is_q ? a.q_norm_w : a.k_norm_w);
-        float x[8];
-        const uint32_t rw[4] = {raw.x, raw.y, raw.z, raw.w};
-        float sq = 0.0f;
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const int h = first + i * PER;
+        if (__all_sync(0xFFFFFFFFu, h >= heads)) break;  // whole warps stay together: at d 128 a warp has two heads
+        const bool is_q = h < a.H_q, is_v = h >= a.H_q + a.H_kv, mine = h < heads;
+        const int hk = is_v ? h - a.H_q - a.H_kv : h - a.H_q;
+        const auto cache_row = [&](void* base, const int64_t (&st)[3]) {
+            return reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + pg * st[0] + at * st[1] + hk * st[2] + lane * 8);
+        };
+        const uint32_t rw[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        float x[8], sq = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 f = unpack2<BF16>(rw[e]);
@@ -311,37 +368,25 @@ __global__ void __launch_bounds__(PRE_WARPS * 32) khq_paged_prestep_kernel(const
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xFFFFFFFFu, sq, o, LANES);
-        const float inv = 1.0f / sqrtf(sq / (float)D + a.rms_eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= inv;
+        const float inv = rsqrtf(sq * (1.0f / D) + a.rms_eps);
+        const float* w = static_cast<const float*>(is_q ? a.q_norm_w : a.k_norm_w);
+        float4 w0 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w1 = w0;
         if (w) {
-            const float4 w0 = reinterpret_cast<const float4*>(w + lane * 8)[0], w1 = reinterpret_cast<const float4*>(w + lane * 8)[1];
-            x[0] *= w0.x; x[1] *= w0.y; x[2] *= w0.z; x[3] *= w0.w;
-            x[4] *= w1.x; x[5] *= w1.y; x[6] *= w1.z; x[7] *= w1.w;
+            w0 = __ldg(reinterpret_cast<const float4*>(w + lane * 8));
+            w1 = __ldg(reinterpret_cast<const float4*>(w + lane * 8) + 1);
         }
-        const auto cache_row = [&](void* base, const int64_t (&st)[3]) {
-            return reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + pg * st[0] + at * st[1] + hk * st[2] + lane * 8);
-        };
-        if (mine && !is_q && slot >= 0 && a.u_cache) *cache_row(a.u_cache, a.u_cache_stride) = pack8<BF16>(x);
-        // the rotary pair of value e of lane l is value e of lane l +- half_lanes
-        const bool low = lane < half_lanes, turned = lane < 2 * half_lanes;
-        const int partner = low ? lane + half_lanes : turned ? lane - half_lanes : lane;
+        const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= inv * wv[e];
+        if (mine && !is_q && !is_v && slot >= 0 && a.u_cache) *cache_row(a.u_cache, a.u_cache_stride) = pack8<BF16>(x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float y = __shfl_sync(0xFFFFFFFFu, x[e], partner, LANES);
-            if (turned) {
-                const float2 cs = turn[(low ? lane : partner) * 8 + e];
-                x[e] = low ? x[e] * cs.x - y * cs.y : y * cs.y + x[e] * cs.x;
-            }
+            x[e] = x[e] * cs[e] + y * sn[e];
         }
-        const uint4 res = pack8<BF16>(x);
         if (!mine) continue;
-        if (is_q) {
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + t * a.q_out_stride[0] + h * a.q_out_stride[1] + lane * 8) = res;
-        } else if (slot >= 0) {
-            *cache_row(a.k_cache, a.k_cache_stride) = res;
-            *cache_row(a.v_cache, a.v_cache_stride) = vv;
-        }
+        if (is_q) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + t * a.q_out_stride[0] + h * a.q_out_stride[1] + lane * 8) = pack8<BF16>(x);
+        else if (slot >= 0) *(is_v ? cache_row(a.v_cache, a.v_cache_stride) : cache_row(a.k_cache, a.k_cache_stride)) = is_v ? raw[i] : pack8<BF16>(x);
     }
 }
 
@@ -369,23 +414,36 @@ int launch_prestep(const khq_paged_prestep_args* args, bool bf16, cudaStream_t s
     p.page_shift = log2_page(a.page_size);
     for (int i = 0; i < MAX_PAIRS; ++i)
         p.freq[i] = i < a.rotary_dim / 2 ? pow((double)a.rope_theta, -2.0 * i / a.rotary_dim) / 6.283185307179586476925 : 0.0;
-    cudaError_t err;
-    const unsigned grid = (unsigned)a.tokens, threads = PRE_WARPS * 32;
-    if (a.d == 256)
-        err = bf16 ? khq::launch_pdl(khq_paged_prestep_kernel<256, true>, grid, 0, 0, stream, threads, p)
-                   : khq::launch_pdl(khq_paged_prestep_kernel<256, false>, grid, 0, 0, stream, threads, p);
-    else
-        err = bf16 ? khq::launch_pdl(khq_paged_prestep_kernel<128, true>, grid, 0, 0, stream, threads, p)
-                   : khq::launch_pdl(khq_paged_prestep_kernel<128, false>, grid, 0, 0, stream, threads, p);
-    return static_cast<int>(err);
+    const auto launch = [&](auto kernel, int per_cta) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)a.tokens, (unsigned)((a.H_q + 2 * a.H_kv + per_cta - 1) / per_cta), 1);
+        cfg.blockDim = dim3(PRE_WARPS * 32, 1, 1);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, p));
+    };
+    // Few tokens: a head per warp, so that a token's heads are spread over more SMs.  Many: four, so that its angles are formed once or
+    // twice and more bytes are in flight.
+    const int per_warp = a.d == 256 ? 1 : 2, wide = a.tokens >= 2 * khq::sm_count() ? 4 : 1;
+    const int per_cta = PRE_WARPS * per_warp * wide;
+    if (a.d == 256) {
+        if (wide == 4) return bf16 ? launch(khq_paged_prestep_kernel<256, true, 4>, per_cta) : launch(khq_paged_prestep_kernel<256, false, 4>, per_cta);
+        return bf16 ? launch(khq_paged_prestep_kernel<256, true, 1>, per_cta) : launch(khq_paged_prestep_kernel<256, false, 1>, per_cta);
+    }
+    if (wide == 4) return bf16 ? launch(khq_paged_prestep_kernel<128, true, 4>, per_cta) : launch(khq_paged_prestep_kernel<128, false, 4>, per_cta);
+    return bf16 ? launch(khq_paged_prestep_kernel<128, true, 1>, per_cta) : launch(khq_paged_prestep_kernel<128, false, 1>, per_cta);
 }
 
 }  // namespace khq_paged
 
-extern "C" size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, int H_q, int H_kv) {
+extern "C" size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, int H_q, int H_kv, int d) {
     using namespace khq_paged;
-    if (requests <= 0 || max_tokens <= 0 || max_new <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || H_q / H_kv > MAX_REP) return 0;
-    return (size_t)schedule_of(requests, max_tokens, max_new, H_q, H_kv).ints * 4;
+    if (requests <= 0 || max_tokens <= 0 || max_new <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || H_q / H_kv > MAX_REP || (d != 128 && d != 256)) return 0;
+    return (size_t)schedule_of(requests, max_tokens, max_new, H_q, H_kv, d).ints * 4;
 }
 
 extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream_t stream) {
@@ -397,18 +455,18 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
         return -100;
     if (p.free_list ? (p.n_pages <= 0 || !p.free_count || !p.free_count_out) : (p.free_count || p.free_count_out)) return -100;
     const int shift = log2_page(p.page_size);
-    if (shift < 0 || p.H_q % p.H_kv != 0 || p.H_q / p.H_kv > MAX_REP || p.requests > PLAN_MAX_REQUESTS || p.max_tokens > PLAN_MAX_TOKENS ||
+    if (shift < 0 || (p.d != 128 && p.d != 256) || p.H_q % p.H_kv != 0 || p.H_q / p.H_kv > MAX_REP || p.requests > PLAN_MAX_REQUESTS || p.max_tokens > PLAN_MAX_TOKENS ||
         (long long)p.requests * p.max_pages > 0x7FFFFFFFLL || p.table_stride < p.max_pages || (long long)p.max_pages << shift > (1LL << 30))
         return -103;
     const void* ptrs[] = {p.ctx_lens, p.new_lens, p.block_table, p.free_list, p.free_count, p.free_count_out, p.cu_new, p.kv_lens, p.positions, p.info};
     for (const void* q : ptrs)
         if ((reinterpret_cast<uintptr_t>(q) & 3) != 0) return -104;
     if ((reinterpret_cast<uintptr_t>(p.slots) & 7) != 0 || (reinterpret_cast<uintptr_t>(p.schedule) & 15) != 0) return -104;
-    const Schedule sched = schedule_of(p.requests, p.max_tokens, p.max_new, p.H_q, p.H_kv);
+    const Schedule sched = schedule_of(p.requests, p.max_tokens, p.max_new, p.H_q, p.H_kv, p.d);
     if (p.schedule_bytes < (size_t)sched.ints * 4) return -105;
     // the key blocks of all items are counted in 32 bits
     const long long row = ((long long)p.max_pages << shift) + p.max_tokens;
-    if (sched.chunk_cap * (row / TILE_KEYS + 1 + CHUNK_OVER) > 0x7FFFFFFFLL || sched.decode_cap * (row / DECODE_KEYS + 1) > 0x7FFFFFFFLL) return -103;
+    if (sched.chunk_cap * (row / TILE_KEYS + 1 + CHUNK_OVER) > 0x7FFFFFFFLL || sched.decode_cap * (row / sched.decode_keys + 1) > 0x7FFFFFFFLL) return -103;
     PlanArgs a;
     a.ctx_lens = static_cast<const int*>(p.ctx_lens);
     a.new_lens = static_cast<const int*>(p.new_lens);
@@ -429,15 +487,22 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
     a.page_shift = shift;
     a.max_tokens = p.max_tokens;
     a.max_new = p.max_new;
+    a.H_kv = p.H_kv;
+    a.workers = khq::sm_count() < MAX_WORKERS ? khq::sm_count() : MAX_WORKERS;
     a.sched = sched;
-    const size_t smem = (size_t)3 * (p.requests + 1) * 4;
+    // the items' sums in shared memory too, where there is room
+    constexpr size_t room = (size_t)3 * (PLAN_MAX_REQUESTS + 1) * 4;
+    size_t smem = (size_t)3 * (p.requests + 1) * 4;
+    const size_t cum = (size_t)(sched.chunk_cap > sched.decode_cap ? sched.chunk_cap : sched.decode_cap) * 4;
+    a.cum_in_smem = smem + cum <= room;
+    if (a.cum_in_smem) smem += cum;
     static bool attr_done[64] = {};
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return static_cast<int>(err);
     if (dev < 0 || dev >= 64) return -100;
     if (!attr_done[dev]) {
-        err = cudaFuncSetAttribute((const void*)khq_paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (PLAN_MAX_REQUESTS + 1) * 4);
+        err = cudaFuncSetAttribute((const void*)khq_paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
         if (err != cudaSuccess) return static_cast<int>(err);
         attr_done[dev] = true;
     }

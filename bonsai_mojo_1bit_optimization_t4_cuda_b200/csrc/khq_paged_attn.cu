@@ -45,6 +45,12 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* st
     return bounded([&] { return khq::mbar_try_wait(bar, parity); }, [](bool x) { return x; }, status);
 }
 
+// By worker: how many records there are of the segment which begins in it and goes on in the next ones (0: none), and what joining them needs.
+struct alignas(16) Meta {
+    int n, h, row0, ntok;
+    int first, total, pad[2];  // with fewer blocks than workers: the segment's first block, the blocks; else first is -1
+};
+
 struct Params {
     const uint16_t *q, *gate;
     uint16_t* out;
@@ -52,9 +58,9 @@ struct Params {
     long long q_ts, q_hs, g_ts, g_hs, o_ts, o_hs, table_stride;
     const int *table, *schedule;
     const Item* items;
-    const int* cum;
+    const Start* starts;
     float* records;
-    int4* meta;  // by worker (CTA or pair): records of the segment which begins in it and goes on (0: none), item, kv head, first block
+    Meta* meta;
     int tokens, max_pages, n_pages, page_shift, page_mask, H_q, H_kv, n_rep, rep_mul;  // x / n_rep = x * rep_mul >> 16 for x < 128
     float scale_log2e;
 };
@@ -73,25 +79,24 @@ __device__ __forceinline__ void load_segment(const Params& p, Segment& s) {
     s.row0 = y.x;
     s.pos0 = y.y;
 }
-// Block w of the row of all blocks, in which each item stands with `over` blocks in front of its own that stand for its fixed cost.  Returns
-// where the item begins in that row; s.blk: the block, 0 for those in front.  A warp bisects by 32.
-__device__ __forceinline__ long long find_segment(const Params& p, int n_items, long long per_head, int over, long long w, Segment& s) {
-    const int lane = threadIdx.x & 31;
-    s.h = (int)(w / per_head);
-    const int r = (int)(w % per_head);
-    int lo = 0, n = n_items;  // the last item of [lo, lo + n) that begins at r or in front
-    while (n > 1) {
-        const int step = (n + 31) / 32, at = lane * step < n ? lo + lane * step : lo;
-        const unsigned below = __ballot_sync(0xFFFFFFFFu, lane * step < n && __ldg(p.cum + at) + at * over <= r);
-        const int last = 31 - __clz((int)(below | 1u));
-        lo += last * step;
-        n = min(step, n - last * step);
-    }
-    s.item = lo;
-    load_segment(p, s);
-    const int off = r - __ldg(p.cum + lo) - lo * over;
-    s.blk = max(off - over, 0);
-    return w - off;
+// The worker's first segment; false: none.
+__device__ __forceinline__ bool first_segment(const Params& p, int worker, Segment& s, int& n_items, long long& begins, long long& hi) {
+    const int4* at = reinterpret_cast<const int4*>(p.starts + worker);
+    const int4 x = at[0], y = at[1], z = at[2];  // (ordinary loads: nothing else keeps them behind the wait for the plan)
+    const longlong2 w = *reinterpret_cast<const longlong2*>(at + 3);
+    s.b = x.x;
+    s.n_blocks = x.y;
+    s.ntok = x.z;
+    s.kv = x.w;
+    s.row0 = y.x;
+    s.pos0 = y.y;
+    s.item = z.x;
+    s.h = z.y;
+    s.blk = z.z;
+    n_items = z.w;
+    begins = w.x;
+    hi = w.y;
+    return hi > 0;
 }
 // Every item has a key block at least (its own tokens).
 __device__ __forceinline__ void next_segment(const Params& p, int n_items, Segment& s) {
@@ -122,35 +127,39 @@ __device__ __forceinline__ void store_out(const Params& p, int row, int head, in
 
 // Who shares a segment of blocks [seg_lo, seg_hi) that begins with worker `first`: the workers whose stretch has blocks of it.  (With fewer blocks than workers some
 // have none.)
-__device__ __forceinline__ int4 shared_segment(long long seg_lo, long long seg_hi, long long total, int first, int workers, int item, int h) {
-    const int last = (int)((seg_hi * workers - 1) / total);
-    return make_int4(total >= workers ? last - first + 1 : (int)(seg_hi - seg_lo), item, h, total >= workers ? -1 : (int)seg_lo);
+__device__ __forceinline__ void write_meta(Meta* meta, long long seg_lo, long long seg_hi, long long total, int first, int workers, const Segment& s) {
+    const bool all = total >= workers;
+    int4* const at = reinterpret_cast<int4*>(meta + first);
+    at[0] = make_int4(all ? (int)((seg_hi * workers - 1) / total) - first + 1 : (int)(seg_hi - seg_lo), s.h, s.row0, s.ntok);
+    at[1] = make_int4(all ? -1 : (int)seg_lo, all ? 0 : (int)total, 0, 0);
+}
+__device__ __forceinline__ Meta read_meta(const Meta* meta) {
+    const int4* at = reinterpret_cast<const int4*>(meta);
+    const int4 x = at[0], y = at[1];
+    return Meta{x.x, x.y, x.z, x.w, y.x, y.y, {0, 0}};
 }
 // The worker of the segment's i-th record.
-__device__ __forceinline__ int record_worker(const int4& meta, int first, int i, long long total, int workers) {
-    return meta.w < 0 ? first + i : (int)(((meta.w + i + 1LL) * workers - 1) / total);
+__device__ __forceinline__ int record_worker(const Meta& m, int begins_in, int i, int workers) {
+    return m.first < 0 ? begins_in + i : ((m.first + i + 1) * workers - 1) / m.total;
 }
 
 // Joins the records of the segment that begins in CTA blockIdx.x of the decode kernel and goes on in the next ones; rows blockIdx.y, + gridDim.y, ..
 // A CTA's record 1 is of the segment that begins in it, record 0 of one that it took over.  Groups of D / 4 threads take the records in
 // turn, 4 columns a thread.
-constexpr int MERGE_THREADS = 256, MAX_WORKERS = 256;
+constexpr int MERGE_THREADS = 256;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Params p, int record_floats, int workers) {
-    constexpr int PER_ROW = D / 4, GROUPS = MERGE_THREADS / PER_ROW;
+    constexpr int PER_ROW = D / 4, GROUPS = MERGE_THREADS / PER_ROW, ROWS = DECODE_ROWS;
     __shared__ float factor[MAX_WORKERS];
     __shared__ int base[MAX_WORKERS];
     __shared__ float4 sums[GROUPS][PER_ROW];
     khq::pdl_wait();
     khq::pdl_trigger();
-    const int4 meta = p.meta[blockIdx.x];
-    if (meta.x == 0) return;
-    Segment seg;
-    seg.item = meta.y;
-    load_segment(p, seg);
-    const int R = seg.ntok * p.n_rep, n = meta.x, tid = threadIdx.x, lane = tid & 31;
-    const long long total = (long long)p.schedule[3] * p.H_kv;
-    for (int i = tid; i < n; i += MERGE_THREADS) base[i] = 2 * record_worker(meta, blockIdx.x, i, total, workers) + (i == 0);
+    const Meta meta = read_meta(p.meta + blockIdx.x);
+    const int n = meta.n, tid = threadIdx.x, lane = tid & 31;
+    if (n == 0) return;
+    const int R = meta.ntok * p.n_rep;
+    for (int i = tid; i < n; i += MERGE_THREADS) base[i] = 2 * record_worker(meta, blockIdx.x, i, workers) + (i == 0);
     const int col = tid % PER_ROW, group = tid / PER_ROW;
     for (int r = blockIdx.y; r < R; r += gridDim.y) {
         __syncthreads();
@@ -161,7 +170,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Pa
         for (int k = 0; k < MAX_WORKERS / 32; ++k) {
             const int i = k * 32 + lane;
             ml[k] = make_float2(-INFINITY, 0.0f);
-            if (i < n) ml[k] = *reinterpret_cast<const float2*>(p.records + (long long)base[i] * record_floats + DECODE_ROWS * D + 2 * r);
+            if (i < n) ml[k] = *reinterpret_cast<const float2*>(p.records + (long long)base[i] * record_floats + ROWS * D + 2 * r);
             M = fmaxf(M, ml[k].x);
         }
 #pragma unroll
@@ -188,7 +197,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Pa
         }
         sums[group][col] = acc;
         __syncthreads();
-        const int row = seg.row0 + r / p.n_rep, head = meta.z * p.n_rep + r % p.n_rep;
+        const int t = (r * p.rep_mul) >> 16, row = meta.row0 + t, head = meta.h * p.n_rep + (r - t * p.n_rep);
         if (group != 0 || row >= p.tokens) continue;
 #pragma unroll
         for (int g = 1; g < GROUPS; ++g) {
@@ -272,9 +281,9 @@ Work work_of(const Schedule& sched, int d) {
     w.ctas = khq::sm_count() < MAX_WORKERS ? khq::sm_count() : MAX_WORKERS;  // one per SM
     w.pairs = w.ctas / 2;
     w.decode_meta = 0;
-    w.decode_records = w.decode_meta + (size_t)w.ctas * 16;
+    w.decode_records = w.decode_meta + (size_t)w.ctas * sizeof(Meta);
     w.chunk_meta = w.decode_records + (sched.decodes ? (size_t)2 * w.ctas * (d == 256 ? decode::Shape<256>::RECORD : decode::Shape<128>::RECORD) * 4 : 0);
-    w.chunk_records = w.chunk_meta + (sched.chunks ? (size_t)w.pairs * 16 : 0);
+    w.chunk_records = w.chunk_meta + (sched.chunks ? (size_t)w.pairs * sizeof(Meta) : 0);
     w.bytes = w.chunk_records + (sched.chunks ? (size_t)4 * w.pairs * (d == 256 ? tile::Shape<256>::RECORD : tile::Shape<128>::RECORD) * 4 : 0);
     return w;
 }
@@ -314,16 +323,16 @@ template <int D, bool BF16>
 int launch_kernels(const khq_paged_attn_args& a, Params p, const Schedule& sched, const Work& w, cudaStream_t stream) {
     int rc = prepare_kernels<D, BF16>();
     unsigned char* const ws = static_cast<unsigned char*>(a.workspace);
-    const auto of_kernel = [&](long long items, long long cum, size_t meta, size_t records) {
+    const auto of_kernel = [&](long long starts, long long items, size_t meta, size_t records) {
+        p.starts = reinterpret_cast<const Start*>(p.schedule + starts);
         p.items = reinterpret_cast<const Item*>(p.schedule + items);
-        p.cum = p.schedule + cum;
-        p.meta = reinterpret_cast<int4*>(ws + meta);
+        p.meta = reinterpret_cast<Meta*>(ws + meta);
         p.records = reinterpret_cast<float*>(ws + records);
     };
     cudaError_t err;
     if (sched.chunks) {
         using S = tile::Shape<D>;
-        of_kernel(sched.chunk_items, sched.chunk_cum, w.chunk_meta, w.chunk_records);
+        of_kernel(sched.chunk_starts, sched.chunk_items, w.chunk_meta, w.chunk_records);
         CUtensorMap mq, mk, mv;
         if (rc == 0) rc = query_map(&mq, a.q, a.q_stride, a.tokens, a.H_q, D, p.n_rep, tile::BR / p.n_rep, BF16);
         if (rc == 0)
@@ -335,10 +344,10 @@ int launch_kernels(const khq_paged_attn_args& a, Params p, const Schedule& sched
     }
     const Params chunk = p;
     if (sched.decodes) {
-        of_kernel(sched.decode_items, sched.decode_cum, w.decode_meta, w.decode_records);
+        of_kernel(sched.decode_starts, sched.decode_items, w.decode_meta, w.decode_records);
         CUtensorMap mk, mv;
-        if (rc == 0) rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
-        if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::UNIT, D / 64, BF16);
+        if (rc == 0) rc = cache_map(&mk, a.k_cache, a.k_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::box_tokens<D>(a.page_size), decode::box_groups<D>(a.page_size), BF16);
+        if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::box_tokens<D>(a.page_size), decode::box_groups<D>(a.page_size), BF16);
         if (rc != 0) return rc;
         err = khq::launch_pdl(decode::khq_paged_decode_kernel<D, BF16>, (unsigned)w.ctas, 0, (size_t)decode::Shape<D>::SMEM, stream,
                               (unsigned)(decode::WARPS * 32), mk, mv, p, (int)sched.chunks);
@@ -378,7 +387,7 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
         if (((a.q_stride[i] | (a.gate ? a.gate_stride[i] : 0) | a.out_stride[i]) & 7) != 0) return -104;
     for (int i = 0; i < 3; ++i)
         if (((a.k_cache_stride[i] | a.v_cache_stride[i]) & 7) != 0 || a.k_cache_stride[i] < 0 || a.v_cache_stride[i] < 0) return -104;
-    const Schedule sched = schedule_of(a.requests, a.max_tokens, a.max_new, a.H_q, a.H_kv);
+    const Schedule sched = schedule_of(a.requests, a.max_tokens, a.max_new, a.H_q, a.H_kv, a.d);
     const Work w = work_of(sched, a.d);
     if (a.schedule_bytes < (size_t)sched.ints * 4 || a.workspace_bytes < w.bytes) return -105;
     Params p;
@@ -413,7 +422,7 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
 
 extern "C" size_t khq_b200_paged_workspace_bytes(int max_new, int H_q, int H_kv, int d) {
     if (max_new <= 0 || !heads_ok(H_q, H_kv) || (d != 128 && d != 256)) return 0;
-    return (work_of(schedule_of(1, 1, max_new, H_q, H_kv), d).bytes + 255) / 256 * 256;
+    return (work_of(schedule_of(1, 1, max_new, H_q, H_kv, d), d).bytes + 255) / 256 * 256;
 }
 
 extern "C" int launch_khq_paged_attn_fp16(const khq_paged_attn_args* args, khq_stream_t stream) { return launch_attn(args, false, stream); }

@@ -1,28 +1,37 @@
 // khq_paged_decode.cuh -- attention over the paged cache for tiles of up to 16 query rows (a decode step: one or a few new tokens a
 // request).  Included by khq_paged_attn.cu.
 //
-// Every K and V byte is used by 16 rows at most, so the cache's bytes bound it.  The key blocks (64 keys) of all (kv head,
+// Every K and V byte is used by 16 rows at most, so the cache's bytes bound it.  The key blocks (64 keys, 128 at d 128) of all (kv head,
 // item) pairs stand in one row, and each CTA takes an equal stretch of it (one CTA per SM): any mix of lengths is even, and a CTA ends up with at most two
 // segments that it shares with others.  Those leave records (unnormalised rows, maximum, sum) that khq_paged_merge_kernel joins
 // in a fixed order; the others are finished here.
 //
-// A warp takes 16 keys of each block and runs alone: its first lane brings the 16 rows of K and V in by TMA (pages of 16 tokens and more hold
-// them in one piece) some units ahead, into a ring that no other warp touches; S = Q K^T and O += P V are mma.sync m16n8k16 with the query rows
-// as M and all of O in registers.  Only at a segment's end the four warps join their maxima, sums and rows through shared memory.
+// A warp takes a unit of each block, 16 keys (32 at d 128), and runs alone: its first lanes bring their rows of K and V in by TMA three units
+// ahead, into a ring that no other warp touches; S = Q K^T and O += P V are mma.sync m16n8k16 with the query rows as M and all of O in
+// registers.  Only at a segment's end the four warps join their maxima, sums and rows through shared memory.
+// One warp a scheduler, so a unit's chain of latencies counts (2100 cycles for 16 keys at d 128): 16 KB a unit and one wait for both halves
+// of it keep the chain below the time that memory takes.  64 sequences of 4200 tokens, d 256: 185 us; with eight warps and half the
+// ring for each 235; with K and V waited for one after the other, and one chain of products instead of two, 251.
 #pragma once
 
 namespace khq_paged {
 namespace decode {
 
-constexpr int WARPS = 4, UNIT = 16;  // keys a warp takes at a time
-static_assert(WARPS * UNIT == DECODE_KEYS, "a block is a unit per warp");
+constexpr int WARPS = 4;
+constexpr int JOIN_ROWS = 8;  // rows that are joined at a time
 template <int D> struct Shape {
-    static constexpr int UNIT_BYTES = UNIT * D * 2, STAGE_BYTES = 2 * UNIT_BYTES, STAGES = 3 * 256 / D;
+    static constexpr int KEYS = 64 * 256 / D, UNIT = KEYS / WARPS;   // of a block, of a warp's share of it
+    static constexpr int G = D / 64, PIECE = UNIT * D * 2, STAGES = 3;  // column groups; K or V of a unit; units in a warp's ring
+    static constexpr int NT = UNIT / 8;  // tiles of 8 keys
     static constexpr int ROW = D + 8;  // floats of a row in the join buffer: rows 8 banks apart
-    static constexpr int OFF_JOIN = WARPS * STAGES * STAGE_BYTES, OFF_ML = OFF_JOIN + WARPS * 8 * ROW * 4;
+    static constexpr int OFF_JOIN = WARPS * STAGES * 2 * PIECE, OFF_ML = OFF_JOIN + WARPS * JOIN_ROWS * ROW * 4;
     static constexpr int OFF_BARS = OFF_ML + WARPS * DECODE_ROWS * 8, SMEM = OFF_BARS + WARPS * STAGES * 8;
+    static_assert(SMEM <= 227 * 1024, "shared memory");
     static constexpr int RECORD = DECODE_ROWS * D + 2 * DECODE_ROWS;  // floats
 };
+// A piece is one box where a page holds the unit; else (32 keys, pages of 16) one per page and column group.
+template <int D> int box_tokens(int page_size) { return page_size < Shape<D>::UNIT ? page_size : Shape<D>::UNIT; }
+template <int D> int box_groups(int page_size) { return page_size < Shape<D>::UNIT ? 1 : Shape<D>::G; }
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -58,6 +67,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     if (lane == 0) {
         for (int s = 0; s < S::STAGES; ++s) khq::mbar_init(&bars[warp * S::STAGES + s], 1);
         khq::fence_barrier_init();
+        prefetch_map(warp & 1 ? &tm_k : &tm_v);
     }
     __syncthreads();
     // Behind the chunk kernel of the same step (`beside`) there is nothing to wait for: that one lets this one start once everything before
@@ -67,31 +77,31 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     khq::pdl_trigger();
 
     // ---- this CTA's stretch of the key blocks ------------------------------------------------------
-    const int n_items = p.schedule[2];
-    const long long per_head = p.schedule[3], total = per_head * p.H_kv;
-    const long long lo = blockIdx.x * total / gridDim.x, hi = (blockIdx.x + 1) * total / gridDim.x;
-    if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);  // overwritten below if a segment goes on in the next CTA
-    if (lo >= hi) {
+    Segment in, cur;  // where the loads and where the products are
+    int n_items;
+    long long begins, hi;
+    const bool work = first_segment(p, blockIdx.x, in, n_items, begins, hi);
+    if (tid == 0) p.meta[blockIdx.x].n = 0;  // overwritten below if a segment goes on in the next CTA
+    if (!work) {
         if (beside) khq::pdl_wait();
         return;
     }
-    Segment in, cur;  // where the loads and where the products are
-    find_segment(p, n_items, per_head, 0, lo, in);
+    const int blocks = (int)(hi - begins) - in.blk;  // of the stretch, which begins at begins + in.blk
     cur = in;
     uint64_t* const bar = bars + warp * S::STAGES;
-    const uint32_t ring = smem_u32(smem) + warp * S::STAGES * S::STAGE_BYTES;
+    const uint32_t ring = smem_u32(smem) + warp * S::STAGES * 2 * S::PIECE;
 
     // ---- loads ---------------------------------------------------------------------------------------
-    // Lane i of `pages` has the page of the unit i blocks behind `pages_at`, the next 32 are on their way; n_pages: none (the copy then fills in
-    // zeros, and the unit is skipped).
+    // The lanes hold the pages of the units of 32 blocks (16, where a unit has two), the next ones are on their way; n_pages: none (the
+    // copy then fills in zeros, and the keys are masked).
+    constexpr int UNIT = S::UNIT;
+    const int log_per = UNIT == 32 && p.page_shift == 4 ? 1 : 0, groups = log_per ? S::G : 1;
     int pages = 0, pages_next = 0, pages_at = -1;
-    long long w_in = lo;
-    int s_in = 0;
-    uint32_t missing = 0;  // by stage: the unit has no page
+    int w_in = 0, s_in = 0;
+    uint32_t missing = 0;  // two bits by unit of the ring: its first, second page is not there
     bool ok = true;        // no wait has run out
-    int issued = 0;        // units, by lane 0
     const auto fetch_pages = [&](int blk) {
-        const int key = (blk + lane) * DECODE_KEYS + warp * UNIT, col = key >> p.page_shift;
+        const int key = (blk + (lane >> log_per)) * S::KEYS + warp * UNIT + ((lane & log_per) << 4), col = key >> p.page_shift;
         int pg = p.n_pages;
         if (key < in.kv && col < p.max_pages) {
             pg = __ldg(p.table + in.b * p.table_stride + col);
@@ -100,25 +110,27 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         return pg;
     };
     const auto issue = [&]() {
-        if (w_in >= hi) return;
-        if (pages_at < 0 || in.blk - pages_at >= 32) {
+        if (w_in >= blocks) return;
+        if (pages_at < 0 || in.blk - pages_at >= (32 >> log_per)) {
             pages = pages_at < 0 ? fetch_pages(in.blk) : pages_next;
             pages_at = in.blk;
-            pages_next = fetch_pages(in.blk + 32);
+            pages_next = fetch_pages(in.blk + (32 >> log_per));
         }
-        const int page = __shfl_sync(0xFFFFFFFFu, pages, in.blk - pages_at);
-        const int key = in.blk * DECODE_KEYS + warp * UNIT;
-        missing = (missing & ~(1u << s_in)) | ((uint32_t)(page == p.n_pages) << s_in);
-        if (ok && lane == 0) {
-            ++issued;
-            const uint32_t dst = ring + s_in * S::STAGE_BYTES;
-            khq::mbar_arrive_expect_tx(&bar[s_in], S::STAGE_BYTES);
-            tma_load_5d(dst, &tm_k, &bar[s_in], key & p.page_mask, 0, in.h, page);
-            tma_load_5d(dst + S::UNIT_BYTES, &tm_v, &bar[s_in], key & p.page_mask, 0, in.h, page);
+        const int page = __shfl_sync(0xFFFFFFFFu, pages, ((in.blk - pages_at) << log_per) + ((lane >> 3) & log_per));  // of this lane's box
+        const uint32_t holes = __ballot_sync(0xFFFFFFFFu, page == p.n_pages);  // lane 0: the first page, lane 8: the second
+        missing = (missing & ~(3u << (2 * s_in))) | (((holes & 1u) | ((holes >> 7) & 2u)) << (2 * s_in));
+        if (ok) {
+            if (lane == 0) khq::mbar_arrive_expect_tx(&bar[s_in], 2 * S::PIECE);
+            __syncwarp();
+            // boxes: one each of K and V, by lanes 0 and 4; or one by page (lane / 8), K or V (lane / 4 % 2) and group (lane % 4)
+            const int c = lane & 3;
+            if (lane < 8 << log_per && c < groups)
+                tma_load_5d(ring + (2 * s_in + ((lane >> 2) & 1)) * S::PIECE + c * (UNIT * 128) + (lane >> 3) * (16 * 128), lane & 4 ? &tm_v : &tm_k, &bar[s_in],
+                            (in.blk * S::KEYS + warp * UNIT) & p.page_mask, c, in.h, page);
         }
         s_in = s_in + 1 == S::STAGES ? 0 : s_in + 1;
         ++w_in;
-        if (++in.blk == in.n_blocks && w_in < hi) {
+        if (++in.blk == in.n_blocks && w_in < blocks) {
             next_segment(p, n_items, in);
             pages_at = -1;
         }
@@ -133,21 +145,20 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     // addresses of this lane's rows for ldmatrix; chunk c of key k is at (c ^ (k & 7)) << 4
     const int k_key = (lane & 7) + ((lane >> 4) & 1) * 8, k_chunk = (lane >> 3) & 1;
     const int v_key = (lane & 7) + ((lane >> 3) & 1) * 8, v_chunk = lane >> 4;
-    const uint32_t k_row = k_key * 128, v_row = S::UNIT_BYTES + v_key * 128, sw = (lane & 7);
+    const uint32_t k_row = k_key * 128, v_row = S::PIECE + v_key * 128, sw = (lane & 7);
     int s = 0;
     uint32_t phase = 0;
     bool fresh = true;
-    const int R_max = DECODE_ROWS;
 #pragma unroll 1
-    for (long long w = lo; w < hi; ++w) {
+    for (int w = 0; w < blocks; ++w) {
         const int R = cur.ntok * p.n_rep;
         if (fresh) {
             fresh = false;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int r = g + 8 * half, row = cur.row0 + r / p.n_rep;
+                const int r = g + 8 * half, t = (r * p.rep_mul) >> 16, row = cur.row0 + t;
                 const bool live = r < R && row < p.tokens;
-                const uint16_t* q = p.q + (live ? row * p.q_ts + (long long)(cur.h * p.n_rep + r % p.n_rep) * p.q_hs : 0) + t2;
+                const uint16_t* q = p.q + (live ? row * p.q_ts + (long long)(cur.h * p.n_rep + r - t * p.n_rep) * p.q_hs : 0) + t2;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     qf[kk][half] = live ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16)) : 0u;
@@ -160,44 +171,53 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
         }
         // (after a wait that ran out the warp goes on without data, so that the others are not left at a barrier; the status word tells)
-        ok = ok && __all_sync(0xFFFFFFFFu, wait_for(&bar[s], phase, status));
-        const int key0 = cur.blk * DECODE_KEYS + warp * UNIT;
-        if (ok && !((missing >> s) & 1u)) {
-            const uint32_t base = ring + s * S::STAGE_BYTES;
-            float x[2][4] = {}, y[2][4] = {};  // two chains each
+        if (ok && !(ok = __all_sync(0xFFFFFFFFu, wait_for(&bar[s], phase, status))))
+            for (int i = 1; i < S::STAGES; ++i) wait_for(&bar[(s + i) % S::STAGES], phase ^ (uint32_t)(s + i >= S::STAGES), status);  // what is still in flight
+        const int key0 = cur.blk * S::KEYS + warp * UNIT;
+        const uint32_t holes = (missing >> (2 * s)) & 3u;
+        constexpr int NT = S::NT;
+        if (ok && holes != 3u) {
+            const uint32_t base = ring + 2 * s * S::PIECE;
+            float x[NT][4] = {}, y[NT][4] = {};  // two chains each
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                uint32_t b[4];
-                ldsm4(base + (kk >> 2) * (UNIT * 128) + k_row + (((uint32_t)((kk & 3) * 2 + k_chunk) ^ sw) << 4), b);
-                if (kk & 1) {
-                    mma16816<BF16>(y[0], qf[kk], b[0], b[1]);
-                    mma16816<BF16>(y[1], qf[kk], b[2], b[3]);
-                } else {
-                    mma16816<BF16>(x[0], qf[kk], b[0], b[1]);
-                    mma16816<BF16>(x[1], qf[kk], b[2], b[3]);
+            for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t b[4];
+                    ldsm4(base + (kk >> 2) * (UNIT * 128) + n * (8 * 128) + k_row + (((uint32_t)((kk & 3) * 2 + k_chunk) ^ sw) << 4), b);
+                    mma16816<BF16>(kk & 1 ? y[n] : x[n], qf[kk], b[0], b[1]);
+                    mma16816<BF16>(kk & 1 ? y[n + 1] : x[n + 1], qf[kk], b[2], b[3]);
                 }
-            }
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[n][e] = (x[n][e] + y[n][e]) * p.scale_log2e;
-            const bool tail = key0 + UNIT > cur.kv;
             if (key0 + UNIT - 1 > cur.pos0) {  // some row's position lies in front of the unit's last key
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int at = cur.pos0 + (g + 8 * half) / p.n_rep;
+                    const int at = cur.pos0 + (((g + 8 * half) * p.rep_mul) >> 16);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
                             if (key0 + n * 8 + t2 + e > at) x[n][half * 2 + e] = -INFINITY;
                 }
             }
+            if (NT > 2 && holes) {  // one of the unit's two pages
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((holes >> (n >> 1)) & 1u) x[n][e] = -INFINITY;
+            }
+            uint32_t pf[NT / 2][4];
             float factor[2];
             bool grow = false;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                float mx = fmaxf(fmaxf(x[0][half * 2], x[0][half * 2 + 1]), fmaxf(x[1][half * 2], x[1][half * 2 + 1]));
+                float mx = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(x[n][half * 2], x[n][half * 2 + 1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
                 factor[half] = 1.0f;
@@ -209,15 +229,17 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     grow = true;
                 }
             }
-            uint32_t pf[4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const float ref = m[half] == -INFINITY ? 0.0f : m[half];
-                const float p0 = ex2_approx(x[0][half * 2] - ref), p1 = ex2_approx(x[0][half * 2 + 1] - ref);
-                const float p2 = ex2_approx(x[1][half * 2] - ref), p3 = ex2_approx(x[1][half * 2 + 1] - ref);
-                l[half] = l[half] * factor[half] + ((p0 + p1) + (p2 + p3));
-                pf[half] = pack2<BF16>(p0, p1);
-                pf[2 + half] = pack2<BF16>(p2, p3);
+                float sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float p0 = ex2_approx(x[n][half * 2] - ref), p1 = ex2_approx(x[n][half * 2 + 1] - ref);
+                    sum += p0 + p1;
+                    pf[n >> 1][(n & 1) * 2 + half] = pack2<BF16>(p0, p1);
+                }
+                l[half] = l[half] * factor[half] + sum;
             }
             if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
@@ -229,50 +251,54 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 }
             }
             // rows of V behind the request's last token may hold anything: a weight of 0 does not undo that
-            uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
-            if (tail) {
-                const int n = cur.kv - key0;  // keys that exist; this lane's are t2, t2 + 1 and those 8 further
-                keep0 = (t2 < n ? 0x0000FFFFu : 0u) | (t2 + 1 < n ? 0xFFFF0000u : 0u);
-                keep1 = (t2 + 8 < n ? 0x0000FFFFu : 0u) | (t2 + 9 < n ? 0xFFFF0000u : 0u);
+            uint32_t keep[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) keep[n] = 0xFFFFFFFFu;
+            if (key0 + UNIT > cur.kv) {
+                const int left = cur.kv - key0;  // keys that exist; this lane's are t2 and t2 + 1 of each 8
+#pragma unroll
+                for (int n = 0; n < NT; ++n) keep[n] = (n * 8 + t2 < left ? 0x0000FFFFu : 0u) | (n * 8 + t2 + 1 < left ? 0xFFFF0000u : 0u);
             }
 #pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-                uint32_t b[4];
-                ldsm4_trans(base + (n >> 2) * (UNIT * 128) + v_row + (((uint32_t)((n & 3) * 2 + v_chunk) ^ sw) << 4), b);
-                mma16816<BF16>(o[2 * n], pf, b[0] & keep0, b[1] & keep1);
-                mma16816<BF16>(o[2 * n + 1], pf, b[2] & keep0, b[3] & keep1);
-            }
+            for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+                for (int k = 0; k < NT / 2; ++k) {
+                    uint32_t b[4];
+                    ldsm4_trans(base + (n >> 2) * (UNIT * 128) + k * (16 * 128) + v_row + (((uint32_t)((n & 3) * 2 + v_chunk) ^ sw) << 4), b);
+                    mma16816<BF16>(o[2 * n], pf[k], b[0] & keep[2 * k], b[1] & keep[2 * k + 1]);
+                    mma16816<BF16>(o[2 * n + 1], pf[k], b[2] & keep[2 * k], b[3] & keep[2 * k + 1]);
+                }
         }
         __syncwarp();  // all lanes have read the stage
         s = s + 1 == S::STAGES ? 0 : s + 1;
         phase ^= (uint32_t)(s == 0);
         issue();
         const bool ends = cur.blk + 1 == cur.n_blocks;
-        if (ends || w + 1 == hi) {
+        if (ends || w + 1 == blocks) {
             // ---- join the warps ----------------------------------------------------------------------
-            const long long seg_lo = w - cur.blk, seg_hi = seg_lo + cur.n_blocks;
-            const bool whole = seg_lo >= lo && seg_hi <= hi;
+            const int seg_lo = w - cur.blk, seg_hi = seg_lo + cur.n_blocks;  // from the stretch's begin
+            const bool whole = seg_lo >= 0 && ends;
             float* const join = reinterpret_cast<float*>(smem + S::OFF_JOIN);
             float2* const ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 1);
                 l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 2);
-                if ((lane & 3) == 0) ml[warp * R_max + g + 8 * half] = make_float2(m[half], l[half]);
+                if ((lane & 3) == 0) ml[warp * DECODE_ROWS + half * 8 + g] = make_float2(m[half], l[half]);
             }
             __syncthreads();
             const auto top = [&](int r) {
                 float M = ml[r].x;
 #pragma unroll
-                for (int v = 1; v < WARPS; ++v) M = fmaxf(M, ml[v * R_max + r].x);
+                for (int v = 1; v < WARPS; ++v) M = fmaxf(M, ml[v * DECODE_ROWS + r].x);
                 return M;
             };
-            float* const rec = p.records + (2LL * blockIdx.x + (seg_lo >= lo ? 1 : 0)) * S::RECORD;
+            float* const rec = p.records + (2LL * blockIdx.x + (seg_lo >= 0 ? 1 : 0)) * S::RECORD;
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
                 if (half * 8 >= R) break;
-                const float M = top(g + 8 * half), f = m[half] == -INFINITY ? 0.0f : exp2f(m[half] - M);
-                float* const mine = join + (warp * 8 + g) * S::ROW + t2;
+                const float M = top(half * 8 + g), f = m[half] == -INFINITY ? 0.0f : ex2_approx(m[half] - M);
+                float* const mine = join + (warp * JOIN_ROWS + g) * S::ROW + t2;
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n)
                     *reinterpret_cast<float2*>(mine + n * 8) = half == 0 ? make_float2(o[n][0] * f, o[n][1] * f) : make_float2(o[n][2] * f, o[n][3] * f);
@@ -283,10 +309,10 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     float L = 0.0f;
 #pragma unroll
                     for (int v = 0; v < WARPS; ++v) {
-                        const float2 a = ml[v * R_max + r];
-                        L += a.x == -INFINITY ? 0.0f : a.y * exp2f(a.x - Mr);
+                        const float2 a = ml[v * DECODE_ROWS + r];
+                        L += a.x == -INFINITY ? 0.0f : a.y * ex2_approx(a.x - Mr);
                     }
-                    const int row = cur.row0 + r / p.n_rep, head = cur.h * p.n_rep + r % p.n_rep;
+                    const int t = (r * p.rep_mul) >> 16, row = cur.row0 + t, head = cur.h * p.n_rep + (r - t * p.n_rep);
                     const bool live = row < p.tokens;
                     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;  // a NaN stays one
 #pragma unroll
@@ -295,7 +321,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                         for (int v = 0; v < WARPS; ++v) {
-                            const float4 a = *reinterpret_cast<const float4*>(join + (v * 8 + rr) * S::ROW + c);
+                            const float4 a = *reinterpret_cast<const float4*>(join + (v * JOIN_ROWS + rr) * S::ROW + c);
                             acc.x += a.x;
                             acc.y += a.y;
                             acc.z += a.z;
@@ -311,16 +337,15 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 }
                 __syncthreads();
             }
-            if (tid == 0 && seg_lo >= lo && seg_hi > hi)
-                p.meta[blockIdx.x] = shared_segment(seg_lo, seg_hi, total, blockIdx.x, gridDim.x, cur.item, cur.h);
+            if (tid == 0 && seg_lo >= 0 && !ends) {
+                const long long lo = p.starts[blockIdx.x].begins + p.starts[blockIdx.x].blk;
+                write_meta(p.meta, lo + seg_lo, lo + seg_hi, (long long)p.schedule[3] * p.H_kv, blockIdx.x, gridDim.x, cur);
+            }
             fresh = true;
         }
         ++cur.blk;
-        if (ends && w + 1 < hi) next_segment(p, n_items, cur);
+        if (ends && w + 1 < blocks) next_segment(p, n_items, cur);
     }
-    // nothing this warp started may still be in flight when the CTA leaves
-    if (!ok && lane == 0)
-        for (int i = max(0, issued - S::STAGES); i < issued; ++i) wait_for(&bar[i % S::STAGES], (uint32_t)((i / S::STAGES) & 1), status);
     if (beside) khq::pdl_wait();
 }
 

@@ -94,11 +94,8 @@ struct Walk {
     long long begins, hi;  // where the segment's item begins, the stretch's end
     int n;                 // its blocks in this stretch
     Segment s;
-    __device__ __forceinline__ bool begin(const Params& p, int n_items, long long per_head) {
-        const long long total = per_head * p.H_kv, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, w = pair * total / pairs;
-        hi = (pair + 1) * total / pairs;
-        if (w >= hi) return false;
-        begins = find_segment(p, n_items, per_head, CHUNK_OVER, w, s);
+    __device__ __forceinline__ bool begin(const Params& p, int& n_items) {
+        if (!first_segment(p, blockIdx.x >> 1, s, n_items, begins, hi)) return false;
         count();
         return n > 0;
     }
@@ -185,8 +182,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     else asm volatile("bar.sync 1, %0;" ::"n"(NTHREADS) : "memory");
     tc_fence_after();
 
-    const int n_items = p.schedule[0];
-    const long long per_head = p.schedule[1] + (long long)n_items * CHUNK_OVER;
+    int n_items = 0;
     const int log_per = 7 - p.page_shift;  // pages of a block
     Walk walk;
     // 384 threads start with 168 registers each; the softmax threads, who hold 128 scores, take 208 and leave the others 88: together
@@ -200,7 +196,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         int g = 0, i = 0;
         bool ok = true;
         Pages pages;
-        for (bool more = walk.begin(p, n_items, per_head); ok && more; more = walk.step(p, n_items), ++i) {
+        for (bool more = walk.begin(p, n_items); ok && more; more = walk.step(p, n_items), ++i) {
             if (i > 0 && !(ok = tile::warp_wait(&bars[B_QFREE], (uint32_t)((i - 1) & 1), status))) break;
             if (lane == 0) {
                 if (rank == 0) khq::mbar_arrive_expect_tx(&bars[B_QFULL], 2u * (uint32_t)(rows * 128 * S::G));
@@ -248,7 +244,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         int g = 0, lands = 0;
         bool ok = true;
         Pages pages;
-        for (bool more = walk.begin(p, n_items, per_head); ok && more; more = walk.step(p, n_items)) {
+        for (bool more = walk.begin(p, n_items); ok && more; more = walk.step(p, n_items)) {
             pages.begin(p, walk.s, walk.s.blk, log_per);
             for (int j = 0; j < walk.n; ++j, ++g) {
                 const int s = g % S::STAGES, blk = walk.s.blk + j, key0 = blk * BC;
@@ -325,7 +321,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 umma2_commit(one, &bars[B_KFREE + ks_at]);
             };
             int g = 0, i = 0;
-            bool more = walk.begin(p, n_items, per_head);
+            bool more = walk.begin(p, n_items);
             if (more) ok = tile::warp_wait(&bars[B_PEER], 0u, status);
             for (; ok && more; more = walk.step(p, n_items), ++i) {
                 ok = tile::warp_wait(&bars[B_QFULL], (uint32_t)(i & 1), status);
@@ -387,7 +383,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         unsigned char* const stage = smem + S::OFF_STG + warp * STG_BYTES;
         bool ok = true;
         int g0 = 0, i = 0;  // running index of the segment's first block; segments
-        if (tid == 0 && rank == 0) p.meta[blockIdx.x >> 1] = make_int4(0, 0, 0, 0);  // overwritten below if a segment goes on in the next pair
+        if (tid == 0 && rank == 0) p.meta[blockIdx.x >> 1].n = 0;  // overwritten below if a segment goes on in the next pair
         // pages that are not there, of block `blk` of a segment: bit by page
         const auto fetch_holes = [&](const Segment& sg, int blk) {
             const int col = (blk << log_per) + lane;
@@ -396,7 +392,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 hole = col >= p.max_pages || (unsigned)__ldg(p.table + sg.b * p.table_stride + (col < p.max_pages ? col : 0)) >= (unsigned)p.n_pages;
             return hole;
         };
-        bool more = walk.begin(p, n_items, per_head);
+        bool more = walk.begin(p, n_items);
         int hole_next = more && walk.n > grp ? fetch_holes(walk.s, walk.s.blk + grp) : 0;
         for (; ok && more; ++i) {
             const Segment& sg = walk.s;
@@ -604,8 +600,8 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 __syncwarp();
                 if (lane == 0) arrive_leader(&bars[B_OFREE]);
                 if (tid == 0 && rank == 0 && sg.blk == 0)  // it goes on in the next pairs
-                    p.meta[blockIdx.x >> 1] = shared_segment(walk.begins + CHUNK_OVER, walk.begins + CHUNK_OVER + sg.n_blocks, per_head * p.H_kv, (int)(blockIdx.x >> 1),
-                                                             (int)(gridDim.x >> 1), sg.item, sg.h);
+                    write_meta(p.meta, walk.begins + CHUNK_OVER, walk.begins + CHUNK_OVER + sg.n_blocks, (p.schedule[1] + (long long)n_items * CHUNK_OVER) * p.H_kv,
+                               (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1), sg);
             }
             g0 = last + 1;
             if (more) walk.step_to(next);
@@ -627,17 +623,13 @@ __global__ void __launch_bounds__(BR) khq_paged_tile_merge_kernel(const Params p
     __shared__ int base[MAX_WORKERS];
     khq::pdl_wait();
     khq::pdl_trigger();
-    const int4 meta = p.meta[blockIdx.x];
-    if (meta.x == 0) return;
-    const int rank = blockIdx.y / parts, part = blockIdx.y % parts, r = threadIdx.x, n = meta.x;
-    Segment s;
-    s.item = meta.y;
-    load_segment(p, s);
-    const int tok = BR / p.n_rep, t = (r * p.rep_mul) >> 16, n_tok = min(s.ntok - rank * tok, tok), row = s.row0 + rank * tok + t;
+    const Meta meta = read_meta(p.meta + blockIdx.x);
+    const int rank = blockIdx.y / parts, part = blockIdx.y % parts, r = threadIdx.x, n = meta.n;
+    if (n == 0) return;
+    const int tok = BR / p.n_rep, t = (r * p.rep_mul) >> 16, n_tok = min(meta.ntok - rank * tok, tok), row = meta.row0 + rank * tok + t;
     if (n_tok <= 0) return;
-    const long long total = (p.schedule[1] + (long long)p.schedule[0] * CHUNK_OVER) * p.H_kv;
     // record 1 is of the segment that begins in a pair, record 0 of one that it took over
-    for (int i = r; i < n; i += BR) base[i] = 2 * (2 * record_worker(meta, blockIdx.x, i, total, pairs) + rank) + (i == 0);
+    for (int i = r; i < n; i += BR) base[i] = 2 * (2 * record_worker(meta, blockIdx.x, i, pairs) + rank) + (i == 0);
     __syncthreads();
     if (t >= n_tok || row >= p.tokens) return;
     float M = -INFINITY;
@@ -665,7 +657,7 @@ __global__ void __launch_bounds__(BR) khq_paged_tile_merge_kernel(const Params p
             acc[c].w += a[c].w * f;
         }
     }
-    const int head = meta.z * p.n_rep + (r - t * p.n_rep);
+    const int head = meta.h * p.n_rep + (r - t * p.n_rep);
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
 #pragma unroll
     for (int c = 0; c < COLS; ++c) store_out<BF16>(p, row, head, (part * COLS + c) * 4, acc[c], inv);

@@ -71,7 +71,7 @@ SIGNATURES = {
     "launch_khq_compress_batched_fp16": (
         c_int, [_P, c_int, c_int] + [_P] * 9 + [c_int, c_float, c_float, c_int, c_longlong, _P]),
     "launch_khq_update_descs": (c_int, [_P, _P, c_int, c_int, _P]),
-    "khq_b200_paged_schedule_bytes": (c_size_t, [c_int] * 5),
+    "khq_b200_paged_schedule_bytes": (c_size_t, [c_int] * 6),
     "launch_khq_paged_plan": (c_int, [_P, _P]),
     "launch_khq_paged_prestep_fp16": (c_int, [_P, _P]),
     "launch_khq_paged_prestep_bf16": (c_int, [_P, _P]),

@@ -23,28 +23,41 @@ from typing import Optional
 import torch
 
 from . import lib as _lib
-from .lib import KhqLaunchError, check
+from .lib import check
 
 # the structs of include/khq_b200.h, field by field ("@": native alignment)
-_PLAN_ARGS = struct.Struct("@12PNq8i0q")
+_PLAN_ARGS = struct.Struct("@12PNq9i0q")
 _PRESTEP_ARGS = struct.Struct("@11P17q7i2f0q")
 _ATTN_ARGS = struct.Struct("@9P2N12qq10if0q")
 _TYPES = {torch.float16: "fp16", torch.bfloat16: "bf16"}
 
 
+# A step's host time is mostly the look at its tensors (some 0.1 us per property): each is asked for what it is checked by once.
+
+
 def _launch(fn, name: str, packed: bytes, device: int) -> None:
-    if torch.cuda.current_device() != device:
+    if _current_device() != device:
         with torch.cuda.device(device):
-            rc = fn(packed, _lib.current_stream())
+            rc = fn(packed, _current_stream(device))
     else:
-        rc = fn(packed, _lib.current_stream())
+        rc = fn(packed, _current_stream(device))
     if rc != 0:
         check(name, rc)
 
 
-def _want(cond: bool, text: str) -> None:
-    if not cond:
-        raise ValueError(text)
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _current_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _refuse(t, name: str, want, dtype, device: int):
+    if t.get_device() != device or t.dtype is not dtype or len(t.shape) != len(want) or any(w is not None and w != s for w, s in zip(want, t.shape)):
+        shape = ", ".join("any" if w is None else str(w) for w in want)
+        raise ValueError(f"{name}: wants ({shape}) {dtype} on cuda:{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    raise ValueError(f"{name}: the last dimension has to be contiguous, strides {t.stride()}")
 
 
 def _ints(t: torch.Tensor, name: str, numel: Optional[int], device: int, dtype=torch.int32) -> int:
@@ -54,27 +67,25 @@ def _ints(t: torch.Tensor, name: str, numel: Optional[int], device: int, dtype=t
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, heads: int, d: int, tokens: Optional[int], dtype, device: int):
+def _rows(t: torch.Tensor, name: str, heads: int, d: int, tokens: int, dtype, device: int):
     """(tokens, heads, d) with any strides over tokens and heads."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != d or (tokens is not None and t.shape[0] != tokens) or t.dtype is not dtype or t.get_device() != device:
-        raise ValueError(f"{name}: wants ({tokens if tokens is not None else 'tokens'}, {heads}, {d}) {dtype} on cuda:{device}, got {tuple(t.shape)} "
-                         f"{t.dtype} on {t.device}")
     st = t.stride()
-    if st[2] != 1:
-        raise ValueError(f"{name}: the last dimension has to be contiguous, strides {st}")
+    if t.shape != (tokens, heads, d) or st[2] != 1 or t.dtype is not dtype or t.get_device() != device:
+        _refuse(t, name, (tokens, heads, d), dtype, device)
     return t.data_ptr(), st[0], st[1]
 
 
-def _cache(t: torch.Tensor, name: str, heads: int, d: int, page_size: int, pages: Optional[int], dtype, device: int):
+def _cache(t: torch.Tensor, name: str, shape, dtype, device: int):
     """(n_pages, page_size, heads, d) with any strides over the first three."""
-    if (t.dim() != 4 or t.shape[1] != page_size or t.shape[2] != heads or t.shape[3] != d or (pages is not None and t.shape[0] != pages) or t.dtype is not dtype
-            or t.get_device() != device):
-        raise ValueError(f"{name}: wants ({pages if pages is not None else 'n_pages'}, {page_size}, {heads}, {d}) {dtype} on cuda:{device}, got "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
     st = t.stride()
-    if st[3] != 1:
-        raise ValueError(f"{name}: the last dimension has to be contiguous, strides {st}")
+    if t.shape != shape or st[3] != 1 or t.dtype is not dtype or t.get_device() != device:
+        _refuse(t, name, shape, dtype, device)
     return t.data_ptr(), st[0], st[1], st[2]
+
+
+def _pages_of(t: torch.Tensor, page_size: int, heads: int, d: int):
+    """The shape that a cache with as many pages as this one has."""
+    return (t.shape[0] if t.dim() == 4 else None, page_size, heads, d)
 
 
 class PagedPlan:
@@ -91,13 +102,14 @@ class PagedPlan:
     def __init__(self, max_requests: int, max_tokens: int, page_size: int, H_q: int, H_kv: int, d: int, max_new: Optional[int] = None, device="cuda"):
         self.lib = _lib.load()
         device = torch.device(device)
-        _want(device.type == "cuda", "PagedPlan: a CUDA device")
+        if device.type != "cuda":
+            raise ValueError(f"PagedPlan: a CUDA device, got {device}")
         self.device = device.index if device.index is not None else torch.cuda.current_device()
         self.max_requests, self.max_tokens, self.page_size = int(max_requests), int(max_tokens), int(page_size)
         self.H_q, self.H_kv, self.d = int(H_q), int(H_kv), int(d)
         self.max_new = min(int(max_new), self.max_tokens) if max_new is not None else self.max_tokens
         with torch.cuda.device(self.device):
-            n = int(self.lib.khq_b200_paged_schedule_bytes(self.max_requests, self.max_tokens, self.max_new, self.H_q, self.H_kv))
+            n = int(self.lib.khq_b200_paged_schedule_bytes(self.max_requests, self.max_tokens, self.max_new, self.H_q, self.H_kv, self.d))
             w = int(self.lib.khq_b200_paged_workspace_bytes(self.max_new, self.H_q, self.H_kv, self.d))
         if n == 0 or w == 0 or self.page_size not in (16, 32, 64, 128):
             raise ValueError(f"PagedPlan: max_requests={max_requests} max_tokens={max_tokens} max_new={max_new} page_size={page_size} H_q={H_q} H_kv={H_kv} d={d} "
@@ -108,7 +120,9 @@ class PagedPlan:
         self.info = torch.zeros(8, dtype=torch.int32, device=self.positions.device)
         self.schedule, self._workspace_bytes = empty(n, torch.uint8), w
         self.workspace = self.new_workspace()
+        self._scratch, self._schedule_bytes = (self.workspace.data_ptr(), w), n
         self.requests = self.max_pages = 0  # of the last build
+        self._fns = {dt: (getattr(self.lib, "launch_khq_paged_prestep_" + t), getattr(self.lib, "launch_khq_paged_attn_" + t)) for dt, t in _TYPES.items()}
         self._own = (self._cu_new.data_ptr(), self._kv_lens.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.info.data_ptr(),
                      self.schedule.data_ptr())
 
@@ -134,10 +148,9 @@ class PagedPlan:
         if not 0 < n <= self.max_requests:
             raise ValueError(f"PagedPlan.build: {n} requests, built for 1 to {self.max_requests}")
         ctx, new = _ints(ctx_lens, "ctx_lens", n, dev), _ints(new_lens, "new_lens", n, dev)
-        if (block_table.dim() != 2 or block_table.shape[0] != n or block_table.dtype is not torch.int32 or block_table.get_device() != dev
-                or block_table.shape[1] < 1 or block_table.stride(1) != 1):
-            raise ValueError(f"block_table: wants ({n}, max_pages) int32 on cuda:{dev} with contiguous rows, got {tuple(block_table.shape)} {block_table.dtype} "
-                             f"on {block_table.device}")
+        st, shape = block_table.stride(), block_table.shape
+        if len(shape) != 2 or shape[0] != n or shape[1] < 1 or st[1] != 1 or block_table.dtype is not torch.int32 or block_table.get_device() != dev:
+            _refuse(block_table, "block_table", (n, None), torch.int32, dev)
         fl = fc = fo = n_pages = 0
         if free_list is not None:
             if free_count is None:
@@ -147,11 +160,9 @@ class PagedPlan:
             fo = fc if free_count_out is None else _ints(free_count_out, "free_count_out", 1, dev)
         elif free_count is not None or free_count_out is not None:
             raise ValueError("PagedPlan.build: free_count without free_list")
-        max_pages = block_table.shape[1]
-        cu, kv, pos, slots, info, sched = self._own
-        packed = _PLAN_ARGS.pack(ctx, new, block_table.data_ptr(), fl, fc, fo, cu, kv, pos, slots, info, sched, self.schedule.numel(),
-                                 block_table.stride(0) if n > 1 else max_pages, n, max_pages, n_pages, self.page_size, self.max_tokens, self.max_new,
-                                 self.H_q, self.H_kv)
+        max_pages = shape[1]
+        packed = _PLAN_ARGS.pack(ctx, new, block_table.data_ptr(), fl, fc, fo, *self._own, self._schedule_bytes, st[0] if n > 1 else max_pages, n, max_pages,
+                                 n_pages, self.page_size, self.max_tokens, self.max_new, self.H_q, self.H_kv, self.d)
         _launch(self.lib.launch_khq_paged_plan, "launch_khq_paged_plan", packed, dev)
         self.requests, self.max_pages = n, max_pages
         return self
@@ -162,29 +173,33 @@ def paged_prestep(plan: PagedPlan, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, 
     """Head RMS norms of ``q`` and ``k`` (weights fp32 (d) or None), rotation of the first ``rotary_dim`` dims at the plan's positions; ``q``
     to ``q_out`` (which may be ``q``), rotated ``k``, ``v`` and, with ``u_cache``, un-rotated ``k`` to the plan's slots.  The
     counterpart of ``CudaOps.prestep`` for ragged rows and pages."""
-    dev, H_q, H_kv, d, dt = plan.device, plan.H_q, plan.H_kv, plan.d, q.dtype
-    if dt not in _TYPES:
+    dev, H_q, H_kv, d, P, dt = plan.device, plan.H_q, plan.H_kv, plan.d, plan.page_size, q.dtype
+    fns = plan._fns.get(dt)
+    if fns is None:
         raise TypeError(f"paged_prestep: fp16 or bf16, got {dt}")
     T = q.shape[0]
     if not 0 < T <= plan.max_tokens:
         raise ValueError(f"paged_prestep: {T} rows, the plan is for 1 to {plan.max_tokens}")
     if plan.requests == 0:
         raise ValueError("paged_prestep: the plan has not been built")
+    cache = _pages_of(k_cache, P, H_kv, d)
+    packed = _PRESTEP_ARGS.pack(*_prestep_pointers(plan, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, v_cache, u_cache, T, cache, dt, dev), T, cache[0], P,
+                                H_q, H_kv, d, rotary_dim, rope_theta, rms_eps)
+    _launch(fns[0], "launch_khq_paged_prestep_" + _TYPES[dt], packed, dev)
+
+
+def _prestep_pointers(plan, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, v_cache, u_cache, T, cache, dt, dev):
+    H_q, H_kv, d = plan.H_q, plan.H_kv, plan.d
     qp, q0, q1 = _rows(q, "q", H_q, d, T, dt, dev)
     kp, k0, k1 = _rows(k, "k", H_kv, d, T, dt, dev)
     vp, v0, v1 = _rows(v, "v", H_kv, d, T, dt, dev)
     op, o0, o1 = _rows(q_out, "q_out", H_q, d, T, dt, dev)
-    P = plan.page_size
-    kc, kc0, kc1, kc2 = _cache(k_cache, "k_cache", H_kv, d, P, None, dt, dev)
-    n_pages = k_cache.shape[0]
-    vc, vc0, vc1, vc2 = _cache(v_cache, "v_cache", H_kv, d, P, n_pages, dt, dev)
-    uc, uc0, uc1, uc2 = _cache(u_cache, "u_cache", H_kv, d, P, n_pages, dt, dev) if u_cache is not None else (0, 0, 0, 0)
+    kc, kc0, kc1, kc2 = _cache(k_cache, "k_cache", cache, dt, dev)
+    vc, vc0, vc1, vc2 = _cache(v_cache, "v_cache", cache, dt, dev)
+    uc, uc0, uc1, uc2 = _cache(u_cache, "u_cache", cache, dt, dev) if u_cache is not None else (0, 0, 0, 0)
     qw = _ints(q_norm_w, "q_norm_w", d, dev, torch.float32) if q_norm_w is not None else 0
     kw = _ints(k_norm_w, "k_norm_w", d, dev, torch.float32) if k_norm_w is not None else 0
-    packed = _PRESTEP_ARGS.pack(qp, kp, vp, qw, kw, op, kc, vc, uc, plan._own[2], plan._own[3], q0, q1, k0, k1, v0, v1, o0, o1, kc0, kc1, kc2,
-                                vc0, vc1, vc2, uc0, uc1, uc2, T, n_pages, P, H_q, H_kv, d, int(rotary_dim), float(rope_theta), float(rms_eps))
-    name = "launch_khq_paged_prestep_" + _TYPES[dt]
-    _launch(getattr(plan.lib, name), name, packed, dev)
+    return (qp, kp, vp, qw, kw, op, kc, vc, uc, plan._own[2], plan._own[3], q0, q1, k0, k1, v0, v1, o0, o1, kc0, kc1, kc2, vc0, vc1, vc2, uc0, uc1, uc2)
 
 
 def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scale: float, gate=None, lse=None, workspace=None) -> None:
@@ -192,32 +207,29 @@ def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scal
     pre-step has run).  ``out`` (tokens, H_q, d); ``gate`` (tokens, H_q, d): logits of the output gate, as in
     ``CudaOps.gqa_prefill``; ``lse`` (tokens, H_q) fp32: log of the sum of exponentials.  ``q`` and ``gate`` may be the two halves of an
     interleaved projection."""
-    dev, H_q, H_kv, d, dt = plan.device, plan.H_q, plan.H_kv, plan.d, q.dtype
-    if dt not in _TYPES:
+    dev, H_q, H_kv, d, P, dt = plan.device, plan.H_q, plan.H_kv, plan.d, plan.page_size, q.dtype
+    fns = plan._fns.get(dt)
+    if fns is None:
         raise TypeError(f"paged_attention: fp16 or bf16, got {dt}")
-    T = q.shape[0]
+    T, B, M = q.shape[0], plan.requests, plan.max_pages
     if not 0 < T <= plan.max_tokens:
         raise ValueError(f"paged_attention: {T} rows, the plan is for 1 to {plan.max_tokens}")
-    if plan.requests == 0:
+    if B == 0:
         raise ValueError("paged_attention: the plan has not been built")
     qp, q0, q1 = _rows(q, "q", H_q, d, T, dt, dev)
     op, o0, o1 = _rows(out, "out", H_q, d, T, dt, dev)
     gp, g0, g1 = _rows(gate, "gate", H_q, d, T, dt, dev) if gate is not None else (0, 0, 0)
-    P = plan.page_size
-    kc, kc0, kc1, kc2 = _cache(k_cache, "k_cache", H_kv, d, P, None, dt, dev)
-    n_pages = k_cache.shape[0]
-    vc, vc0, vc1, vc2 = _cache(v_cache, "v_cache", H_kv, d, P, n_pages, dt, dev)
-    if (block_table.dim() != 2 or block_table.shape[0] != plan.requests or block_table.shape[1] != plan.max_pages or block_table.dtype is not torch.int32
-            or block_table.get_device() != dev or block_table.stride(1) != 1):
-        raise ValueError(f"block_table: wants the plan's ({plan.requests}, {plan.max_pages}) int32 on cuda:{dev}, got {tuple(block_table.shape)} "
-                         f"{block_table.dtype} on {block_table.device}")
+    cache = _pages_of(k_cache, P, H_kv, d)
+    kc, kc0, kc1, kc2 = _cache(k_cache, "k_cache", cache, dt, dev)
+    vc, vc0, vc1, vc2 = _cache(v_cache, "v_cache", cache, dt, dev)
+    st = block_table.stride()
+    if block_table.shape != (B, M) or st[1] != 1 or block_table.dtype is not torch.int32 or block_table.get_device() != dev:
+        _refuse(block_table, "block_table (the plan's)", (B, M), torch.int32, dev)
     lp = _ints(lse, "lse", T * H_q, dev, torch.float32) if lse is not None else 0
     if workspace is None:
-        workspace = plan.workspace
-    ws = _ints(workspace, "workspace", None, dev, torch.uint8)
-    packed = _ATTN_ARGS.pack(qp, gp, kc, vc, block_table.data_ptr(), plan._own[5], op, lp, ws, plan.schedule.numel(),
-                             workspace.numel(), q0, q1, g0, g1, o0, o1, kc0, kc1, kc2, vc0, vc1, vc2,
-                             block_table.stride(0) if plan.requests > 1 else plan.max_pages, T, plan.max_tokens, plan.max_new, plan.requests, plan.max_pages,
-                             n_pages, P, H_q, H_kv, d, float(scale))
-    name = "launch_khq_paged_attn_" + _TYPES[dt]
-    _launch(getattr(plan.lib, name), name, packed, dev)
+        ws, n_ws = plan._scratch
+    else:
+        ws, n_ws = _ints(workspace, "workspace", None, dev, torch.uint8), workspace.numel()
+    packed = _ATTN_ARGS.pack(qp, gp, kc, vc, block_table.data_ptr(), plan._own[5], op, lp, ws, plan._schedule_bytes, n_ws, q0, q1, g0, g1, o0, o1,
+                             kc0, kc1, kc2, vc0, vc1, vc2, st[0] if B > 1 else M, T, plan.max_tokens, plan.max_new, B, M, cache[0], P, H_q, H_kv, d, scale)
+    _launch(fns[1], "launch_khq_paged_attn_" + _TYPES[dt], packed, dev)

@@ -381,9 +381,9 @@ typedef struct khq_paged_plan_args {
     void *free_count_out, *cu_new, *kv_lens, *positions, *slots, *info, *schedule;
     size_t schedule_bytes;
     long long table_stride;
-    int32_t requests, max_pages, n_pages, page_size, max_tokens, max_new, H_q, H_kv;
+    int32_t requests, max_pages, n_pages, page_size, max_tokens, max_new, H_q, H_kv, d;
 } khq_paged_plan_args;
-size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, int H_q, int H_kv); /* 0: bad arguments */
+size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, int H_q, int H_kv, int d); /* 0: bad arguments */
 int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream_t stream);
 
 /* The pre-step of `tokens` rows: head RMS norms of q and k (fp32 weights of d, or NULL), rotation of the pairs (i, i + rotary_dim / 2) of the first
@@ -408,7 +408,7 @@ int launch_khq_paged_prestep_bf16(const khq_paged_prestep_args* args, khq_stream
  * and, unless lse is NULL, lse[t,h] = log sum_u exp(q . K * scale) (tokens, H_q) fp32.  Softmax statistics, weights' sums and outputs in fp32;
  * the weights enter the product with V as 16-bit values.  A row that attends nothing (no page of it could be had) gets out 0 and lse
  * -inf.  Stale cache rows behind a request's last token are not attended, whatever they hold, NaN included.  schedule is
- * a plan's, max_tokens, max_new, requests, page_size and the head counts the same as there; `tokens` rows of q, gate,
+ * a plan's, max_tokens, max_new, requests, page_size, d and the head counts the same as there; `tokens` rows of q, gate,
  * out and lse exist (the plan must not have more).  Page numbers outside 0..n_pages-1 are not attended.  Rows behind the plan's last are left alone.
  * scale > 0.  workspace: khq_b200_paged_workspace_bytes(...) at 256 bytes; calls that may run at the same time need their own.  Returns -100, -103,
  * -104, -105, -107 / -108 (no tensor map). */

@@ -19,7 +19,7 @@ def lib():
 
 PLAN = [("ctx_lens", P), ("new_lens", P), ("block_table", P), ("free_list", P), ("free_count", P), ("free_count_out", P), ("cu_new", P), ("kv_lens", P),
         ("positions", P), ("slots", P), ("info", P), ("schedule", P), ("schedule_bytes", 1 << 40), ("table_stride", 9), ("requests", 3), ("max_pages", 9),
-        ("n_pages", 40), ("page_size", 16), ("max_tokens", 64), ("max_new", 64), ("H_q", 24), ("H_kv", 4)]
+        ("n_pages", 40), ("page_size", 16), ("max_tokens", 64), ("max_new", 64), ("H_q", 24), ("H_kv", 4), ("d", 256)]
 PRESTEP = ([(n, P) for n in ("q", "k", "v", "q_norm_w", "k_norm_w", "q_out", "k_cache", "v_cache", "u_cache", "positions", "slots")]
            + [(n, 256) for n in ("q0", "q1", "k0", "k1", "v0", "v1", "o0", "o1", "kc0", "kc1", "kc2", "vc0", "vc1", "vc2", "uc0", "uc1", "uc2")]
            + [("tokens", 5), ("n_pages", 4), ("page_size", 16), ("H_q", 24), ("H_kv", 4), ("d", 256), ("rotary_dim", 64), ("rope_theta", 1e7), ("rms_eps", 1e-6)])
@@ -53,7 +53,7 @@ def test_layouts_are_the_structs(tmp_path):
 @pytest.mark.parametrize("change,code", [
     (dict(requests=0), -100), (dict(max_tokens=0), -100), (dict(max_new=-1), -100), (dict(max_pages=0), -100), (dict(ctx_lens=0), -100),
     (dict(slots=0), -100), (dict(schedule=0), -100), (dict(free_count=0), -100), (dict(free_count_out=0), -100), (dict(n_pages=0), -100),
-    (dict(free_list=0), -100), (dict(page_size=17), -103), (dict(page_size=0), -103), (dict(H_q=25), -103), (dict(requests=16385), -103),
+    (dict(free_list=0), -100), (dict(page_size=17), -103), (dict(page_size=0), -103), (dict(H_q=25), -103), (dict(d=64), -103), (dict(requests=16385), -103),
     (dict(max_tokens=(1 << 20) + 1), -103), (dict(table_stride=8), -103), (dict(max_pages=1 << 27, table_stride=1 << 27), -103),
     (dict(ctx_lens=P + 2), -104), (dict(slots=P + 4), -104), (dict(schedule=P + 8), -104), (dict(schedule_bytes=64), -105),
 ])
@@ -91,11 +91,11 @@ def test_null_arguments(lib):
 
 
 def test_sizes(lib):
-    assert lib.khq_b200_paged_schedule_bytes(0, 8, 8, 24, 4) == 0
-    assert lib.khq_b200_paged_schedule_bytes(2, 8, 8, 24, 5) == 0
+    assert lib.khq_b200_paged_schedule_bytes(0, 8, 8, 24, 4, 256) == 0
+    assert lib.khq_b200_paged_schedule_bytes(2, 8, 8, 24, 5, 256) == 0
     assert lib.khq_b200_paged_workspace_bytes(1, 24, 4, 64) == 0
     for requests, tokens, new in ((1, 1, 1), (3, 4096, 2048), (16384, 1 << 20, 1 << 20)):
-        n = lib.khq_b200_paged_schedule_bytes(requests, tokens, new, 24, 4)
+        n = lib.khq_b200_paged_schedule_bytes(requests, tokens, new, 24, 4, 256)
         assert n > 16 * requests
         w = lib.khq_b200_paged_workspace_bytes(new, 24, 4, 256)
         assert w > 0 and w % 256 == 0

@@ -285,6 +285,14 @@ def test_attention_chunks_between_decodes(cuda_ops, H_q, H_kv, d, page):
         attend("bf16", H_q, H_kv, d, page, ctx, new, max_new=300, seed=len(ctx))
 
 
+@pytest.mark.parametrize("H_q,H_kv,d", [(24, 4, 256), (20, 4, 128)])
+def test_attention_few_and_many_rows_in_turn(cuda_ops, H_q, H_kv, d):
+    """Tiles with one, some and all of their rows in use, one after the other in the same CTAs."""
+    rng = random.Random(7)
+    rows = [(rng.randint(0, 600), rng.choice([4, 5, 7, 9, 12, 16, 21, 22, 30, 43, 70])) for _ in range(300)]
+    attend("fp16", H_q, H_kv, d, 32, [c for c, _ in rows], [n for _, n in rows], seed=21)
+
+
 def test_attention_long_contexts_shared(cuda_ops):
     """Few requests over long contexts: every segment is shared by many CTAs."""
     attend("fp16", 24, 4, 256, 128, [40000], [30], seed=1)
