@@ -143,73 +143,68 @@ __device__ __forceinline__ int record_worker(const Meta& m, int begins_in, int i
     return m.first < 0 ? begins_in + i : ((m.first + i + 1) * workers - 1) / m.total;
 }
 
-// Joins the records of the segment that begins in CTA blockIdx.x of the decode kernel and goes on in the next ones; rows blockIdx.y, + gridDim.y, ..
+// Joins row blockIdx.y of the records of the segment that begins in CTA blockIdx.x of the decode kernel and goes on in the next ones.
 // A CTA's record 1 is of the segment that begins in it, record 0 of one that it took over.  Groups of D / 4 threads take the records in
-// turn, 4 columns a thread.
+// turn, 4 columns a thread.  Latency bounds it (one token over 4001: 37 records a row): a row per CTA, and the first records are on their way while
+// their factors are formed.
 constexpr int MERGE_THREADS = 256;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Params p, int record_floats, int workers) {
-    constexpr int PER_ROW = D / 4, GROUPS = MERGE_THREADS / PER_ROW, ROWS = DECODE_ROWS;
+    constexpr int PER_ROW = D / 4, GROUPS = MERGE_THREADS / PER_ROW, AHEAD = 6;
     __shared__ float factor[MAX_WORKERS];
-    __shared__ int base[MAX_WORKERS];
     __shared__ float4 sums[GROUPS][PER_ROW];
     khq::pdl_wait();
     khq::pdl_trigger();
     const Meta meta = read_meta(p.meta + blockIdx.x);
-    const int n = meta.n, tid = threadIdx.x, lane = tid & 31;
-    if (n == 0) return;
-    const int R = meta.ntok * p.n_rep;
-    for (int i = tid; i < n; i += MERGE_THREADS) base[i] = 2 * record_worker(meta, blockIdx.x, i, workers) + (i == 0);
+    const int n = meta.n, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+    if (n == 0 || r >= meta.ntok * p.n_rep) return;
+    const auto record = [&](int i) { return p.records + (2LL * record_worker(meta, blockIdx.x, i, workers) + (i == 0)) * record_floats; };
     const int col = tid % PER_ROW, group = tid / PER_ROW;
-    for (int r = blockIdx.y; r < R; r += gridDim.y) {
-        __syncthreads();
-        // every warp for itself: the row's maximum, its sum, and each record's factor
-        float2 ml[MAX_WORKERS / 32];
-        float M = -INFINITY, L = 0.0f;
+    float4 a[AHEAD];
 #pragma unroll
-        for (int k = 0; k < MAX_WORKERS / 32; ++k) {
-            const int i = k * 32 + lane;
-            ml[k] = make_float2(-INFINITY, 0.0f);
-            if (i < n) ml[k] = *reinterpret_cast<const float2*>(p.records + (long long)base[i] * record_floats + ROWS * D + 2 * r);
-            M = fmaxf(M, ml[k].x);
-        }
+    for (int k = 0; k < AHEAD; ++k)
+        if (group + k * GROUPS < n) a[k] = *reinterpret_cast<const float4*>(record(group + k * GROUPS) + r * D + col * 4);
+    // every warp for itself: the row's maximum, its sum, and each record's factor
+    float2 ml[MAX_WORKERS / 32];
+    float M = -INFINITY, L = 0.0f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-#pragma unroll
-        for (int k = 0; k < MAX_WORKERS / 32; ++k) {
-            const int i = k * 32 + lane;
-            const float f = ml[k].x == -INFINITY ? 0.0f : exp2f(ml[k].x - M);
-            L += ml[k].y * f;
-            if (tid < 32 && i < n) factor[i] = f;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
-        __syncthreads();
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int i = group; i < n; i += GROUPS) {
-            const float4 a = *reinterpret_cast<const float4*>(p.records + (long long)base[i] * record_floats + r * D + col * 4);
-            const float f = factor[i];
-            acc.x += a.x * f;
-            acc.y += a.y * f;
-            acc.z += a.z * f;
-            acc.w += a.w * f;
-        }
-        sums[group][col] = acc;
-        __syncthreads();
-        const int t = (r * p.rep_mul) >> 16, row = meta.row0 + t, head = meta.h * p.n_rep + (r - t * p.n_rep);
-        if (group != 0 || row >= p.tokens) continue;
-#pragma unroll
-        for (int g = 1; g < GROUPS; ++g) {
-            const float4 a = sums[g][col];
-            acc.x += a.x;
-            acc.y += a.y;
-            acc.z += a.z;
-            acc.w += a.w;
-        }
-        store_out<BF16>(p, row, head, col * 4, acc, L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L);
-        if (p.lse && col == 0) p.lse[(long long)row * p.H_q + head] = (M + log2f(L)) * 0.6931471805599453f;
+    for (int k = 0; k < MAX_WORKERS / 32; ++k) {
+        const int i = k * 32 + lane;
+        ml[k] = i < n ? *reinterpret_cast<const float2*>(record(i) + DECODE_ROWS * D + 2 * r) : make_float2(-INFINITY, 0.0f);
+        M = fmaxf(M, ml[k].x);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+#pragma unroll
+    for (int k = 0; k < MAX_WORKERS / 32; ++k) {
+        const int i = k * 32 + lane;
+        const float f = ml[k].x == -INFINITY ? 0.0f : ex2_approx(ml[k].x - M);
+        L += ml[k].y * f;
+        if (tid < 32 && i < n) factor[i] = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
+    __syncthreads();
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](const float4& x, float f) {
+        acc.x += x.x * f;
+        acc.y += x.y * f;
+        acc.z += x.z * f;
+        acc.w += x.w * f;
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+        if (group + k * GROUPS < n) add(a[k], factor[group + k * GROUPS]);
+#pragma unroll 8
+    for (int i = group + AHEAD * GROUPS; i < n; i += GROUPS) add(*reinterpret_cast<const float4*>(record(i) + r * D + col * 4), factor[i]);
+    sums[group][col] = acc;
+    __syncthreads();
+    const int t = (r * p.rep_mul) >> 16, row = meta.row0 + t, head = meta.h * p.n_rep + (r - t * p.n_rep);
+    if (group != 0 || row >= p.tokens) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) add(sums[g][col], 1.0f);
+    store_out<BF16>(p, row, head, col * 4, acc, L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L);
+    if (p.lse && col == 0) p.lse[(long long)row * p.H_q + head] = (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace khq_paged
@@ -359,7 +354,8 @@ int launch_kernels(const khq_paged_attn_args& a, Params p, const Schedule& sched
         if (err != cudaSuccess) return static_cast<int>(err);
     }
     if (sched.decodes) {
-        err = launch_merge(khq_paged_merge_kernel<D, BF16>, dim3((unsigned)w.ctas, 4, 1), MERGE_THREADS, stream, p, (int)decode::Shape<D>::RECORD, w.ctas);
+        const int rows = (a.max_new < sched.decode_tokens ? a.max_new : sched.decode_tokens) * p.n_rep;  // of a request, at most
+        err = launch_merge(khq_paged_merge_kernel<D, BF16>, dim3((unsigned)w.ctas, (unsigned)rows, 1), MERGE_THREADS, stream, p, (int)decode::Shape<D>::RECORD, w.ctas);
         if (err != cudaSuccess) return static_cast<int>(err);
     }
     return 0;
