@@ -222,29 +222,60 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
             a.schedule[2 * rank + 1] = blocks;
         }
         __syncthreads();
-        // each worker's stretch of the blocks of all kv heads
-        const int over = decodes ? 0 : CHUNK_OVER, workers = decodes ? a.workers : a.workers / 2;
+        // Each worker's stretch of the blocks of all kv heads: equal ones, but that an end which falls into an item's first or last `snap` blocks
+        // goes to the item's.  No more workers than blocks, so that every worker between an item's first and last has some of it.
+        const int over = decodes ? 0 : CHUNK_OVER, snap = decodes ? 0 : CHUNK_SNAP;
         const long long per_head = blocks + (long long)items * over, total = per_head * a.H_kv;
+        const int workers = (int)min((long long)(decodes ? a.workers : a.workers / 2), total);
         Start* const starts = reinterpret_cast<Start*>(a.schedule + (decodes ? a.sched.decode_starts : a.sched.chunk_starts));
-        if (tid < workers) {
-            Start st = {};
-            const long long w = tid * total / workers, hi = (tid + 1) * total / workers;
-            if (w < hi) {
-                st.h = (int)(w / per_head);
-                const int r = (int)(w % per_head);
-                int lo = 0, up = items;  // the last item that begins at r or in front
-                while (up - lo > 1) {
-                    const int mid = (lo + up) >> 1;
-                    if (cum[mid] + mid * over <= r) lo = mid;
-                    else up = mid;
+        struct Cut {
+            int item, h, off, n;  // position `off` of the item, its blocks (off 0: where it begins)
+            long long at;
+        };
+        const auto cut = [&](int k) {
+            const long long v = k * total / workers;
+            Cut c = {0, (int)(v / per_head), 0, 0, v};
+            if (v == total) return c;
+            const int r = (int)(v % per_head);
+            int lo = 0, up = items;  // the last item that begins at r or in front
+            while (up - lo > 1) {
+                const int mid = (lo + up) >> 1;
+                if (cum[mid] + mid * over <= r) lo = mid;
+                else up = mid;
+            }
+            c.item = lo;
+            c.n = (lo + 1 < items ? cum[lo + 1] : blocks) - cum[lo];
+            c.off = r - cum[lo] - lo * over;
+            const int blk = max(c.off - over, 0), rest = c.n - blk;
+            if (blk == 0 || (blk < snap && blk <= rest)) {
+                c.at -= c.off;
+                c.off = 0;
+            } else if (rest < snap) {
+                c.at += rest;
+                c.off = 0;
+                if (++c.item == items) {
+                    c.item = 0;
+                    ++c.h;
                 }
-                const int off = r - cum[lo] - lo * over;
-                st.it = list[lo];
-                st.item = lo;
-                st.blk = max(off - over, 0);
-                st.n_items = items;
-                st.begins = w - off;
-                st.hi = hi;
+            }
+            return c;
+        };
+        if (tid < (decodes ? a.workers : a.workers / 2)) {
+            Start st = {};
+            if (tid < workers) {
+                const Cut from = cut(tid), to = cut(tid + 1);
+                if (from.at < to.at) {
+                    st.it = list[from.item];
+                    st.item = from.item;
+                    st.h = from.h;
+                    st.blk = max(from.off - over, 0);
+                    st.n_items = items;
+                    st.begins = from.at - from.off;
+                    st.length = (int)(to.at - st.begins);
+                    // the first cut behind the item's last undivided block ends it
+                    const long long end = to.at - to.off + over + (snap > 0 ? to.n - snap + 1 : to.n);
+                    if (to.off > 0) st.share = (int)((end * workers + total - 1) / total) - tid;
+                }
             }
             starts[tid] = st;
         }
@@ -464,9 +495,9 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
     if ((reinterpret_cast<uintptr_t>(p.slots) & 7) != 0 || (reinterpret_cast<uintptr_t>(p.schedule) & 15) != 0) return -104;
     const Schedule sched = schedule_of(p.requests, p.max_tokens, p.max_new, p.H_q, p.H_kv, p.d);
     if (p.schedule_bytes < (size_t)sched.ints * 4) return -105;
-    // the key blocks of all items are counted in 32 bits
+    // the key blocks of all items and kv heads are counted in 32 bits
     const long long row = ((long long)p.max_pages << shift) + p.max_tokens;
-    if (sched.chunk_cap * (row / TILE_KEYS + 1 + CHUNK_OVER) > 0x7FFFFFFFLL || sched.decode_cap * (row / sched.decode_keys + 1) > 0x7FFFFFFFLL) return -103;
+    if (sched.chunk_cap * (row / TILE_KEYS + 1 + CHUNK_OVER) > 0x7FFFFFFFLL / p.H_kv || sched.decode_cap * (row / sched.decode_keys + 1) > 0x7FFFFFFFLL / p.H_kv) return -103;
     PlanArgs a;
     a.ctx_lens = static_cast<const int*>(p.ctx_lens);
     a.new_lens = static_cast<const int*>(p.new_lens);

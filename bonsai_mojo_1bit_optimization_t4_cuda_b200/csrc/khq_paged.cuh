@@ -17,7 +17,8 @@ constexpr int ITEM_INTS = sizeof(Item) / 4;
 struct alignas(16) Start {
     Item it;
     int item, h, blk, n_items;  // blk: the item's first block in the stretch
-    long long begins, hi;       // where the item begins in the row of all blocks, the stretch's end (0: nothing to do)
+    long long begins;           // where the item begins in the row of all blocks
+    int length, share;          // from there to the stretch's end (0: nothing to do); the workers from this one on that share the item it ends in
 };
 constexpr int START_INTS = sizeof(Start) / 4, MAX_WORKERS = 256;
 static_assert(START_INTS == 16, "four 16-byte loads");
@@ -28,8 +29,9 @@ static_assert(START_INTS == 16, "four 16-byte loads");
 constexpr int MAX_REP = 128;  // query heads of a kv head
 constexpr int DECODE_ROWS = 16, TILE_ROWS = 128, TILE_KEYS = 128;
 constexpr int decode_keys(int d) { return 64 * 256 / d; }  // keys of a block of the decode kernel: 64 KB of K and V
-// What a tile costs beside its key blocks, in blocks: its queries, gates and outputs, and the pipe's run-in.
-constexpr int CHUNK_OVER = 3;
+// What a tile costs beside its key blocks, in blocks: its queries, gates and outputs, and the pipe's run-in.  And how near to an item's ends its
+// blocks are not divided between two pairs: 264 KB of partial rows from each of them would have to be written and read again.
+constexpr int CHUNK_OVER = 3, CHUNK_SNAP = 4;
 struct Schedule {
     bool chunks, decodes;             // the lists that the step can have
     int tile_tokens, decode_tokens;   // new tokens of a tile; the most of a request for the decode kernel (0: none)

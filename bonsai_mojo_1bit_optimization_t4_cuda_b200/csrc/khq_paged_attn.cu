@@ -46,9 +46,9 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* st
 }
 
 // By worker: how many records there are of the segment which begins in it and goes on in the next ones (0: none), and what joining them needs.
+// Record 1 of a worker is of the segment that begins in it, record 0 of one that it took over.
 struct alignas(16) Meta {
     int n, h, row0, ntok;
-    int first, total, pad[2];  // with fewer blocks than workers: the segment's first block, the blocks; else first is -1
 };
 
 struct Params {
@@ -80,10 +80,9 @@ __device__ __forceinline__ void load_segment(const Params& p, Segment& s) {
     s.pos0 = y.y;
 }
 // The worker's first segment; false: none.
-__device__ __forceinline__ bool first_segment(const Params& p, int worker, Segment& s, int& n_items, long long& begins, long long& hi) {
+__device__ __forceinline__ bool first_segment(const Params& p, int worker, Segment& s, int& n_items, int& length, int& share) {
     const int4* at = reinterpret_cast<const int4*>(p.starts + worker);
-    const int4 x = at[0], y = at[1], z = at[2];  // (ordinary loads: nothing else keeps them behind the wait for the plan)
-    const longlong2 w = *reinterpret_cast<const longlong2*>(at + 3);
+    const int4 x = at[0], y = at[1], z = at[2], w = at[3];  // (ordinary loads: nothing else keeps them behind the wait for the plan)
     s.b = x.x;
     s.n_blocks = x.y;
     s.ntok = x.z;
@@ -94,9 +93,9 @@ __device__ __forceinline__ bool first_segment(const Params& p, int worker, Segme
     s.h = z.y;
     s.blk = z.z;
     n_items = z.w;
-    begins = w.x;
-    hi = w.y;
-    return hi > 0;
+    length = w.z;
+    share = w.w;
+    return length > 0;
 }
 // Every item has a key block at least (its own tokens).
 __device__ __forceinline__ void next_segment(const Params& p, int n_items, Segment& s) {
@@ -125,40 +124,19 @@ __device__ __forceinline__ void store_out(const Params& p, int row, int head, in
     *reinterpret_cast<uint2*>(p.out + row * p.o_ts + head * p.o_hs + c) = make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
 }
 
-// Who shares a segment of blocks [seg_lo, seg_hi) that begins with worker `first`: the workers whose stretch has blocks of it.  (With fewer blocks than workers some
-// have none.)
-__device__ __forceinline__ void write_meta(Meta* meta, long long seg_lo, long long seg_hi, long long total, int first, int workers, const Segment& s) {
-    const bool all = total >= workers;
-    int4* const at = reinterpret_cast<int4*>(meta + first);
-    at[0] = make_int4(all ? (int)((seg_hi * workers - 1) / total) - first + 1 : (int)(seg_hi - seg_lo), s.h, s.row0, s.ntok);
-    at[1] = make_int4(all ? -1 : (int)seg_lo, all ? 0 : (int)total, 0, 0);
-}
-__device__ __forceinline__ Meta read_meta(const Meta* meta) {
-    const int4* at = reinterpret_cast<const int4*>(meta);
-    const int4 x = at[0], y = at[1];
-    return Meta{x.x, x.y, x.z, x.w, y.x, y.y, {0, 0}};
-}
-// The worker of the segment's i-th record.
-__device__ __forceinline__ int record_worker(const Meta& m, int begins_in, int i, int workers) {
-    return m.first < 0 ? begins_in + i : ((m.first + i + 1) * workers - 1) / m.total;
-}
-
-// Joins row blockIdx.y of the records of the segment that begins in CTA blockIdx.x of the decode kernel and goes on in the next ones.
-// A CTA's record 1 is of the segment that begins in it, record 0 of one that it took over.  Groups of D / 4 threads take the records in
-// turn, 4 columns a thread.  Latency bounds it (one token over 4001: 37 records a row): a row per CTA, and the first records are on their way while
-// their factors are formed.
+// Joins row r of the records of the segment that begins in CTA `worker` of the decode kernel and goes on in the next ones.  Groups of D / 4 threads take the
+// records in turn, 4 columns a thread.  Latency bounds it (one token over 4001: 37 records a row): a row per CTA, and the first records are on
+// their way while their factors are formed.
 constexpr int MERGE_THREADS = 256;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Params p, int record_floats, int workers) {
+__device__ __forceinline__ void merge_decode(const Params& p, int record_floats, int worker, int r) {
     constexpr int PER_ROW = D / 4, GROUPS = MERGE_THREADS / PER_ROW, AHEAD = 6;
     __shared__ float factor[MAX_WORKERS];
     __shared__ float4 sums[GROUPS][PER_ROW];
-    khq::pdl_wait();
-    khq::pdl_trigger();
-    const Meta meta = read_meta(p.meta + blockIdx.x);
-    const int n = meta.n, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-    if (n == 0 || r >= meta.ntok * p.n_rep) return;
-    const auto record = [&](int i) { return p.records + (2LL * record_worker(meta, blockIdx.x, i, workers) + (i == 0)) * record_floats; };
+    const int4 meta = *reinterpret_cast<const int4*>(p.meta + worker);
+    const int n = meta.x, tid = threadIdx.x, lane = tid & 31;
+    if (n == 0 || r >= meta.w * p.n_rep) return;
+    const auto record = [&](int i) { return p.records + (2LL * (worker + i) + (i == 0)) * record_floats; };
     const int col = tid % PER_ROW, group = tid / PER_ROW;
     float4 a[AHEAD];
 #pragma unroll
@@ -199,7 +177,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Pa
     for (int i = group + AHEAD * GROUPS; i < n; i += GROUPS) add(*reinterpret_cast<const float4*>(record(i) + r * D + col * 4), factor[i]);
     sums[group][col] = acc;
     __syncthreads();
-    const int t = (r * p.rep_mul) >> 16, row = meta.row0 + t, head = meta.h * p.n_rep + (r - t * p.n_rep);
+    const int t = (r * p.rep_mul) >> 16, row = meta.z + t, head = meta.y * p.n_rep + (r - t * p.n_rep);
     if (group != 0 || row >= p.tokens) return;
 #pragma unroll
     for (int g = 1; g < GROUPS; ++g) add(sums[g][col], 1.0f);
@@ -211,6 +189,21 @@ __global__ void __launch_bounds__(MERGE_THREADS) khq_paged_merge_kernel(const Pa
 
 #include "khq_paged_decode.cuh"
 #include "khq_paged_tile.cuh"
+
+namespace khq_paged {
+
+// The records of both kernels: the first `chunk_ctas` CTAs those of the chunk kernel, the others the decode kernel's.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(MERGE_THREADS)
+khq_paged_merge_kernel(const __grid_constant__ Params chunk, const __grid_constant__ Params dec, int chunk_ctas, int rows) {
+    khq::pdl_wait();
+    khq::pdl_trigger();
+    const int cta = blockIdx.x;
+    if (cta < chunk_ctas) tile::merge_chunk<D, BF16>(chunk, cta / tile::MERGE_CTAS, cta % tile::MERGE_CTAS);
+    else merge_decode<D, BF16>(dec, decode::Shape<D>::RECORD, (cta - chunk_ctas) / rows, (cta - chunk_ctas) % rows);
+}
+
+}  // namespace khq_paged
 
 // ---- host side -----------------------------------------------------------------------------------
 namespace {
@@ -283,20 +276,6 @@ Work work_of(const Schedule& sched, int d) {
     return w;
 }
 
-template <typename... Params_>
-cudaError_t launch_merge(void (*kernel)(Params_...), dim3 grid, unsigned threads, cudaStream_t stream, Params_... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads, 1, 1);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Both kernels' shared memory, once per device.
 template <int D, bool BF16>
 int prepare_kernels() {
@@ -348,16 +327,20 @@ int launch_kernels(const khq_paged_attn_args& a, Params p, const Schedule& sched
                               (unsigned)(decode::WARPS * 32), mk, mv, p, (int)sched.chunks);
         if (err != cudaSuccess) return static_cast<int>(err);
     }
-    if (sched.chunks) {
-        constexpr int parts = 16;
-        err = launch_merge(tile::khq_paged_tile_merge_kernel<D, BF16>, dim3((unsigned)w.pairs, 2 * parts, 1), tile::BR, stream, chunk, w.pairs, parts);
-        if (err != cudaSuccess) return static_cast<int>(err);
-    }
-    if (sched.decodes) {
-        const int rows = (a.max_new < sched.decode_tokens ? a.max_new : sched.decode_tokens) * p.n_rep;  // of a request, at most
-        err = launch_merge(khq_paged_merge_kernel<D, BF16>, dim3((unsigned)w.ctas, (unsigned)rows, 1), MERGE_THREADS, stream, p, (int)decode::Shape<D>::RECORD, w.ctas);
-        if (err != cudaSuccess) return static_cast<int>(err);
-    }
+    // rows of a request for the decode kernel, at most
+    const int rows = (a.max_new < sched.decode_tokens ? a.max_new : sched.decode_tokens) * p.n_rep;
+    const int chunk_ctas = sched.chunks ? w.pairs * tile::MERGE_CTAS : 0, decode_ctas = sched.decodes ? w.ctas * rows : 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(chunk_ctas + decode_ctas), 1, 1);
+    cfg.blockDim = dim3(MERGE_THREADS, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    err = cudaLaunchKernelEx(&cfg, khq_paged_merge_kernel<D, BF16>, chunk, p, chunk_ctas, rows);
+    if (err != cudaSuccess) return static_cast<int>(err);
     return 0;
 }
 

@@ -78,15 +78,14 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 
     // ---- this CTA's stretch of the key blocks ------------------------------------------------------
     Segment in, cur;  // where the loads and where the products are
-    int n_items;
-    long long begins, hi;
-    const bool work = first_segment(p, blockIdx.x, in, n_items, begins, hi);
+    int n_items, length, share;
+    const bool work = first_segment(p, blockIdx.x, in, n_items, length, share);
     if (tid == 0) p.meta[blockIdx.x].n = 0;  // overwritten below if a segment goes on in the next CTA
     if (!work) {
         if (beside) khq::pdl_wait();
         return;
     }
-    const int blocks = (int)(hi - begins) - in.blk;  // of the stretch, which begins at begins + in.blk
+    const int blocks = length - in.blk;  // of the stretch
     cur = in;
     uint64_t* const bar = bars + warp * S::STAGES;
     const uint32_t ring = smem_u32(smem) + warp * S::STAGES * 2 * S::PIECE;
@@ -276,7 +275,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         const bool ends = cur.blk + 1 == cur.n_blocks;
         if (ends || w + 1 == blocks) {
             // ---- join the warps ----------------------------------------------------------------------
-            const int seg_lo = w - cur.blk, seg_hi = seg_lo + cur.n_blocks;  // from the stretch's begin
+            const int seg_lo = w - cur.blk;  // from the stretch's begin
             const bool whole = seg_lo >= 0 && ends;
             float* const join = reinterpret_cast<float*>(smem + S::OFF_JOIN);
             float2* const ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
@@ -337,10 +336,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 }
                 __syncthreads();
             }
-            if (tid == 0 && seg_lo >= 0 && !ends) {
-                const long long lo = p.starts[blockIdx.x].begins + p.starts[blockIdx.x].blk;
-                write_meta(p.meta, lo + seg_lo, lo + seg_hi, (long long)p.schedule[3] * p.H_kv, blockIdx.x, gridDim.x, cur);
-            }
+            if (tid == 0 && seg_lo >= 0 && !ends) *reinterpret_cast<int4*>(p.meta + blockIdx.x) = make_int4(share, cur.h, cur.row0, cur.ntok);
             fresh = true;
         }
         ++cur.blk;

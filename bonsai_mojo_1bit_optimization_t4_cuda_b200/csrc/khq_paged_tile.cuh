@@ -91,18 +91,18 @@ struct Pages {
 
 // The pair's segments one after the other, as every role walks them.  Positions count the CHUNK_OVER blocks in front of every item.
 struct Walk {
-    long long begins, hi;  // where the segment's item begins, the stretch's end
-    int n;                 // its blocks in this stretch
+    int left, share;  // from where the segment's item begins to the stretch's end; the pairs that share the item there
+    int n;            // its blocks in this stretch
     Segment s;
     __device__ __forceinline__ bool begin(const Params& p, int& n_items) {
-        if (!first_segment(p, blockIdx.x >> 1, s, n_items, begins, hi)) return false;
+        if (!first_segment(p, blockIdx.x >> 1, s, n_items, left, share)) return false;
         count();
         return n > 0;
     }
-    __device__ __forceinline__ void count() { n = (int)min((long long)s.n_blocks, hi - begins - CHUNK_OVER) - s.blk; }
-    __device__ __forceinline__ bool more() const { return begins + s.n_blocks + 2 * CHUNK_OVER < hi; }
+    __device__ __forceinline__ void count() { n = min(s.n_blocks, left - CHUNK_OVER) - s.blk; }
+    __device__ __forceinline__ bool more() const { return s.n_blocks + 2 * CHUNK_OVER < left; }
     __device__ __forceinline__ void step_to(const Segment& next) {
-        begins += s.n_blocks + CHUNK_OVER;
+        left -= s.n_blocks + CHUNK_OVER;
         s = next;
         count();
     }
@@ -600,8 +600,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 __syncwarp();
                 if (lane == 0) arrive_leader(&bars[B_OFREE]);
                 if (tid == 0 && rank == 0 && sg.blk == 0)  // it goes on in the next pairs
-                    write_meta(p.meta, walk.begins + CHUNK_OVER, walk.begins + CHUNK_OVER + sg.n_blocks, (p.schedule[1] + (long long)n_items * CHUNK_OVER) * p.H_kv,
-                               (int)(blockIdx.x >> 1), (int)(gridDim.x >> 1), sg);
+                    *reinterpret_cast<int4*>(p.meta + (blockIdx.x >> 1)) = make_int4(walk.share, sg.h, sg.row0, sg.ntok);
             }
             g0 = last + 1;
             if (more) walk.step_to(next);
@@ -615,34 +614,31 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "n"(TM_COLS) : "memory");
 }
 
-// Joins the records of the segment that begins in pair blockIdx.x of the chunk kernel and goes on in the next ones.  A thread takes a row;
-// blockIdx.y: the CTA of the pair and a part of its columns.
+// Joins the records of the segment that begins in pair `pair` of the chunk kernel and goes on in the next ones.  Two threads take a row of a CTA's 128
+// and 16 of its columns each; `part`: the CTA of the pair and the columns.
+constexpr int MERGE_CTAS = 16;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(BR) khq_paged_tile_merge_kernel(const Params p, int pairs, int parts) {
+__device__ __forceinline__ void merge_chunk(const Params& p, int pair, int part) {
     using S = Shape<D>;
-    __shared__ int base[MAX_WORKERS];
-    khq::pdl_wait();
-    khq::pdl_trigger();
-    const Meta meta = read_meta(p.meta + blockIdx.x);
-    const int rank = blockIdx.y / parts, part = blockIdx.y % parts, r = threadIdx.x, n = meta.n;
+    constexpr int COLS = D / 4 / MERGE_CTAS;
+    static_assert(MERGE_THREADS == 2 * BR, "two threads a row");
+    const int4 meta = *reinterpret_cast<const int4*>(p.meta + pair);
+    const int rank = part & 1, r = threadIdx.x & 127, n = meta.x;
+    part = (part >> 1) * 2 + (threadIdx.x >> 7);
     if (n == 0) return;
-    const int tok = BR / p.n_rep, t = (r * p.rep_mul) >> 16, n_tok = min(meta.ntok - rank * tok, tok), row = meta.row0 + rank * tok + t;
-    if (n_tok <= 0) return;
-    // record 1 is of the segment that begins in a pair, record 0 of one that it took over
-    for (int i = r; i < n; i += BR) base[i] = 2 * (2 * record_worker(meta, blockIdx.x, i, pairs) + rank) + (i == 0);
-    __syncthreads();
+    const int tok = BR / p.n_rep, t = (r * p.rep_mul) >> 16, n_tok = min(meta.w - rank * tok, tok), row = meta.z + rank * tok + t;
     if (t >= n_tok || row >= p.tokens) return;
+    const auto record = [&](int i) { return p.records + (2LL * (2 * (pair + i) + rank) + (i == 0)) * S::RECORD; };
     float M = -INFINITY;
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) M = fmaxf(M, p.records[(long long)base[i] * S::RECORD + BR * D + 2 * r]);
-    constexpr int COLS = D / 4 / 16;  // groups of 4 columns per part
+    for (int i = 0; i < n; ++i) M = fmaxf(M, record(i)[BR * D + 2 * r]);
     float4 acc[COLS];
 #pragma unroll
     for (int c = 0; c < COLS; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float L = 0.0f;
 #pragma unroll 2
     for (int i = 0; i < n; ++i) {
-        const float* rec = p.records + (long long)base[i] * S::RECORD;
+        const float* rec = record(i);
         const float2 ml = *reinterpret_cast<const float2*>(rec + BR * D + 2 * r);
         float4 a[COLS];
 #pragma unroll
@@ -657,7 +653,7 @@ __global__ void __launch_bounds__(BR) khq_paged_tile_merge_kernel(const Params p
             acc[c].w += a[c].w * f;
         }
     }
-    const int head = meta.h * p.n_rep + (r - t * p.n_rep);
+    const int head = meta.y * p.n_rep + (r - t * p.n_rep);
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
 #pragma unroll
     for (int c = 0; c < COLS; ++c) store_out<BF16>(p, row, head, (part * COLS + c) * 4, acc[c], inv);
