@@ -337,6 +337,30 @@ class BatchEngine:
         self.ring_v[layer][seq, slots] = v.reshape(wl, KV)
         self.ring_u[layer][seq, slots] = (k_unroped if k_unroped is not None else k_roped).reshape(wl, KV)
 
+    def load_pages(self, layer: int, seq: int, k_cache: torch.Tensor, v_cache: torch.Tensor, u_cache: torch.Tensor, block_row: torch.Tensor) -> None:
+        """The sequence's state of one layer from the pages of its prompt (``paged``), which has as many tokens as the sequence starts
+        with: the first ``c_len`` are compressed, the others go into the ring.  Caches (n_pages, page_size, 4, 256) fp16, token-major,
+        ``u_cache``: K not rotated; ``block_row`` int32: the request's row of the block table.  Waits for the device."""
+        from . import paged
+
+        tokens, c = int(self.write_pos[seq]), int(self.boundary[seq])
+        pages = paged.prompt_pages(block_row, tokens, k_cache, v_cache, u_cache, H_KV, D)
+        tb, P, st = self.tables[layer], self.pay[layer], current_stream()
+        if c:
+            runs = paged.page_runs(pages, c, u_cache, int(self.row_off[seq]))
+            common = (runs.data_ptr(), runs.shape[0], k_cache.shape[1] * H_KV)
+            check("launch_khq_compress_batched_fp16", self.lib.launch_khq_compress_batched_fp16(
+                *common, tb["d_k"].data_ptr(), tb["k_rotor"].data_ptr(), tb["cents_k"].data_ptr(), tb["cents_k"].data_ptr(), P["k_mask"].data_ptr(),
+                P["k_norms"].data_ptr(), P["k_r_norms"].data_ptr(), P["k_payload"].data_ptr(), P["v_shared_meta"].data_ptr(), D, float(tb["ts_k"]),
+                float(tb["alpha_k"]), 0, 0, st))
+            check("launch_khq_compress_batched_fp16", self.lib.launch_khq_compress_batched_fp16(
+                *common, tb["d_v"].data_ptr(), tb["v_rotor"].data_ptr(), tb["cents_v"].data_ptr(), tb["vq"].data_ptr(), P["k_mask"].data_ptr(),
+                P["v_norms"].data_ptr(), P["v_r_norms"].data_ptr(), P["v_payload"].data_ptr(), P["v_shared_meta"].data_ptr(), D, float(tb["ts_v"]),
+                float(tb["alpha_v"]), 1, v_cache.data_ptr() - u_cache.data_ptr(), st))
+        if tokens > c:
+            rows = [paged.page_rows(pages, c, tokens, x) for x in (k_cache, v_cache, u_cache)]
+            self.load_window(layer, seq, *rows)
+
     def fill_synthetic(self, seed: int, chunk_tokens: int = 16384) -> None:
         """Seeded synthetic state: per layer and kv-head channel scales exp(0.5 N(0,1)) with four x8
         outlier channels; K/V ~ N(0, s_c); compressed with the library's own compress kernel."""

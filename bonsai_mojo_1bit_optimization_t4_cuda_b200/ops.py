@@ -185,6 +185,15 @@ class CudaOps:
 
     # -- ring appends (khq_ring_dual_sm75_gpu / copy_vec_sm75_gpu,
     #    src/kernels/elementwise_sm75.mojo:277-312): device-to-device copies ------------------
+    # -- launch_khq_compress_batched_fp16 over the pages of a finished prompt -----------------------------
+    def compress_runs(self, runs, rows_per_run, d_vec, rotor, centroids, vq_centroids, out_mask, out_norms, out_r_norms, out_payload, out_shared_meta, d, ts,
+                      alpha, is_v, x_byte_offset):
+        """``runs``: (n, 2) int64 on the device, address of a run's first row and its first output row (``paged.page_runs``)."""
+        rc = self.lib.launch_khq_compress_batched_fp16(
+            ptr(runs), int(runs.shape[0]), int(rows_per_run), ptr(d_vec), ptr(rotor), ptr(centroids), ptr(vq_centroids), ptr(out_mask), ptr(out_norms),
+            ptr(out_r_norms), ptr(out_payload), ptr(out_shared_meta), int(d), float(ts), float(alpha), 1 if is_v else 0, int(x_byte_offset), current_stream())
+        check("launch_khq_compress_batched_fp16", rc)
+
     # -- launch_khq_cal_kstatic_fp32: K-static fit (op 2 of the reference's launch_cal_op) -------------
     def cal_kstatic(self, rot, rows, cents, out_ts, sigma_out=None):
         rc = self.lib.launch_khq_cal_kstatic_fp32(ptr(rot), int(rows), ptr(cents), ptr(out_ts), ptr(sigma_out), current_stream())

@@ -233,3 +233,42 @@ def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scal
     packed = _ATTN_ARGS.pack(qp, gp, kc, vc, block_table.data_ptr(), plan._own[5], op, lp, ws, plan._schedule_bytes, n_ws, q0, q1, g0, g1, o0, o1,
                              kc0, kc1, kc2, vc0, vc1, vc2, st[0] if B > 1 else M, T, plan.max_tokens, plan.max_new, B, M, cache[0], P, H_q, H_kv, d, scale)
     _launch(fns[1], "launch_khq_paged_attn_" + _TYPES[dt], packed, dev)
+
+
+# ---- a finished prompt: from pages to code words --------------------------------------------------------------------------------
+def prompt_pages(block_row: torch.Tensor, tokens: int, k_cache, v_cache, u_cache, H_kv: int, d: int) -> torch.Tensor:
+    """The pages of a prompt's ``tokens`` tokens as an int64 tensor, checked: fp16 caches of one shape with token-major pages (a page is a run of
+    page_size * H_kv contiguous rows), ``u_cache`` and ``v_cache`` with the same distance between pages, page numbers inside the
+    cache.  Waits for the device (the page numbers)."""
+    shape = k_cache.shape
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache), ("u_cache", u_cache)):
+        if c.shape != shape or c.dim() != 4 or c.shape[2:] != (H_kv, d) or c.dtype is not torch.float16 or c.device != block_row.device:
+            raise ValueError(f"{name}: wants fp16 (n_pages, page_size, {H_kv}, {d}) on {block_row.device}, got {tuple(c.shape)} {c.dtype} on {c.device}")
+        if c.stride()[1:] != (H_kv * d, d, 1) or c.data_ptr() & 15 or c.stride(0) & 7:
+            raise ValueError(f"{name}: wants token-major pages on 16 bytes, strides {c.stride()}")
+    if u_cache.stride(0) != v_cache.stride(0):
+        raise ValueError(f"u_cache and v_cache: pages {u_cache.stride(0)} and {v_cache.stride(0)} apart")
+    page_size = shape[1]
+    if page_size not in (16, 32, 64, 128):
+        raise ValueError(f"page_size {page_size}: 16, 32, 64 or 128")
+    n = -(-int(tokens) // page_size)
+    if block_row.dim() != 1 or block_row.dtype is not torch.int32 or block_row.numel() < n:
+        raise ValueError(f"block_row: wants int32 with {n} pages or more for {tokens} tokens, got {tuple(block_row.shape)} {block_row.dtype}")
+    pages = block_row[:n].long()
+    if n and bool(((pages < 0) | (pages >= shape[0])).any()):
+        raise ValueError("block_row: a page that is not in the cache")
+    return pages
+
+
+def page_runs(pages: torch.Tensor, tokens: int, u_cache, row0: int = 0) -> torch.Tensor:
+    """The first ``tokens`` tokens (whole pages) of a prompt as runs for ``CudaOps.compress_runs``: K un-rotated, V at the byte distance of the caches."""
+    _, page_size, H_kv, _ = u_cache.shape
+    n = tokens // page_size
+    at = u_cache.data_ptr() + pages[:n] * (u_cache.stride(0) * 2)
+    return torch.stack((at, row0 + torch.arange(n, device=pages.device) * (page_size * H_kv)), 1)
+
+
+def page_rows(pages: torch.Tensor, first: int, last: int, cache: torch.Tensor) -> torch.Tensor:
+    """Rows ``first`` to ``last`` of a prompt from its pages, (last - first, H_kv * d)."""
+    t = torch.arange(first, last, device=pages.device)
+    return cache[pages[t // cache.shape[1]], t % cache.shape[1]].reshape(last - first, -1)

@@ -538,6 +538,37 @@ class KhqRuntime:
         self._prefill_done(layer_idx, L, T, n_chunks)
         return True
 
+    # ------------------------------------------------------------------ a prompt that came in chunks (addition)
+    def khq_adopt_pages(self, layer_idx: int, k_cache, v_cache, u_cache, block_row, tokens: int) -> bool:
+        """A prompt of ``tokens`` tokens whose chunks went through ``paged.paged_prestep`` and ``paged.paged_attention``: its rows
+        leave the pages for this layer's state, which becomes the one that ``khq_prefill`` leaves.  The pages are free afterwards
+        (behind this call's work on the stream).  ``k_cache`` / ``v_cache`` / ``u_cache`` (n_pages, page_size, H_kv, d) fp16, token-major;
+        ``block_row`` int32: the request's row of the block table.  Only on a fresh layer (write_pos == 0).  Waits for the device."""
+        from . import paged
+
+        if not self.active or not self.ready or layer_idx < 0 or layer_idx >= KHQ_MAX_LAYERS:
+            return False
+        L = self.layers[layer_idx]
+        if not L.ready or L.write_pos != 0:
+            return False
+        if tokens <= 0:
+            raise ValueError(f"khq_adopt_pages: {tokens} tokens")
+        pages = paged.prompt_pages(block_row, tokens, k_cache, v_cache, u_cache, L.H_kv, L.D)
+        Tn, kv = L._t, L.H_kv * L.D
+        n_chunks = max(0, min(tokens // KHQ_CHUNK - 1, L.cap // KHQ_CHUNK))
+        if n_chunks > 0:
+            runs, rows = paged.page_runs(pages, n_chunks * KHQ_CHUNK, u_cache), k_cache.shape[1] * L.H_kv
+            self.ops.compress_runs(runs, rows, Tn["dk"], Tn["rk"], Tn["ck"], Tn["ck"], Tn["kmask"], Tn["knorm"], Tn["krn"], Tn["kpay"], Tn["vsm"], L.D, L.ts_k,
+                                   L.alpha_k, False, 0)
+            self.ops.compress_runs(runs, rows, Tn["dv"], Tn["rv"], Tn["cv"], Tn["vq"], Tn["kmask"], Tn["vnorm"], Tn["vrn"], Tn["vpay"], Tn["vsm"], L.D, L.ts_v,
+                                   L.alpha_v, True, v_cache.data_ptr() - u_cache.data_ptr())
+        first = max(0, tokens - KHQ_RING)
+        slots = torch.arange(first, tokens, device=pages.device) % KHQ_RING
+        for name, cache in (("ring_k", k_cache), ("ring_v", v_cache), ("ring_u", u_cache)):
+            Tn[name].view(KHQ_RING, kv)[slots] = paged.page_rows(pages, first, tokens, cache)
+        self._prefill_done(layer_idx, L, tokens, n_chunks)
+        return True
+
     def _prefill_done(self, layer_idx: int, L, T: int, n_chunks: int) -> None:
         L.boundary = n_chunks * KHQ_CHUNK
         L.write_pos = T
