@@ -334,10 +334,20 @@ struct PrestepArgs {
     int page_shift;
 };
 
+// Packed pairs of fp32, one instruction each.
+__device__ __forceinline__ void mul2(float (&x)[8], int e, float a, float b) {
+    asm("{.reg .b64 p, q; mov.b64 p, {%0, %1}; mov.b64 q, {%2, %3}; mul.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p;}" : "+f"(x[e]), "+f"(x[e + 1]) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {  // d += a b
+    asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 d, {%0, %1}; fma.rn.f32x2 d, a, b, d; mov.b64 {%0, %1}, d;}"
+        : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
 // A CTA takes a token, or a part of its heads; the heads of q, then of k, then of v, 8 values (16 bytes) a lane, so d / 8 lanes a head.  The
-// token's bytes bound it: all of a warp's HEADS heads are on their way while the first threads form the cosines and sines.
+// token's bytes bound it: all of a warp's HEADS heads are on their way while the first threads form the cosines and sines.  With a pass
+// over scalars for every head, v's too, it was instructions (190 a head: 8192 tokens 77 us).
 template <int D, bool BF16, int HEADS>
-__global__ void __launch_bounds__(PRE_WARPS * 32) khq_paged_prestep_kernel(const __grid_constant__ PrestepArgs p) {
+__global__ void __launch_bounds__(PRE_WARPS * 32, 4) khq_paged_prestep_kernel(const __grid_constant__ PrestepArgs p) {
     constexpr int LANES = D / 8, PER = PRE_WARPS * 32 / LANES;
     __shared__ float2 turn[MAX_PAIRS];
     const khq_paged_prestep_args& a = p.a;
@@ -348,14 +358,15 @@ __global__ void __launch_bounds__(PRE_WARPS * 32) khq_paged_prestep_kernel(const
     khq::pdl_trigger();
     const int pos = static_cast<const int*>(a.positions)[t];
     long long slot = static_cast<const long long*>(a.slots)[t];
+    const uint16_t* const q = static_cast<const uint16_t*>(a.q) + t * a.q_stride[0] + lane * 8;
+    const uint16_t* const k = static_cast<const uint16_t*>(a.k) + t * a.k_stride[0] + lane * 8;
+    const uint16_t* const v = static_cast<const uint16_t*>(a.v) + t * a.v_stride[0] + lane * 8;
     uint4 raw[HEADS];
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
         const int h = first + i * PER, hk = h - a.H_q, hv = hk - a.H_kv;
-        const uint16_t* src = h < a.H_q ? static_cast<const uint16_t*>(a.q) + t * a.q_stride[0] + h * a.q_stride[1]
-                              : hk < a.H_kv ? static_cast<const uint16_t*>(a.k) + t * a.k_stride[0] + hk * a.k_stride[1]
-                                            : static_cast<const uint16_t*>(a.v) + t * a.v_stride[0] + hv * a.v_stride[1];
-        raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src + lane * 8) : make_uint4(0, 0, 0, 0);
+        const uint16_t* src = hk < 0 ? q + h * a.q_stride[1] : hv < 0 ? k + hk * a.k_stride[1] : v + hv * a.v_stride[1];
+        raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
     }
     if (pos < 0) return;  // behind the last token
     if (slot >= (long long)a.n_pages << p.page_shift) slot = -1;
@@ -379,45 +390,52 @@ __global__ void __launch_bounds__(PRE_WARPS * 32) khq_paged_prestep_kernel(const
         sn[e] = low ? -f.y : f.y;
     }
     const long long pg = slot >> p.page_shift, at = slot & (a.page_size - 1);
+    const auto cache_row = [&](void* base, const int64_t (&st)[3], int h) {
+        return reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + pg * st[0] + at * st[1] + h * st[2] + lane * 8);
+    };
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
-        const int h = first + i * PER;
-        if (__all_sync(0xFFFFFFFFu, h >= heads)) break;  // whole warps stay together: at d 128 a warp has two heads
-        const bool is_q = h < a.H_q, is_v = h >= a.H_q + a.H_kv, mine = h < heads;
-        const int hk = is_v ? h - a.H_q - a.H_kv : h - a.H_q;
-        const auto cache_row = [&](void* base, const int64_t (&st)[3]) {
-            return reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + pg * st[0] + at * st[1] + hk * st[2] + lane * 8);
-        };
+        const int h = first + i * PER, hk = h - a.H_q, hv = hk - a.H_kv;
+        if (__all_sync(0xFFFFFFFFu, hv >= 0)) {  // whole warps: at d 128 one has two heads
+            if (h < heads && slot >= 0) *cache_row(a.v_cache, a.v_cache_stride, hv) = raw[i];
+            continue;
+        }
         const uint32_t rw[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        float x[8], sq = 0.0f;
+        float x[8], sq[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 f = unpack2<BF16>(rw[e]);
             x[2 * e] = f.x;
             x[2 * e + 1] = f.y;
-            sq += f.x * f.x + f.y * f.y;
+            fma2(sq[0], sq[1], f.x, f.y, f.x, f.y);
         }
+        float sum = sq[0] + sq[1];
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xFFFFFFFFu, sq, o, LANES);
-        const float inv = rsqrtf(sq * (1.0f / D) + a.rms_eps);
-        const float* w = static_cast<const float*>(is_q ? a.q_norm_w : a.k_norm_w);
-        float4 w0 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), w1 = w0;
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o, LANES);
+        const float inv = rsqrtf(sum * (1.0f / D) + a.rms_eps);
+        const float* w = static_cast<const float*>(hk < 0 ? a.q_norm_w : a.k_norm_w);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) mul2(x, e, inv, inv);
         if (w) {
-            w0 = __ldg(reinterpret_cast<const float4*>(w + lane * 8));
-            w1 = __ldg(reinterpret_cast<const float4*>(w + lane * 8) + 1);
+            const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + lane * 8)), w1 = __ldg(reinterpret_cast<const float4*>(w + lane * 8) + 1);
+            mul2(x, 0, w0.x, w0.y);
+            mul2(x, 2, w0.z, w0.w);
+            mul2(x, 4, w1.x, w1.y);
+            mul2(x, 6, w1.z, w1.w);
         }
-        const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        if (hk >= 0 && hv < 0 && slot >= 0 && a.u_cache) *cache_row(a.u_cache, a.u_cache_stride, hk) = pack8<BF16>(x);
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= inv * wv[e];
-        if (mine && !is_q && !is_v && slot >= 0 && a.u_cache) *cache_row(a.u_cache, a.u_cache_stride) = pack8<BF16>(x);
+        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xFFFFFFFFu, x[e], partner, LANES);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float y = __shfl_sync(0xFFFFFFFFu, x[e], partner, LANES);
-            x[e] = x[e] * cs[e] + y * sn[e];
+        for (int e = 0; e < 8; e += 2) {
+            mul2(x, e, cs[e], cs[e + 1]);
+            fma2(x[e], x[e + 1], y[e], y[e + 1], sn[e], sn[e + 1]);
         }
-        if (!mine) continue;
-        if (is_q) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + t * a.q_out_stride[0] + h * a.q_out_stride[1] + lane * 8) = pack8<BF16>(x);
-        else if (slot >= 0) *(is_v ? cache_row(a.v_cache, a.v_cache_stride) : cache_row(a.k_cache, a.k_cache_stride)) = is_v ? raw[i] : pack8<BF16>(x);
+        const uint4 res = pack8<BF16>(x);
+        if (hk < 0) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + t * a.q_out_stride[0] + h * a.q_out_stride[1] + lane * 8) = res;
+        else if (hv < 0 && slot >= 0) *cache_row(a.k_cache, a.k_cache_stride, hk) = res;
+        else if (h < heads && slot >= 0) *cache_row(a.v_cache, a.v_cache_stride, hv) = raw[i];
     }
 }
 
