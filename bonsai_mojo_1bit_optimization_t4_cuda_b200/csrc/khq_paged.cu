@@ -34,6 +34,11 @@ struct PlanArgs {
     Schedule sched;
 };
 
+// An end of a worker's stretch: position `off` of the item, which has n blocks (off 0: where it begins).
+struct Cut {
+    int item, h, off, n, at;
+};
+
 // Inclusive sums of two ints over the block.  `part`: 2 x 32 ints.
 __device__ __forceinline__ void block_scan2(int& a, int& b, int* part, int& total_a, int& total_b) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -83,6 +88,7 @@ __device__ __forceinline__ int find(const int* cum, int n, int x) {
 __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS) khq_paged_plan_kernel(const PlanArgs a) {
     extern __shared__ int sums[];  // tokens, pages taken, pages given back: requests + 1 running sums each
     __shared__ int part[64];
+    __shared__ Cut cuts[MAX_WORKERS + 1];
     int *const cu = sums, *const taken = cu + a.requests + 1, *const back = taken + a.requests + 1;
     const int tid = threadIdx.x, rank = blockIdx.x, B = a.requests, page = 1 << a.page_shift;
     khq::pdl_wait();
@@ -93,13 +99,14 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
     const auto pages = [&](int tokens) { return (int)min(((long long)tokens + page - 1) >> a.page_shift, (long long)a.max_pages); };
     const auto ctx_of = [&](int b) { return (int)min((long long)max(a.ctx_lens[b], 0), (long long)a.max_pages << a.page_shift); };
     int sum_tok = 0, sum_taken = 0, sum_back = 0, dropped = 0;
+    int ctx_next = tid < B ? ctx_of(tid) : 0, asked_next = tid < B ? a.new_lens[tid] : 0;
     for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid;
-        int ctx = 0, n = 0, asked = 0;
-        if (b < B) {
-            ctx = ctx_of(b);
-            asked = a.new_lens[b];
-            n = min(max(asked, 0), a.max_new);
+        const int b = b0 + tid, ctx = ctx_next, asked = asked_next, n = min(max(asked, 0), a.max_new);
+        if (b + PLAN_THREADS < B) {  // the next round's lengths are on their way
+            ctx_next = ctx_of(b + PLAN_THREADS);
+            asked_next = a.new_lens[b + PLAN_THREADS];
+        } else {
+            ctx_next = asked_next = 0;
         }
         int incl = min(n, a.max_tokens), unused = 0, total, u;  // sums of up to 2^10 terms of up to 2^20
         block_scan2(incl, unused, part, total, u);
@@ -225,56 +232,60 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         // Each worker's stretch of the blocks of all kv heads: equal ones, but that an end which falls into an item's first or last `snap` blocks
         // goes to the item's.  No more workers than blocks, so that every worker between an item's first and last has some of it.
         const int over = decodes ? 0 : CHUNK_OVER, snap = decodes ? 0 : CHUNK_SNAP;
-        const long long per_head = blocks + (long long)items * over, total = per_head * a.H_kv;
-        const int workers = (int)min((long long)(decodes ? a.workers : a.workers / 2), total);
+        const int per_head = blocks + items * over, total = per_head * a.H_kv;  // (all in 32 bits: the launcher refuses what would not fit)
+        const int most = decodes ? a.workers : a.workers / 2, workers = min(most, total);
+        const int share = workers > 0 ? total / workers : 0, larger = total - share * workers;
+        const auto end_of = [&](int k) { return k * share + k * larger / workers; };  // of the first k workers: k total / workers, rounded down
         Start* const starts = reinterpret_cast<Start*>(a.schedule + (decodes ? a.sched.decode_starts : a.sched.chunk_starts));
-        struct Cut {
-            int item, h, off, n;  // position `off` of the item, its blocks (off 0: where it begins)
-            long long at;
-        };
-        const auto cut = [&](int k) {
-            const long long v = k * total / workers;
-            Cut c = {0, (int)(v / per_head), 0, 0, v};
-            if (v == total) return c;
-            const int r = (int)(v % per_head);
-            int lo = 0, up = items;  // the last item that begins at r or in front
-            while (up - lo > 1) {
-                const int mid = (lo + up) >> 1;
-                if (cum[mid] + mid * over <= r) lo = mid;
-                else up = mid;
-            }
-            c.item = lo;
-            c.n = (lo + 1 < items ? cum[lo + 1] : blocks) - cum[lo];
-            c.off = r - cum[lo] - lo * over;
-            const int blk = max(c.off - over, 0), rest = c.n - blk;
-            if (blk == 0 || (blk < snap && blk <= rest)) {
-                c.at -= c.off;
-                c.off = 0;
-            } else if (rest < snap) {
-                c.at += rest;
-                c.off = 0;
-                if (++c.item == items) {
-                    c.item = 0;
-                    ++c.h;
+        if (tid <= workers) {
+            const int v = workers > 0 ? end_of(tid) : 0;
+            Cut c = {0, 0, 0, 0, v};
+            if (v < total) {
+                c.h = v / per_head;
+                const int r = v - c.h * per_head;
+                int lo = 0, up = items;  // the last item that begins at r or in front
+                while (up - lo > 1) {
+                    const int mid = (lo + up) >> 1;
+                    if (cum[mid] + mid * over <= r) lo = mid;
+                    else up = mid;
+                }
+                c.item = lo;
+                c.n = (lo + 1 < items ? cum[lo + 1] : blocks) - cum[lo];
+                c.off = r - cum[lo] - lo * over;
+                const int blk = max(c.off - over, 0), rest = c.n - blk;
+                if (blk == 0 || (blk < snap && blk <= rest)) {
+                    c.at -= c.off;
+                    c.off = 0;
+                } else if (rest < snap) {
+                    c.at += rest;
+                    c.off = 0;
+                    if (++c.item == items) {
+                        c.item = 0;
+                        ++c.h;
+                    }
                 }
             }
-            return c;
-        };
-        if (tid < (decodes ? a.workers : a.workers / 2)) {
+            cuts[tid] = c;
+        }
+        __syncthreads();
+        if (tid < most) {
             Start st = {};
             if (tid < workers) {
-                const Cut from = cut(tid), to = cut(tid + 1);
+                const Cut from = cuts[tid], to = cuts[tid + 1];
                 if (from.at < to.at) {
                     st.it = list[from.item];
                     st.item = from.item;
                     st.h = from.h;
                     st.blk = max(from.off - over, 0);
                     st.n_items = items;
-                    st.begins = from.at - from.off;
-                    st.length = (int)(to.at - st.begins);
-                    // the first cut behind the item's last undivided block ends it
-                    const long long end = to.at - to.off + over + (snap > 0 ? to.n - snap + 1 : to.n);
-                    if (to.off > 0) st.share = (int)((end * workers + total - 1) / total) - tid;
+                    st.length = to.at - (from.at - from.off);
+                    if (to.off > 0) {  // the first cut behind the item's last undivided block ends it
+                        const int end = to.at - to.off + over + (snap > 0 ? to.n - snap + 1 : to.n);
+                        int k = min(max((int)((float)end / (float)total * (float)workers) - 1, tid + 1), workers);
+                        while (end_of(k) < end) ++k;
+                        while (end_of(k - 1) >= end) --k;
+                        st.share = k - tid;
+                    }
                 }
             }
             starts[tid] = st;
@@ -294,11 +305,20 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
                 const int col = pos[i] >> a.page_shift;
                 page_of[i] = t < sum_tok && col < a.max_pages ? a.table[b * a.table_stride + col] : -1;
             }
+            long long slot[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t0 + i >= a.max_tokens) break;
-                a.positions[t0 + i] = pos[i];
-                a.slots[t0 + i] = page_of[i] >= 0 ? ((long long)page_of[i] << a.page_shift) + (pos[i] & (page - 1)) : -1;
+            for (int i = 0; i < 4; ++i) slot[i] = page_of[i] >= 0 ? ((long long)page_of[i] << a.page_shift) + (pos[i] & (page - 1)) : -1;
+            if (t0 + 4 <= a.max_tokens) {
+                *reinterpret_cast<int4*>(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+                *reinterpret_cast<longlong2*>(a.slots + t0) = make_longlong2(slot[0], slot[1]);
+                *reinterpret_cast<longlong2*>(a.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    if (t0 + i >= a.max_tokens) break;
+                    a.positions[t0 + i] = pos[i];
+                    a.slots[t0 + i] = slot[i];
+                }
             }
         }
     }
@@ -510,7 +530,8 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
     const void* ptrs[] = {p.ctx_lens, p.new_lens, p.block_table, p.free_list, p.free_count, p.free_count_out, p.cu_new, p.kv_lens, p.positions, p.info};
     for (const void* q : ptrs)
         if ((reinterpret_cast<uintptr_t>(q) & 3) != 0) return -104;
-    if ((reinterpret_cast<uintptr_t>(p.slots) & 7) != 0 || (reinterpret_cast<uintptr_t>(p.schedule) & 15) != 0) return -104;
+    for (const void* q : {static_cast<const void*>(p.positions), static_cast<const void*>(p.slots), static_cast<const void*>(p.schedule)})
+        if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return -104;
     const Schedule sched = schedule_of(p.requests, p.max_tokens, p.max_new, p.H_q, p.H_kv, p.d);
     if (p.schedule_bytes < (size_t)sched.ints * 4) return -105;
     // the key blocks of all items and kv heads are counted in 32 bits

@@ -17,8 +17,8 @@ constexpr int ITEM_INTS = sizeof(Item) / 4;
 struct alignas(16) Start {
     Item it;
     int item, h, blk, n_items;  // blk: the item's first block in the stretch
-    long long begins;           // where the item begins in the row of all blocks
-    int length, share;          // from there to the stretch's end (0: nothing to do); the workers from this one on that share the item it ends in
+    int length, share;          // from the item's begin to the stretch's end (0: nothing to do); the workers from this one on that share the item it ends in
+    int pad[2];
 };
 constexpr int START_INTS = sizeof(Start) / 4, MAX_WORKERS = 256;
 static_assert(START_INTS == 16, "four 16-byte loads");

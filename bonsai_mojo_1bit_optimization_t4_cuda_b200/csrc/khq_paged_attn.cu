@@ -82,7 +82,8 @@ __device__ __forceinline__ void load_segment(const Params& p, Segment& s) {
 // The worker's first segment; false: none.
 __device__ __forceinline__ bool first_segment(const Params& p, int worker, Segment& s, int& n_items, int& length, int& share) {
     const int4* at = reinterpret_cast<const int4*>(p.starts + worker);
-    const int4 x = at[0], y = at[1], z = at[2], w = at[3];  // (ordinary loads: nothing else keeps them behind the wait for the plan)
+    const int4 x = at[0], y = at[1], z = at[2];
+    const int2 w = *reinterpret_cast<const int2*>(at + 3);  // (ordinary loads: nothing else keeps them behind the wait for the plan)
     s.b = x.x;
     s.n_blocks = x.y;
     s.ntok = x.z;
@@ -93,8 +94,8 @@ __device__ __forceinline__ bool first_segment(const Params& p, int worker, Segme
     s.h = z.y;
     s.blk = z.z;
     n_items = z.w;
-    length = w.z;
-    share = w.w;
+    length = w.x;
+    share = w.y;
     return length > 0;
 }
 // Every item has a key block at least (its own tokens).
