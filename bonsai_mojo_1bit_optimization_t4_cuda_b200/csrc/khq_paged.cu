@@ -231,7 +231,7 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         __syncthreads();
         // Each worker's stretch of the blocks of all kv heads: equal ones, but that an end which falls into an item's first or last `snap` blocks
         // goes to the item's.  No more workers than blocks, so that every worker between an item's first and last has some of it.
-        const int over = decodes ? 0 : CHUNK_OVER, snap = decodes ? 0 : CHUNK_SNAP;
+        const int over = decodes ? DECODE_OVER : CHUNK_OVER, snap = decodes ? 0 : CHUNK_SNAP;
         const int per_head = blocks + items * over, total = per_head * a.H_kv;  // (all in 32 bits: the launcher refuses what would not fit)
         const int most = decodes ? a.workers : a.workers / 2, workers = min(most, total);
         const int share = workers > 0 ? total / workers : 0, larger = total - share * workers;
@@ -536,7 +536,7 @@ extern "C" int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream
     if (p.schedule_bytes < (size_t)sched.ints * 4) return -105;
     // the key blocks of all items and kv heads are counted in 32 bits
     const long long row = ((long long)p.max_pages << shift) + p.max_tokens;
-    if (sched.chunk_cap * (row / TILE_KEYS + 1 + CHUNK_OVER) > 0x7FFFFFFFLL / p.H_kv || sched.decode_cap * (row / sched.decode_keys + 1) > 0x7FFFFFFFLL / p.H_kv) return -103;
+    if (sched.chunk_cap * (row / TILE_KEYS + 1 + CHUNK_OVER) > 0x7FFFFFFFLL / p.H_kv || sched.decode_cap * (row / sched.decode_keys + 1 + DECODE_OVER) > 0x7FFFFFFFLL / p.H_kv) return -103;
     PlanArgs a;
     a.ctx_lens = static_cast<const int*>(p.ctx_lens);
     a.new_lens = static_cast<const int*>(p.new_lens);

@@ -29,9 +29,12 @@ static_assert(START_INTS == 16, "four 16-byte loads");
 constexpr int MAX_REP = 128;  // query heads of a kv head
 constexpr int DECODE_ROWS = 16, TILE_ROWS = 128, TILE_KEYS = 128;
 constexpr int decode_keys(int d) { return 64 * 256 / d; }  // keys of a block of the decode kernel: 64 KB of K and V
-// What a tile costs beside its key blocks, in blocks: its queries, gates and outputs, and the pipe's run-in.  And how near to an item's ends its
-// blocks are not divided between two pairs: 264 KB of partial rows from each of them would have to be written and read again.
-constexpr int CHUNK_OVER = 3, CHUNK_SNAP = 4;
+// What an item costs beside its key blocks, in blocks: its queries, gates and outputs, and the pipe's run-in; the joining of the warps.  And how
+// near to an item's ends its blocks are not divided between two pairs: 264 KB of partial rows from each of them would have to be written
+// and read again.
+// (4 x 8192 tokens: 2.79 ms with 3 blocks of a chunk's tile, 2.65 with 6; 40 single tokens over 2600 on average: 92 us with 0 of a decode
+// item, 84 with 2.)
+constexpr int CHUNK_OVER = 6, DECODE_OVER = 2, CHUNK_SNAP = 4;
 struct Schedule {
     bool chunks, decodes;             // the lists that the step can have
     int tile_tokens, decode_tokens;   // new tokens of a tile; the most of a request for the decode kernel (0: none)

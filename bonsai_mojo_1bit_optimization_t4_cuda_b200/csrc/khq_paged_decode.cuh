@@ -85,7 +85,9 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         if (beside) khq::pdl_wait();
         return;
     }
-    const int blocks = length - in.blk;  // of the stretch
+    // what is left of the stretch from the item's begin on, and the item's blocks in it
+    const auto of_stretch = [](const Segment& s, int left) { return min(s.n_blocks, left - DECODE_OVER) - s.blk; };
+    int left_in = length, n_in = of_stretch(in, length), left = length, n_seg = n_in;
     cur = in;
     uint64_t* const bar = bars + warp * S::STAGES;
     const uint32_t ring = smem_u32(smem) + warp * S::STAGES * 2 * S::PIECE;
@@ -96,7 +98,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     constexpr int UNIT = S::UNIT;
     const int log_per = UNIT == 32 && p.page_shift == 4 ? 1 : 0, groups = log_per ? S::G : 1;
     int pages = 0, pages_next = 0, pages_at = -1;
-    int w_in = 0, s_in = 0;
+    int s_in = 0;
     uint32_t missing = 0;  // two bits by unit of the ring: its first, second page is not there
     bool ok = true;        // no wait has run out
     const auto fetch_pages = [&](int blk) {
@@ -109,7 +111,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         return pg;
     };
     const auto issue = [&]() {
-        if (w_in >= blocks) return;
+        if (n_in == 0) return;
         if (pages_at < 0 || in.blk - pages_at >= (32 >> log_per)) {
             pages = pages_at < 0 ? fetch_pages(in.blk) : pages_next;
             pages_at = in.blk;
@@ -128,9 +130,10 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                             (in.blk * S::KEYS + warp * UNIT) & p.page_mask, c, in.h, page);
         }
         s_in = s_in + 1 == S::STAGES ? 0 : s_in + 1;
-        ++w_in;
-        if (++in.blk == in.n_blocks && w_in < blocks) {
+        ++in.blk;
+        if (--n_in == 0 && (left_in -= in.n_blocks + DECODE_OVER) > DECODE_OVER) {
             next_segment(p, n_items, in);
+            n_in = of_stretch(in, left_in);
             pages_at = -1;
         }
     };
@@ -147,12 +150,13 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const uint32_t k_row = k_key * 128, v_row = S::PIECE + v_key * 128, sw = (lane & 7);
     int s = 0;
     uint32_t phase = 0;
-    bool fresh = true;
+    bool fresh = true, begins = false;  // a segment's first block; the segment is the item's begin
 #pragma unroll 1
-    for (int w = 0; w < blocks; ++w) {
+    for (;;) {
         const int R = cur.ntok * p.n_rep;
         if (fresh) {
             fresh = false;
+            begins = cur.blk == 0;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int r = g + 8 * half, t = (r * p.rep_mul) >> 16, row = cur.row0 + t;
@@ -273,10 +277,9 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         phase ^= (uint32_t)(s == 0);
         issue();
         const bool ends = cur.blk + 1 == cur.n_blocks;
-        if (ends || w + 1 == blocks) {
+        if (--n_seg == 0) {
             // ---- join the warps ----------------------------------------------------------------------
-            const int seg_lo = w - cur.blk;  // from the stretch's begin
-            const bool whole = seg_lo >= 0 && ends;
+            const bool whole = begins && ends;
             float* const join = reinterpret_cast<float*>(smem + S::OFF_JOIN);
             float2* const ml = reinterpret_cast<float2*>(smem + S::OFF_ML);
 #pragma unroll
@@ -292,7 +295,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 for (int v = 1; v < WARPS; ++v) M = fmaxf(M, ml[v * DECODE_ROWS + r].x);
                 return M;
             };
-            float* const rec = p.records + (2LL * blockIdx.x + (seg_lo >= 0 ? 1 : 0)) * S::RECORD;
+            float* const rec = p.records + (2LL * blockIdx.x + (begins ? 1 : 0)) * S::RECORD;
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
                 if (half * 8 >= R) break;
@@ -336,11 +339,14 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 }
                 __syncthreads();
             }
-            if (tid == 0 && seg_lo >= 0 && !ends) *reinterpret_cast<int4*>(p.meta + blockIdx.x) = make_int4(share, cur.h, cur.row0, cur.ntok);
+            if (tid == 0 && begins && !ends) *reinterpret_cast<int4*>(p.meta + blockIdx.x) = make_int4(share, cur.h, cur.row0, cur.ntok);
+            if ((left -= cur.n_blocks + DECODE_OVER) <= DECODE_OVER) break;
+            next_segment(p, n_items, cur);
+            n_seg = of_stretch(cur, left);
             fresh = true;
+        } else {
+            ++cur.blk;
         }
-        ++cur.blk;
-        if (ends && w + 1 < blocks) next_segment(p, n_items, cur);
     }
     if (beside) khq::pdl_wait();
 }

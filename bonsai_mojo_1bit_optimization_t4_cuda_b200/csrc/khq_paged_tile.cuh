@@ -23,18 +23,23 @@ namespace tile {
 
 constexpr int BR = 128, BC = 128;            // query rows of a CTA, keys of a block
 constexpr int NSOFT = 256, NTHREADS = NSOFT + 128;  // warp 11 has no work: registers are split by groups of four warps
-constexpr uint32_t TM_COLS = 512, TM_S = 256;  // O from column 0
+constexpr uint32_t TM_COLS = 512;            // O from column 0, the S buffers behind it
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr int STG_BYTES = 32 * 64;           // per softmax warp: 32 rows x 32 columns
 constexpr int MAX_STAGES = 4;
-enum Bar {  // K and V by stage, S and P V by block parity
-    B_KFULL = 0, B_KFREE = 4, B_VFULL = 8, B_VFREE = 12, B_SFULL = 16, B_PVDONE = 18, B_PREADY = 20 /* [parity][half of the keys] */, B_QFULL = 24, B_QFREE = 25,
-    B_PEER = 26, B_MREF = 27 /* [group][lane quarter] */, B_LSUM = 35 /* [lane quarter] */, B_OFREE = 39, B_VLAND = 40, B_COUNT = 41
+enum Bar {  // K and V by stage, S by buffer, P V by block parity
+    B_KFULL = 0, B_KFREE = 4, B_VFULL = 8, B_VFREE = 12, B_SFULL = 16, B_PVDONE = 19, B_PREADY = 21 /* [buffer][half of the keys] */, B_QFULL = 27, B_QFREE = 28,
+    B_PEER = 29, B_MREF = 30 /* [group][lane quarter] */, B_LSUM = 38 /* [lane quarter] */, B_OFREE = 42, B_VLAND = 43, B_COUNT = 44
 };
 template <int D> struct Shape {
     static constexpr int G = D / 64;               // column groups
     // K and V blocks in flight: what fits.  Few query rows leave the cache's latency and bytes as the bound.
     static constexpr int STAGES = D == 256 ? 2 : 4;
+    // Score buffers: what tensor memory has room for.  With three, Q K^T runs two blocks ahead of P V, and a softmax group has its next block's scores
+    // when it is done with one (at d 128 the softmax is the longer part of a block).
+    static constexpr int BUFFERS = D == 256 ? 2 : 3, AHEAD = BUFFERS - 1;
+    static constexpr uint32_t TM_S = D;
+    static_assert(TM_S + BUFFERS * BC <= TM_COLS, "tensor memory");
     static constexpr int Q_BYTES = BR * D * 2, TILE_BYTES = 64 * D * 2;  // a CTA's rows; its share of a K or V block
     static constexpr int OFF_Q = 0, OFF_K = OFF_Q + Q_BYTES, OFF_V = OFF_K + STAGES * TILE_BYTES, OFF_STG = OFF_V + STAGES * TILE_BYTES;
     static constexpr int OFF_MREF = OFF_STG + 8 * STG_BYTES;  // float [2 groups][128 rows]: the reference behind the group's last block
@@ -139,20 +144,16 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             khq::mbar_init(&bars[B_VFULL + s], 2);  // the V producers of both CTAs
             khq::mbar_init(&bars[B_VFREE + s], 1);
         }
-        for (int s = 0; s < 2; ++s) {
-            khq::mbar_init(&bars[B_SFULL + s], 1);
-            khq::mbar_init(&bars[B_PVDONE + s], 1);
-        }
+        for (int s = 0; s < 2; ++s) khq::mbar_init(&bars[B_PVDONE + s], 1);
+        for (int s = 0; s < S::BUFFERS; ++s) khq::mbar_init(&bars[B_SFULL + s], 1);
         khq::mbar_init(&bars[B_QFULL], 1);
         khq::mbar_init(&bars[B_QFREE], 1);
         khq::mbar_init(&bars[B_PEER], 1);
         khq::mbar_init(&bars[B_VLAND], 1);
         khq::mbar_init(&bars[B_OFREE], 2 * NSOFT / 32);
         // one elected arrival per softmax warp of both CTAs: separate arrivals on one barrier serialise
-        for (int q = 0; q < 4; ++q) {
-            khq::mbar_init(&bars[B_PREADY + q], 2 * NSOFT / 64);
-            khq::mbar_init(&bars[B_LSUM + q], 2);  // the two warps of a lane quarter
-        }
+        for (int q = 0; q < 2 * S::BUFFERS; ++q) khq::mbar_init(&bars[B_PREADY + q], 2 * NSOFT / 64);
+        for (int q = 0; q < 4; ++q) khq::mbar_init(&bars[B_LSUM + q], 2);  // the two warps of a lane quarter
         for (int q = 0; q < 8; ++q) khq::mbar_init(&bars[B_MREF + q], 1);
         khq::fence_barrier_init();
     } else if (warp == 8 && lane < 3) {
@@ -297,9 +298,9 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             const auto need = [&](uint32_t there, uint64_t* bar, uint32_t parity) {
                 if (ok && !__any_sync(0xFFFFFFFFu, there)) ok = warp_wait(bar, parity, status);
             };
-            // S[g & 1] = Q K^T of block g; the tests are of block g - 1's weights and V
+            // S = Q K^T of block g; the tests are of the weights and V of the block that is multiplied next
             const auto issue_qk = [&](int g, bool test) {
-                const uint32_t s_tmem = tmem + TM_S + (uint32_t)(g & 1) * BC;
+                const uint32_t s_tmem = tmem + S::TM_S + (uint32_t)(g % S::BUFFERS) * BC;
                 const int ks_at = g % S::STAGES;
                 need(k_of == g ? k_there : 0u, &bars[B_KFULL + ks_at], (uint32_t)((g / S::STAGES) & 1));
                 if (!ok) return;
@@ -313,11 +314,12 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     if (ks == 0) umma2_ss<0>(one, s_tmem, q_lo + oa, HI, k_at + ob, HI, IDESC_S);
                     else umma2_ss<1>(one, s_tmem, q_lo + oa, HI, k_at + ob, HI, IDESC_S);
                     if (ks == D / 16 - 5 && test) {
-                        p_there = mbar_test(&bars[B_PREADY + 2 * ((g - 1) & 1)], (uint32_t)(((g - 1) >> 1) & 1));
-                        v_there = mbar_test(&bars[B_VFULL + (g - 1) % S::STAGES], (uint32_t)(((g - 1) / S::STAGES) & 1));
+                        const int n = g - S::AHEAD;
+                        p_there = mbar_test(&bars[B_PREADY + 2 * (n % S::BUFFERS)], (uint32_t)((n / S::BUFFERS) & 1));
+                        v_there = mbar_test(&bars[B_VFULL + n % S::STAGES], (uint32_t)((n / S::STAGES) & 1));
                     }
                 }
-                umma2_commit(one, &bars[B_SFULL + (g & 1)]);
+                umma2_commit(one, &bars[B_SFULL + g % S::BUFFERS]);
                 umma2_commit(one, &bars[B_KFREE + ks_at]);
             };
             int g = 0, i = 0;
@@ -326,17 +328,17 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             for (; ok && more; more = walk.step(p, n_items), ++i) {
                 ok = tile::warp_wait(&bars[B_QFULL], (uint32_t)(i & 1), status);
                 if (!ok) break;
-                issue_qk(g, false);
+                for (int j = 0; ok && j < min(S::AHEAD, walk.n); ++j) issue_qk(g + j, false);
                 if (!ok) break;
-                if (walk.n == 1) umma2_commit(one, &bars[B_QFREE]);
+                if (walk.n <= S::AHEAD) umma2_commit(one, &bars[B_QFREE]);
                 for (int j = 0; j < walk.n; ++j, ++g) {
-                    const int s = g & 1, vs = g % S::STAGES;
-                    const uint32_t par = (uint32_t)((g >> 1) & 1), v_par = (uint32_t)((g / S::STAGES) & 1);
+                    const int s = g % S::BUFFERS, vs = g % S::STAGES;
+                    const uint32_t par = (uint32_t)((g / S::BUFFERS) & 1), v_par = (uint32_t)((g / S::STAGES) & 1);
                     p_there = v_there = 0;
-                    if (j + 1 < walk.n) {
-                        issue_qk(g + 1, true);
+                    if (j + S::AHEAD < walk.n) {
+                        issue_qk(g + S::AHEAD, true);
                         if (!ok) break;
-                        if (j + 2 == walk.n) umma2_commit(one, &bars[B_QFREE]);
+                        if (j + S::AHEAD + 1 == walk.n) umma2_commit(one, &bars[B_QFREE]);
                     }
                     need(p_there, &bars[B_PREADY + 2 * s], par);
                     if ((walk.s.blk + j + 1) * BC > walk.s.kv) {
@@ -349,7 +351,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     if (j == 0 && i > 0 && ok) ok = tile::warp_wait(&bars[B_OFREE], (uint32_t)((i - 1) & 1), status);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t v_at = v_lo + (uint32_t)vs * (S::TILE_BYTES >> 4), p_tmem = tmem + TM_S + (uint32_t)s * BC;
+                    const uint32_t v_at = v_lo + (uint32_t)vs * (S::TILE_BYTES >> 4), p_tmem = tmem + S::TM_S + (uint32_t)s * BC;
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
                         if (kk == 4) {  // the other half of the keys: its weights come while the first half is multiplied
@@ -360,12 +362,12 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                         umma2_ts(one, tmem, p_tmem + kk * 8, v_at + ((uint32_t)(kk * 2048) >> 4), HI, IDESC_O, kk > 0 ? 1u : (uint32_t)(j > 0));  // 16 keys = 2048 bytes
                         if (kk == 1) p_there = mbar_test(&bars[B_PREADY + 2 * s + 1], par);
                         if (kk == 5) {
-                            k_there = mbar_test(&bars[B_KFULL + (g + 2) % S::STAGES], (uint32_t)(((g + 2) / S::STAGES) & 1));
-                            k_of = g + 2;
+                            k_of = g + 1 + S::AHEAD;
+                            k_there = mbar_test(&bars[B_KFULL + k_of % S::STAGES], (uint32_t)((k_of / S::STAGES) & 1));
                         }
                     }
                     if (!ok) break;
-                    umma2_commit(one, &bars[B_PVDONE + s]);
+                    umma2_commit(one, &bars[B_PVDONE + (g & 1)]);
                     umma2_commit(one, &bars[B_VFREE + vs]);
                 }
             }
@@ -418,10 +420,11 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     if (!ok) break;
                     before = mref[(grp ^ 1) * 128 + r];
                 }
-                ok = __all_sync(0xFFFFFFFFu, wait_for(&bars[B_SFULL + grp], (uint32_t)((g >> 1) & 1), status));
+                const int buf = g % S::BUFFERS;
+                ok = __all_sync(0xFFFFFFFFu, wait_for(&bars[B_SFULL + buf], (uint32_t)((g / S::BUFFERS) & 1), status));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t s_addr = lane_base + TM_S + (uint32_t)grp * BC;
+                const uint32_t s_addr = lane_base + S::TM_S + (uint32_t)buf * BC;
                 uint32_t sr[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, sr[c]);
@@ -451,7 +454,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 if (__any_sync(0xFFFFFFFFu, grow)) {
                     // O may only be touched between P V of the previous block and P V of this one.  The completion barriers alternate
                     // between two mbarriers so that a thread may skip phases: barrier (g-1)&1 last completed for block g-3 (certainly, since
-                    // Q K^T of this block was issued behind P V of block g-2) and cannot complete for block g+1 before this
+                    // Q K^T of this block was issued behind P V of block g-2, or g-3 with three buffers) and cannot complete for block g+1 before this
                     // thread's own arrival for block g.
                     ok = __all_sync(0xFFFFFFFFu, wait_for(&bars[B_PVDONE + ((g - 1) & 1)], (uint32_t)(((g - 1) >> 1) & 1), status));
                     if (!ok) break;
@@ -486,7 +489,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) arrive_leader(&bars[B_PREADY + 2 * grp + h]);
+                    if (lane == 0) arrive_leader(&bars[B_PREADY + 2 * buf + h]);
                 }
                 l_run = (m_l == m_used ? l_run : l_run * exp2f(m_l - m_used)) + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
                 m_l = m_used;
