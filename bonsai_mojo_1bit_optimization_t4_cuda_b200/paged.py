@@ -17,75 +17,83 @@ and the sequence goes on in code words.
 """
 from __future__ import annotations
 
-import struct
+import ctypes
 from typing import Optional
 
 import torch
 
 from . import lib as _lib
-from .lib import check
+from .lib import KhqLibraryError, check
 
-# the structs of include/khq_b200.h, field by field ("@": native alignment)
-_PLAN_ARGS = struct.Struct("@12PNq9i0q")
-_PRESTEP_ARGS = struct.Struct("@11P17q7i2f0q")
-_ATTN_ARGS = struct.Struct("@9P2N12qq10if0q")
 _TYPES = {torch.float16: "fp16", torch.bfloat16: "bf16"}
+_NO_FIT = -1000  # of the extension: a tensor is not what the plan asks for
 
 
-# A step's host time is mostly the look at its tensors (some 0.1 us per property): each is asked for what it is checked by once.
+class _PlanInfo(ctypes.Structure):
+    """``PlanInfo`` of csrc/khq_paged_host.cpp."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("device", "H_q", "H_kv", "d", "page_size", "max_requests", "max_tokens", "max_new", "requests", "max_pages")] + [
+        (n, ctypes.c_void_p) for n in ("cu_new", "kv_lens", "positions", "slots", "info", "schedule", "workspace")] + [
+        (n, ctypes.c_int64) for n in ("schedule_bytes", "workspace_bytes")] + [
+        (n, ctypes.c_void_p) for n in ("launch_plan", "launch_prestep_fp16", "launch_prestep_bf16", "launch_attn_fp16", "launch_attn_bf16")]
 
 
-def _launch(fn, name: str, packed: bytes, device: int) -> None:
-    if _current_device() != device:
-        with torch.cuda.device(device):
-            rc = fn(packed, _current_stream(device))
-    else:
-        rc = fn(packed, _current_stream(device))
-    if rc != 0:
-        check(name, rc)
+_host = None
 
 
-def _current_device() -> int:
-    return torch._C._cuda_getDevice()
+def _load_host():
+    """The extension that looks at a call's tensors and launches (csrc/khq_paged_host.cpp)."""
+    global _host
+    if _host is None:
+        try:
+            from . import _khq_paged_host as host
+        except ImportError as e:
+            raise KhqLibraryError(f"the paged operators' extension cannot be loaded ({e}): build it with "
+                                  "`python -m bonsai_mojo_1bit_optimization_t4_cuda_b200.build`") from e
+        if host.info_bytes() != ctypes.sizeof(_PlanInfo):
+            raise KhqLibraryError("the paged operators' extension is stale: build it anew")
+        _host = host
+    return _host
 
 
-def _current_stream(device: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(device)
+# ---- what does not fit, in words (a call comes here only when the extension has refused it) ------------------------------------------------
+def _look(t, name: str, want, dtype, device: int, contiguous: bool = False) -> None:
+    """``want``: the shape, None for any size."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor, got {type(t).__name__}")
+    shape = tuple(t.shape)
+    if t.get_device() != device or t.dtype is not dtype or len(shape) != len(want) or any(w is not None and w != s for w, s in zip(want, shape)):
+        text = ", ".join("any" if w is None else str(w) for w in want)
+        raise ValueError(f"{name}: wants ({text}) {dtype} on cuda:{device}, got {shape} {t.dtype} on {t.device}")
+    if t.stride(-1) != 1 or (contiguous and not t.is_contiguous()):
+        raise ValueError(f"{name}: {'has to be contiguous' if contiguous else 'the last dimension has to be contiguous'}, strides {t.stride()}")
 
 
-def _refuse(t, name: str, want, dtype, device: int):
-    if t.get_device() != device or t.dtype is not dtype or len(t.shape) != len(want) or any(w is not None and w != s for w, s in zip(want, t.shape)):
-        shape = ", ".join("any" if w is None else str(w) for w in want)
-        raise ValueError(f"{name}: wants ({shape}) {dtype} on cuda:{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    raise ValueError(f"{name}: the last dimension has to be contiguous, strides {t.stride()}")
-
-
-def _ints(t: torch.Tensor, name: str, numel: Optional[int], device: int, dtype=torch.int32) -> int:
+def _look_flat(t, name: str, numel: Optional[int], dtype, device: int) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor, got {type(t).__name__}")
     if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or (numel is not None and t.numel() != numel):
         raise ValueError(f"{name}: wants contiguous {dtype} on cuda:{device}" + (f" with {numel} entries" if numel is not None else "")
                          + f", got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, heads: int, d: int, tokens: int, dtype, device: int):
-    """(tokens, heads, d) with any strides over tokens and heads."""
-    st = t.stride()
-    if t.shape != (tokens, heads, d) or st[2] != 1 or t.dtype is not dtype or t.get_device() != device:
-        _refuse(t, name, (tokens, heads, d), dtype, device)
-    return t.data_ptr(), st[0], st[1]
+def _look_step(plan: "PagedPlan", what: str, q) -> int:
+    if q.dtype not in _TYPES:
+        raise TypeError(f"{what}: fp16 or bf16, got {q.dtype}")
+    T = q.shape[0] if q.dim() else 0
+    if not 0 < T <= plan.max_tokens:
+        raise ValueError(f"{what}: {T} rows, the plan is for 1 to {plan.max_tokens}")
+    if plan.requests == 0:
+        raise ValueError(f"{what}: the plan has not been built")
+    return T
 
 
-def _cache(t: torch.Tensor, name: str, shape, dtype, device: int):
-    """(n_pages, page_size, heads, d) with any strides over the first three."""
-    st = t.stride()
-    if t.shape != shape or st[3] != 1 or t.dtype is not dtype or t.get_device() != device:
-        _refuse(t, name, shape, dtype, device)
-    return t.data_ptr(), st[0], st[1], st[2]
-
-
-def _pages_of(t: torch.Tensor, page_size: int, heads: int, d: int):
-    """The shape that a cache with as many pages as this one has."""
-    return (t.shape[0] if t.dim() == 4 else None, page_size, heads, d)
+def _look_caches(plan: "PagedPlan", dtype, **caches) -> None:
+    pages = None
+    for name, c in caches.items():
+        if c is not None:
+            _look(c, name, (pages, plan.page_size, plan.H_kv, plan.d), dtype, plan.device)
+            pages = c.shape[0]
 
 
 class PagedPlan:
@@ -120,11 +128,24 @@ class PagedPlan:
         self.info = torch.zeros(8, dtype=torch.int32, device=self.positions.device)
         self.schedule, self._workspace_bytes = empty(n, torch.uint8), w
         self.workspace = self.new_workspace()
-        self._scratch, self._schedule_bytes = (self.workspace.data_ptr(), w), n
-        self.requests = self.max_pages = 0  # of the last build
-        self._fns = {dt: (getattr(self.lib, "launch_khq_paged_prestep_" + t), getattr(self.lib, "launch_khq_paged_attn_" + t)) for dt, t in _TYPES.items()}
-        self._own = (self._cu_new.data_ptr(), self._kv_lens.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.info.data_ptr(),
-                     self.schedule.data_ptr())
+        fn = lambda name: ctypes.cast(getattr(self.lib, name), ctypes.c_void_p).value
+        self._info = _PlanInfo(
+            self.device, self.H_q, self.H_kv, self.d, self.page_size, self.max_requests, self.max_tokens, self.max_new, 0, 0, self._cu_new.data_ptr(),
+            self._kv_lens.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(), self.info.data_ptr(), self.schedule.data_ptr(),
+            self.workspace.data_ptr(), n, w, fn("launch_khq_paged_plan"), fn("launch_khq_paged_prestep_fp16"), fn("launch_khq_paged_prestep_bf16"),
+            fn("launch_khq_paged_attn_fp16"), fn("launch_khq_paged_attn_bf16"))
+        self._at = ctypes.addressof(self._info)
+        host = _load_host()
+        self._build, self._prestep, self._attention = host.build, host.prestep, host.attention
+
+    @property
+    def requests(self) -> int:
+        """Of the last build (0: none yet)."""
+        return self._info.requests
+
+    @property
+    def max_pages(self) -> int:
+        return self._info.max_pages
 
     def new_workspace(self) -> torch.Tensor:
         """Scratch memory for ``paged_attention`` calls that may run beside those with the plan's own."""
@@ -144,28 +165,28 @@ class PagedPlan:
         ``block_table`` (requests, max_pages) int32.  With ``free_list`` (n_pages) and ``free_count`` (1) int32 the pages of the new
         tokens are taken from it and entered in the table, and those of ended requests go back; ``free_count`` is brought up
         to date, or left as it is and the new count written to ``free_count_out``.  Without, the table has all pages already."""
+        rc = self._build(self._at, ctx_lens, new_lens, block_table, free_list, free_count, free_count_out)
+        if rc != 0:
+            if rc == _NO_FIT:
+                self._look_at_build(ctx_lens, new_lens, block_table, free_list, free_count, free_count_out)
+            check("launch_khq_paged_plan", rc)
+        return self
+
+    def _look_at_build(self, ctx_lens, new_lens, block_table, free_list, free_count, free_count_out) -> None:
         dev, n = self.device, ctx_lens.numel()
         if not 0 < n <= self.max_requests:
             raise ValueError(f"PagedPlan.build: {n} requests, built for 1 to {self.max_requests}")
-        ctx, new = _ints(ctx_lens, "ctx_lens", n, dev), _ints(new_lens, "new_lens", n, dev)
-        st, shape = block_table.stride(), block_table.shape
-        if len(shape) != 2 or shape[0] != n or shape[1] < 1 or st[1] != 1 or block_table.dtype is not torch.int32 or block_table.get_device() != dev:
-            _refuse(block_table, "block_table", (n, None), torch.int32, dev)
-        fl = fc = fo = n_pages = 0
-        if free_list is not None:
-            if free_count is None:
-                raise ValueError("PagedPlan.build: free_list without free_count")
-            n_pages = free_list.numel()
-            fl, fc = _ints(free_list, "free_list", None, dev), _ints(free_count, "free_count", 1, dev)
-            fo = fc if free_count_out is None else _ints(free_count_out, "free_count_out", 1, dev)
-        elif free_count is not None or free_count_out is not None:
+        _look_flat(ctx_lens, "ctx_lens", n, torch.int32, dev)
+        _look_flat(new_lens, "new_lens", n, torch.int32, dev)
+        _look(block_table, "block_table", (n, None), torch.int32, dev)
+        if free_list is None:
             raise ValueError("PagedPlan.build: free_count without free_list")
-        max_pages = shape[1]
-        packed = _PLAN_ARGS.pack(ctx, new, block_table.data_ptr(), fl, fc, fo, *self._own, self._schedule_bytes, st[0] if n > 1 else max_pages, n, max_pages,
-                                 n_pages, self.page_size, self.max_tokens, self.max_new, self.H_q, self.H_kv, self.d)
-        _launch(self.lib.launch_khq_paged_plan, "launch_khq_paged_plan", packed, dev)
-        self.requests, self.max_pages = n, max_pages
-        return self
+        if free_count is None:
+            raise ValueError("PagedPlan.build: free_list without free_count")
+        _look_flat(free_list, "free_list", None, torch.int32, dev)
+        _look_flat(free_count, "free_count", 1, torch.int32, dev)
+        if free_count_out is not None:
+            _look_flat(free_count_out, "free_count_out", 1, torch.int32, dev)
 
 
 def paged_prestep(plan: PagedPlan, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, v_cache, u_cache=None, rotary_dim: int = 64,
@@ -173,33 +194,17 @@ def paged_prestep(plan: PagedPlan, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, 
     """Head RMS norms of ``q`` and ``k`` (weights fp32 (d) or None), rotation of the first ``rotary_dim`` dims at the plan's positions; ``q``
     to ``q_out`` (which may be ``q``), rotated ``k``, ``v`` and, with ``u_cache``, un-rotated ``k`` to the plan's slots.  The
     counterpart of ``CudaOps.prestep`` for ragged rows and pages."""
-    dev, H_q, H_kv, d, P, dt = plan.device, plan.H_q, plan.H_kv, plan.d, plan.page_size, q.dtype
-    fns = plan._fns.get(dt)
-    if fns is None:
-        raise TypeError(f"paged_prestep: fp16 or bf16, got {dt}")
-    T = q.shape[0]
-    if not 0 < T <= plan.max_tokens:
-        raise ValueError(f"paged_prestep: {T} rows, the plan is for 1 to {plan.max_tokens}")
-    if plan.requests == 0:
-        raise ValueError("paged_prestep: the plan has not been built")
-    cache = _pages_of(k_cache, P, H_kv, d)
-    packed = _PRESTEP_ARGS.pack(*_prestep_pointers(plan, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, v_cache, u_cache, T, cache, dt, dev), T, cache[0], P,
-                                H_q, H_kv, d, rotary_dim, rope_theta, rms_eps)
-    _launch(fns[0], "launch_khq_paged_prestep_" + _TYPES[dt], packed, dev)
-
-
-def _prestep_pointers(plan, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, v_cache, u_cache, T, cache, dt, dev):
-    H_q, H_kv, d = plan.H_q, plan.H_kv, plan.d
-    qp, q0, q1 = _rows(q, "q", H_q, d, T, dt, dev)
-    kp, k0, k1 = _rows(k, "k", H_kv, d, T, dt, dev)
-    vp, v0, v1 = _rows(v, "v", H_kv, d, T, dt, dev)
-    op, o0, o1 = _rows(q_out, "q_out", H_q, d, T, dt, dev)
-    kc, kc0, kc1, kc2 = _cache(k_cache, "k_cache", cache, dt, dev)
-    vc, vc0, vc1, vc2 = _cache(v_cache, "v_cache", cache, dt, dev)
-    uc, uc0, uc1, uc2 = _cache(u_cache, "u_cache", cache, dt, dev) if u_cache is not None else (0, 0, 0, 0)
-    qw = _ints(q_norm_w, "q_norm_w", d, dev, torch.float32) if q_norm_w is not None else 0
-    kw = _ints(k_norm_w, "k_norm_w", d, dev, torch.float32) if k_norm_w is not None else 0
-    return (qp, kp, vp, qw, kw, op, kc, vc, uc, plan._own[2], plan._own[3], q0, q1, k0, k1, v0, v1, o0, o1, kc0, kc1, kc2, vc0, vc1, vc2, uc0, uc1, uc2)
+    rc = plan._prestep(plan._at, q, k, v, q_norm_w, k_norm_w, q_out, k_cache, v_cache, u_cache, rotary_dim, rope_theta, rms_eps)
+    if rc != 0:
+        if rc == _NO_FIT:
+            T, dt, dev = _look_step(plan, "paged_prestep", q), q.dtype, plan.device
+            for name, t, heads in (("q", q, plan.H_q), ("k", k, plan.H_kv), ("v", v, plan.H_kv), ("q_out", q_out, plan.H_q)):
+                _look(t, name, (T, heads, plan.d), dt, dev)
+            _look_caches(plan, dt, k_cache=k_cache, v_cache=v_cache, u_cache=u_cache)
+            for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+                if w is not None:
+                    _look_flat(w, name, plan.d, torch.float32, dev)
+        check("launch_khq_paged_prestep_" + _TYPES[q.dtype], rc)
 
 
 def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scale: float, gate=None, lse=None, workspace=None) -> None:
@@ -207,32 +212,20 @@ def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scal
     pre-step has run).  ``out`` (tokens, H_q, d); ``gate`` (tokens, H_q, d): logits of the output gate, as in
     ``CudaOps.gqa_prefill``; ``lse`` (tokens, H_q) fp32: log of the sum of exponentials.  ``q`` and ``gate`` may be the two halves of an
     interleaved projection."""
-    dev, H_q, H_kv, d, P, dt = plan.device, plan.H_q, plan.H_kv, plan.d, plan.page_size, q.dtype
-    fns = plan._fns.get(dt)
-    if fns is None:
-        raise TypeError(f"paged_attention: fp16 or bf16, got {dt}")
-    T, B, M = q.shape[0], plan.requests, plan.max_pages
-    if not 0 < T <= plan.max_tokens:
-        raise ValueError(f"paged_attention: {T} rows, the plan is for 1 to {plan.max_tokens}")
-    if B == 0:
-        raise ValueError("paged_attention: the plan has not been built")
-    qp, q0, q1 = _rows(q, "q", H_q, d, T, dt, dev)
-    op, o0, o1 = _rows(out, "out", H_q, d, T, dt, dev)
-    gp, g0, g1 = _rows(gate, "gate", H_q, d, T, dt, dev) if gate is not None else (0, 0, 0)
-    cache = _pages_of(k_cache, P, H_kv, d)
-    kc, kc0, kc1, kc2 = _cache(k_cache, "k_cache", cache, dt, dev)
-    vc, vc0, vc1, vc2 = _cache(v_cache, "v_cache", cache, dt, dev)
-    st = block_table.stride()
-    if block_table.shape != (B, M) or st[1] != 1 or block_table.dtype is not torch.int32 or block_table.get_device() != dev:
-        _refuse(block_table, "block_table (the plan's)", (B, M), torch.int32, dev)
-    lp = _ints(lse, "lse", T * H_q, dev, torch.float32) if lse is not None else 0
-    if workspace is None:
-        ws, n_ws = plan._scratch
-    else:
-        ws, n_ws = _ints(workspace, "workspace", None, dev, torch.uint8), workspace.numel()
-    packed = _ATTN_ARGS.pack(qp, gp, kc, vc, block_table.data_ptr(), plan._own[5], op, lp, ws, plan._schedule_bytes, n_ws, q0, q1, g0, g1, o0, o1,
-                             kc0, kc1, kc2, vc0, vc1, vc2, st[0] if B > 1 else M, T, plan.max_tokens, plan.max_new, B, M, cache[0], P, H_q, H_kv, d, scale)
-    _launch(fns[1], "launch_khq_paged_attn_" + _TYPES[dt], packed, dev)
+    rc = plan._attention(plan._at, q, k_cache, v_cache, block_table, out, scale, gate, lse, workspace)
+    if rc != 0:
+        if rc == _NO_FIT:
+            T, dt, dev = _look_step(plan, "paged_attention", q), q.dtype, plan.device
+            for name, t in (("q", q), ("out", out), ("gate", gate)):
+                if t is not None:
+                    _look(t, name, (T, plan.H_q, plan.d), dt, dev)
+            _look_caches(plan, dt, k_cache=k_cache, v_cache=v_cache)
+            _look(block_table, "block_table (the plan's)", (plan.requests, plan.max_pages), torch.int32, dev)
+            if lse is not None:
+                _look_flat(lse, "lse", T * plan.H_q, torch.float32, dev)
+            if workspace is not None:
+                _look_flat(workspace, "workspace", None, torch.uint8, dev)
+        check("launch_khq_paged_attn_" + _TYPES[q.dtype], rc)
 
 
 # ---- a finished prompt: from pages to code words --------------------------------------------------------------------------------

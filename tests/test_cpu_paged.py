@@ -1,12 +1,14 @@
 """The paged operators' refusals and sizes through the C ABI: nothing here reaches a launch."""
 import ctypes
+import struct
 
 import pytest
 
 from bonsai_mojo_1bit_optimization_t4_cuda_b200 import lib as _lib
-from bonsai_mojo_1bit_optimization_t4_cuda_b200 import paged
 
 P = 4096  # an aligned address that is never used
+# the argument structs of include/khq_b200.h, field by field
+PLAN_ARGS, PRESTEP_ARGS, ATTN_ARGS = struct.Struct("@12PNq9i0q"), struct.Struct("@11P17q7i2f0q"), struct.Struct("@9P2N12qq10if0q")
 
 
 @pytest.fixture(scope="module")
@@ -47,7 +49,7 @@ def test_layouts_are_the_structs(tmp_path):
     exe = tmp_path / "sizes"
     subprocess.run(["gcc", "-I", str(Path(__file__).resolve().parent.parent / "include"), str(src), "-o", str(exe)], check=True)
     want = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
-    assert [paged._PLAN_ARGS.size, paged._PRESTEP_ARGS.size, paged._ATTN_ARGS.size] == want
+    assert [PLAN_ARGS.size, PRESTEP_ARGS.size, ATTN_ARGS.size] == want
 
 
 @pytest.mark.parametrize("change,code", [
@@ -58,7 +60,7 @@ def test_layouts_are_the_structs(tmp_path):
     (dict(ctx_lens=P + 2), -104), (dict(slots=P + 4), -104), (dict(schedule=P + 8), -104), (dict(schedule_bytes=64), -105),
 ])
 def test_plan_refusals(lib, change, code):
-    assert call(lib.launch_khq_paged_plan, paged._PLAN_ARGS, PLAN, **change) == code
+    assert call(lib.launch_khq_paged_plan, PLAN_ARGS, PLAN, **change) == code
 
 
 @pytest.mark.parametrize("change,code", [
@@ -69,7 +71,7 @@ def test_plan_refusals(lib, change, code):
 ])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_prestep_refusals(lib, dtype, change, code):
-    assert call(getattr(lib, "launch_khq_paged_prestep_" + dtype), paged._PRESTEP_ARGS, PRESTEP, **change) == code
+    assert call(getattr(lib, "launch_khq_paged_prestep_" + dtype), PRESTEP_ARGS, PRESTEP, **change) == code
 
 
 @pytest.mark.parametrize("change,code", [
@@ -81,7 +83,35 @@ def test_prestep_refusals(lib, dtype, change, code):
 ])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_attention_refusals(lib, dtype, change, code):
-    assert call(getattr(lib, "launch_khq_paged_attn_" + dtype), paged._ATTN_ARGS, ATTN, **change) == code
+    assert call(getattr(lib, "launch_khq_paged_attn_" + dtype), ATTN_ARGS, ATTN, **change) == code
+
+
+def test_extension_knows_the_plan(lib):
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200 import paged
+
+    assert paged._load_host().info_bytes() == ctypes.sizeof(paged._PlanInfo)
+
+
+def test_extension_refuses_what_is_no_tensor_of_the_plan(lib):
+    """Host tensors and other objects: refused before anything is launched."""
+    import torch
+
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200 import paged
+
+    host = paged._load_host()
+    info = paged._PlanInfo(0, 24, 4, 256, 16, 4, 64, 64, 2, 3)
+    at = ctypes.addressof(info)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    half = lambda *s: torch.zeros(*s, dtype=torch.float16)
+    q, k, c, table = half(5, 24, 256), half(5, 4, 256), half(9, 16, 4, 256), i32(2, 3)
+    assert host.build(at, i32(2), i32(2), table, None, None, None) == -1000
+    assert host.build(at, 7, i32(2), table, None, None, None) == -1000
+    assert host.prestep(at, q, k, k, None, None, q, c, c, None, 64, 1e7, 1e-6) == -1000
+    assert host.attention(at, q, c, c, table, q, 0.1, None, None, None) == -1000
+    assert host.attention(at, q.float(), c, c, table, q, 0.1, None, None, None) == -1000
+    for call in (lambda: host.build(at, 1), lambda: host.attention(at)):
+        with pytest.raises(TypeError):
+            call()
 
 
 def test_null_arguments(lib):
