@@ -115,8 +115,20 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         const int kept = end - first, held = pages(ctx);
         int t = 0, r = 0;
         if (b < B && pool) {
-            if (asked < 0) r = held;
-            else t = pages(ctx + kept) - held;
+            if (asked >= 0) {
+                t = pages(ctx + kept) - held;
+            } else {
+                r = held;
+                const int* row = a.table + b * a.table_stride;
+                if (held > 0 && row[held - 1] < 0) {  // its pages ran out: the last ones are none
+                    int lo = 0;
+                    while (lo < r) {
+                        const int mid = (lo + r) >> 1;
+                        if (row[mid] >= 0) lo = mid + 1;
+                        else r = mid;
+                    }
+                }
+            }
         }
         const int mine_t = t, mine_r = r;
         int total_t, total_r;

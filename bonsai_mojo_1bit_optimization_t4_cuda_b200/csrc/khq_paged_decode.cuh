@@ -60,8 +60,11 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int* const status = &g_paged_status;
     if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled layout needs a 1024-byte aligned base
-        if (tid == 0) atomicExch(status, 2);
         khq::pdl_wait();
+        if (tid == 0) {
+            atomicExch(status, 2);
+            p.meta[blockIdx.x].n = 0;
+        }
         return;
     }
     if (lane == 0) {

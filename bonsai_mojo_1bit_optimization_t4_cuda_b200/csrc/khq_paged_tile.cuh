@@ -133,7 +133,11 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const int rank = (int)(blockIdx.x & 1);  // the pair's first CTA has the MMA warp
     int* const status = &g_paged_status;
     if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled layouts need a 1024-byte aligned base; the same in both CTAs
-        if (tid == 0) atomicExch(status, 2);
+        khq::pdl_wait();
+        if (tid == 0) {
+            atomicExch(status, 2);
+            p.meta[blockIdx.x >> 1].n = 0;
+        }
         return;
     }
     const int tok = BR / p.n_rep, rows = tok * p.n_rep;  // new tokens and query rows of a CTA

@@ -372,7 +372,7 @@ int launch_khq_engine_step(khq_engine* engine, const khq_engine_layer* layers, c
  * slot = page * page_size + position % page_size, -1 behind the last row; info (8) int32: rows, pages taken, pages given back, pages
  * missing, rows dropped, pages free; schedule: what the attention runs from, schedule_bytes >= khq_b200_paged_schedule_bytes(...)
  * at 16 bytes (like positions and slots).  A row gets at most max_new tokens and all together max_tokens, the rest is dropped.  When pages run out, the table
- * gets -1 and so do the slots: such tokens are not stored and not attended.  Returns -100 (arguments), -103 (a page size, head counts, more than
+ * gets -1 and so do the slots: such tokens are not stored and not attended, and what ends later gives back what it got.  Returns -100 (arguments), -103 (a page size, head counts, more than
  * 16384 requests, 2^20 tokens or 2^30 tokens of a table row), -104 (alignment), -105 (schedule too small). */
 typedef struct khq_paged_plan_args {
     const void *ctx_lens, *new_lens;
@@ -407,9 +407,10 @@ int launch_khq_paged_prestep_bf16(const khq_paged_prestep_args* args, khq_stream
  *   out[t,h,:] = softmax_u(q[t,h] . K[u,h / n_rep] * scale) V[u,h / n_rep] * sigmoid(gate[t,h,:])      (gate NULL: without)
  * and, unless lse is NULL, lse[t,h] = log sum_u exp(q . K * scale) (tokens, H_q) fp32.  Softmax statistics, weights' sums and outputs in fp32;
  * the weights enter the product with V as 16-bit values.  A row that attends nothing (no page of it could be had) gets out 0 and lse
- * -inf.  Stale cache rows behind a request's last token are not attended, whatever they hold, NaN included.  schedule is
+ * -inf.  Stale cache rows behind a request's last token are not attended, whatever they hold, NaN included.  (The step's own
+ * tokens are part of the products: a V that is not finite reaches rows of the same request in front of it, with weight 0.)  schedule is
  * a plan's, max_tokens, max_new, requests, page_size, d and the head counts the same as there; `tokens` rows of q, gate,
- * out and lse exist (the plan must not have more).  Page numbers outside 0..n_pages-1 are not attended.  Rows behind the plan's last are left alone.
+ * out and lse exist, rows that the plan has beyond them are skipped.  Page numbers outside 0..n_pages-1 are not attended.  Rows behind the plan's last are left alone.
  * scale > 0.  workspace: khq_b200_paged_workspace_bytes(...) at 256 bytes; calls that may run at the same time need their own.  Returns -100, -103,
  * -104, -105, -107 / -108 (no tensor map). */
 typedef struct khq_paged_attn_args {

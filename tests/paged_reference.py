@@ -22,8 +22,10 @@ def plan(ctx, new, table, page, max_tokens, max_new, free=None, count=0):
         stack = free[:count]
         for b, n in enumerate(new):
             if n < 0:
-                stack += table[b][:pages(ctx[b])]
-                back += pages(ctx[b])
+                held = table[b][:pages(ctx[b])]
+                held = held[:held.index(-1)] if -1 in held else held  # its pages ran out
+                stack += held
+                back += len(held)
         for i in range(count, min(len(stack), len(free))):
             free[i] = stack[i]
         for b, n in enumerate(new):

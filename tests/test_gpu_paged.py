@@ -84,6 +84,23 @@ def test_plan_pages_run_out(cuda_ops):
     check_plan(ctx, new, 16, 300, 100, 12, seed=3)
 
 
+def test_plan_row_that_ran_out_ends(cuda_ops):
+    """Its pages go back, the ones that it never got do not."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan
+
+    table, free, count = i32([[-1] * 6, [-1] * 6]), i32([0, 1, 2, 3, 4]), i32([5])
+    t, f = table.tolist(), free.tolist()
+    plan, c, lens = PagedPlan(2, 96, 16, 24, 4, 256), 5, [0, 0]
+    for new in ([20, 70], [-1, 0], [0, -1], [40, 40]):
+        plan.build(i32(lens), i32(new), table, free, count)
+        want = ref.plan(lens, new, t, 16, 96, 96, f, c)
+        c = want["count"]
+        assert table.tolist() == t and free.tolist() == f and count.item() == c and plan.slots.tolist() == want["slots"]
+        assert plan.info[:5].tolist() == want["info"]
+        lens = [0 if n < 0 else x + n for x, n in zip(lens, new)]
+    assert c == 0 and sorted(x for row in t for x in row[:3]) == [-1, 0, 1, 2, 3, 4]  # every page is in use once
+
+
 def test_plan_drops_what_does_not_fit(cuda_ops):
     check_plan([3, 50, 7], [30, 20, 9], 16, 41, 25, 20, seed=4)
 
@@ -390,6 +407,64 @@ def test_attention_chunked_is_the_whole_prompt(cuda_ops):
     assert at == T
     # two kernels, each within its rounding of the weights and of the output: 4 half steps of values below 2
     assert (parts.float() - whole.float()).abs().max().item() <= 4 * 2.0 ** -11 * 2
+
+
+def test_attention_beyond_32_bits(cuda_ops):
+    """Pages whose first value lies more than 2^32 values into the cache."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan, paged_attention, paged_prestep
+
+    H_q, H_kv, d, page, pool = 16, 16, 256, 128, 8300
+    kc = torch.empty(pool, page, H_kv, d, dtype=torch.bfloat16, device="cuda")
+    vc = torch.empty_like(kc)
+    assert kc.numel() > 1 << 32
+    torch.manual_seed(0)
+    for new in (1, 70):
+        table, free, count = torch.full((2, 3), -1, dtype=torch.int32, device="cuda"), i32([0, 1, pool - 1, 5, pool - 2]), i32([5])
+        plan = PagedPlan(2, 400, page, H_q, H_kv, d)
+        lens = [0, 0]
+        for n in ([200, 100], [new, new]):
+            plan.build(i32(lens), i32(n), table, free, count)
+            T = sum(n)
+            q, k, v = (torch.randn(T, h, d, device="cuda").bfloat16() for h in (H_q, H_kv, H_kv))
+            paged_prestep(plan, q, k, v, None, None, q, kc, vc)
+            out = torch.empty_like(q)
+            paged_attention(plan, q, kc, vc, table, out, d ** -0.5)
+            want, _, tol, _ = ref.attention(q, kc, vc, table.tolist(), lens, n, d ** -0.5)
+            assert ((out.double() - want).abs() <= tol).all()
+            lens = [a + b for a, b in zip(lens, n)]
+        assert pool - 2 in table.tolist()[0] + table.tolist()[1]
+
+
+def test_attention_two_calls_at_once(cuda_ops):
+    """One plan, two layers on two streams, each with scratch memory of its own; and the same call again."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import paged_attention
+
+    torch.manual_seed(1)
+    ctx, new = [5000, 300, 40, 7000], [1, 130, 1, 30]
+    table, pool = make_table(ctx, new, 64, torch.Generator().manual_seed(3))
+    T, d_table = sum(new), i32(table)
+    plan = built(ctx, new, d_table, 64, 24, 4, 256)
+    layers = []
+    for _ in range(2):
+        q = torch.randn(T, 24, 256, device="cuda").half()
+        layers.append((q, *(torch.randn(pool, 64, 4, 256, device="cuda").half() for _ in range(2))))
+    single = []
+    for q, kc, vc in layers:
+        out = torch.empty_like(q)
+        paged_attention(plan, q, kc, vc, d_table, out, 1 / 16)
+        single.append(out)
+    scratch, streams = [None, plan.new_workspace()], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        outs = []
+        for (q, kc, vc), ws, s in zip(layers, scratch, streams):
+            with torch.cuda.stream(s):
+                out = torch.empty_like(q)
+                paged_attention(plan, q, kc, vc, d_table, out, 1 / 16, workspace=ws)
+                outs.append(out)
+        torch.cuda.synchronize()
+        for a, b in zip(outs, single):
+            assert torch.equal(a, b)
 
 
 def test_attention_on_another_stream(cuda_ops):
