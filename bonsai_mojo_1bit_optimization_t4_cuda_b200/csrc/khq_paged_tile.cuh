@@ -533,6 +533,9 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             if (lane == 0) khq::mbar_arrive(&bars[B_LSUM + quarter]);
             if (ok) ok = wait_for(&bars[B_LSUM + quarter], (uint32_t)(i & 1), status);
             if (ok) l_run += lsum[(grp ^ 1) * 128 + r];
+            // With three buffers the last scores only say that P V of block last - 3 is complete; the barrier of block last would still show the phase of
+            // last - 4 as long as last - 2 runs.  Behind block last - 1, last - 2 is complete too.
+            if (S::AHEAD == 2 && ok && last > 0) ok = wait_for(&bars[B_PVDONE + ((last - 1) & 1)], (uint32_t)(((last - 1) >> 1) & 1), status);
             if (ok) ok = wait_for(&bars[B_PVDONE + (last & 1)], (uint32_t)((last >> 1) & 1), status);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;

@@ -467,6 +467,26 @@ def test_attention_two_calls_at_once(cuda_ops):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("H_q,H_kv,d,ctx,new", [(17, 1, 128, [2295], [333]), (128, 1, 128, [2549, 2159], [306, 273]), (20, 4, 128, [900, 0, 70], [5, 300, 40]),
+                                               (24, 4, 256, [900, 0, 70], [5, 300, 40])])
+def test_attention_is_the_same_every_time(cuda_ops, H_q, H_kv, d, ctx, new):
+    """Segments of all lengths, shared and whole: bit for bit the same output in every run, whatever else the GPU's clocks do."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import paged_attention
+
+    torch.manual_seed(5)
+    table, pool = make_table(ctx, new, 64, torch.Generator().manual_seed(5))
+    T, d_table = sum(new), i32(table)
+    plan = built(ctx, new, d_table, 64, H_q, H_kv, d)
+    q = (2 * torch.randn(T, H_q, d, device="cuda")).bfloat16()
+    kc, vc = (torch.randn(pool, 64, H_kv, d, device="cuda").bfloat16() for _ in range(2))
+    outs = torch.empty(150, T, H_q, d, dtype=torch.bfloat16, device="cuda")
+    for i in range(len(outs)):
+        paged_attention(plan, q, kc, vc, d_table, outs[i], d ** -0.5)
+    want, _, tol, _ = ref.attention(q, kc, vc, table, ctx, new, d ** -0.5)
+    assert ((outs[0].double() - want).abs() <= tol).all()
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
+
+
 def test_attention_on_another_stream(cuda_ops):
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
