@@ -4,10 +4,9 @@
 
 namespace khq_paged {
 
-// The schedule in device memory: a header of 16 ints, then for the chunk kernel and for the decode kernel a list of items (in the order
-// of the requests) and the items' first key blocks counted through (cum[n_items] = the total).  Each kernel runs over H_kv copies of its
-// list, one kv head after the other.
-constexpr int SCHED_HEADER = 16;  // ints: [0] items, [1] key blocks of one kv head, for the chunk kernel; [2], [3] for the decode kernel
+// The schedule in device memory: for the chunk kernel and for the decode kernel where each worker begins, then a list of items (in the order
+// of the requests); the attention runs over H_kv copies of a list, one kv head after the other.  Behind them the items' first key blocks
+// counted through, where the plan has no room for them in shared memory.
 struct alignas(16) Item {
     int b, n_blocks, ntok, kv;  // request; key blocks (causal: up to the tile's last token); new tokens of the tile; the request's tokens
     int row0, pos0, pad[2];     // the tile's first row in the ragged tensors, that row's position
@@ -52,7 +51,7 @@ inline Schedule schedule_of(int requests, int max_tokens, int max_new, int H_q, 
     s.decodes = s.decode_tokens > 0;
     s.chunk_cap = s.chunks ? (long long)max_tokens / s.tile_tokens + requests : 0;
     s.decode_cap = s.decodes ? requests : 0;
-    s.chunk_starts = SCHED_HEADER;
+    s.chunk_starts = 0;
     s.decode_starts = s.chunk_starts + START_INTS * MAX_WORKERS;
     s.chunk_items = s.decode_starts + START_INTS * MAX_WORKERS;
     s.decode_items = s.chunk_items + ITEM_INTS * s.chunk_cap;

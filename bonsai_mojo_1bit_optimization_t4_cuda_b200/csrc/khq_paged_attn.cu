@@ -56,7 +56,7 @@ struct Params {
     uint16_t* out;
     float* lse;
     long long q_ts, q_hs, g_ts, g_hs, o_ts, o_hs, table_stride;
-    const int *table, *schedule;
+    const int* table;
     const Item* items;
     const Start* starts;
     float* records;
@@ -299,8 +299,8 @@ int launch_kernels(const khq_paged_attn_args& a, Params p, const Schedule& sched
     int rc = prepare_kernels<D, BF16>();
     unsigned char* const ws = static_cast<unsigned char*>(a.workspace);
     const auto of_kernel = [&](long long starts, long long items, size_t meta, size_t records) {
-        p.starts = reinterpret_cast<const Start*>(p.schedule + starts);
-        p.items = reinterpret_cast<const Item*>(p.schedule + items);
+        p.starts = reinterpret_cast<const Start*>(static_cast<const int*>(a.schedule) + starts);
+        p.items = reinterpret_cast<const Item*>(static_cast<const int*>(a.schedule) + items);
         p.meta = reinterpret_cast<Meta*>(ws + meta);
         p.records = reinterpret_cast<float*>(ws + records);
     };
@@ -383,7 +383,6 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     p.o_hs = a.out_stride[1];
     p.table_stride = a.table_stride;
     p.table = static_cast<const int*>(a.block_table);
-    p.schedule = static_cast<const int*>(a.schedule);
     p.tokens = a.tokens;
     p.max_pages = a.max_pages;
     p.n_pages = a.n_pages;

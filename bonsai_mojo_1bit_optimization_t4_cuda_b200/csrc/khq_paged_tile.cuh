@@ -193,190 +193,190 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     // 384 threads start with 168 registers each; the softmax threads, who hold 128 scores, take 208 and leave the others 88: together
     // the same 64512.  (Behind a point where both come together the compiler counts on the smaller number.)
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8) {
-        // ================================ producer of Q and K: the CTA's 64 keys of a block as [group][64 keys][128 B] =============
-        // boxes: 64 keys x all groups, or page x one group
-        const int per_half = p.page_shift >= 6 ? 1 : 1 << (6 - p.page_shift), boxes = p.page_shift >= 6 ? 1 : per_half * S::G;
-        int g = 0, i = 0;
-        bool ok = true;
-        Pages pages;
-        for (bool more = walk.begin(p, n_items); ok && more; more = walk.step(p, n_items), ++i) {
-            if (i > 0 && !(ok = tile::warp_wait(&bars[B_QFREE], (uint32_t)((i - 1) & 1), status))) break;
-            if (lane == 0) {
-                if (rank == 0) khq::mbar_arrive_expect_tx(&bars[B_QFULL], 2u * (uint32_t)(rows * 128 * S::G));
-#pragma unroll
-                for (int c = 0; c < S::G; ++c)
-                    asm volatile(
-                        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
-                            sbase + S::OFF_Q + c * (BR * 128)),
-                        "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(in_leader(&bars[B_QFULL])), "r"(0), "r"(walk.s.h * p.n_rep), "r"(walk.s.row0 + rank * tok),
-                        "r"(c)
-                        : "memory");
-            }
-            pages.begin(p, walk.s, walk.s.blk, log_per);
-            const bool ahead = walk.more();  // the next segment's queries to L2: their load waits for this one's last Q K^T
-            Segment next = walk.s;
-            if (ahead) next_segment(p, n_items, next);
-            for (int j = 0; j < walk.n; ++j, ++g) {
-                if (j == 0 && ahead && lane < S::G)
-                    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(0),
-                                 "r"(next.h * p.n_rep), "r"(next.row0 + rank * tok), "r"(lane)
-                                 : "memory");
-                const int s = g % S::STAGES, blk = walk.s.blk + j;
-                const int at = pages.seek(p, walk.s, blk, log_per);
-                // the page of this lane's box: keys rank * 64 + (lane / groups) pages further
-                const int mine = p.page_shift >= 6 ? at + ((rank * 64) >> p.page_shift) : at + rank * per_half + lane / S::G;
-                const int page = __shfl_sync(0xFFFFFFFFu, pages.now, mine & 31);
-                if (g >= S::STAGES && !(ok = tile::warp_wait(&bars[B_KFREE + s], (uint32_t)((g / S::STAGES - 1) & 1), status))) break;
-                if (rank == 0 && lane == 0) khq::mbar_arrive_expect_tx(&bars[B_KFULL + s], 2 * S::TILE_BYTES);
-                __syncwarp();
-                if (lane < boxes) {
-                    const int piece = lane / S::G, c = p.page_shift >= 6 ? 0 : lane % S::G;
-                    load_for_pair(sbase + S::OFF_K + s * S::TILE_BYTES + (p.page_shift >= 6 ? 0 : c * (64 * 128) + (piece << p.page_shift) * 128), &tm_k,
-                                  in_leader(&bars[B_KFULL + s]), p.page_shift == 7 ? rank * 64 : 0, c, walk.s.h, page);
-                }
-                __syncwarp();
-            }
-        }
-        // nothing may still be in flight when the pair leaves: the first CTA waits for the loads of both
-        if (!ok && rank == 0 && lane == 0)
-            for (int k = max(0, g - S::STAGES); k < g; ++k) wait_for(&bars[B_KFULL + k % S::STAGES], (uint32_t)((k / S::STAGES) & 1), status);
-    } else if (warp == 10) {
-        // ================================ producer of V: the CTA's d / 2 head dims as [group][128 keys][128 B] ======================
-        constexpr int VG = S::G / 2;
-        const int pieces = 1 << log_per, boxes = log_per == 0 ? 1 : pieces * VG;
-        int g = 0, lands = 0;
-        bool ok = true;
-        Pages pages;
-        for (bool more = walk.begin(p, n_items); ok && more; more = walk.step(p, n_items)) {
-            pages.begin(p, walk.s, walk.s.blk, log_per);
-            for (int j = 0; j < walk.n; ++j, ++g) {
-                const int s = g % S::STAGES, blk = walk.s.blk + j, key0 = blk * BC;
-                const int at = pages.seek(p, walk.s, blk, log_per);
-                const int page = __shfl_sync(0xFFFFFFFFu, pages.now, (log_per == 0 ? at : at + lane / VG) & 31);
-                if (g >= S::STAGES && !(ok = tile::warp_wait(&bars[B_VFREE + s], (uint32_t)((g / S::STAGES - 1) & 1), status))) break;
-                const bool tail = key0 + BC > walk.s.kv && (walk.s.kv & p.page_mask) != 0;
-                if (lane == 0) {
-                    if (tail) khq::mbar_arrive_expect_tx(&bars[B_VLAND], S::TILE_BYTES);
-                    else arrive_leader_expect(&bars[B_VFULL + s], S::TILE_BYTES);
-                }
-                __syncwarp();
-                const uint32_t dst = sbase + S::OFF_V + s * S::TILE_BYTES;
-                if (lane < boxes) {
-                    const int piece = log_per == 0 ? 0 : lane / VG, c = log_per == 0 ? 0 : lane % VG;
-                    const uint32_t to = dst + c * (BC * 128) + (piece << p.page_shift) * 128;
-                    if (tail) tma_load_5d(to, &tm_v, &bars[B_VLAND], 0, rank * VG + c, walk.s.h, page);
-                    else load_for_pair(to, &tm_v, in_leader(&bars[B_VFULL + s]), 0, rank * VG + c, walk.s.h, page);
-                }
-                __syncwarp();
-                if (tail) {
-                    if (!(ok = tile::warp_wait(&bars[B_VLAND], (uint32_t)(lands++ & 1), status))) break;
-                    // the rest of the request's last page
-                    const int r0 = walk.s.kv - key0, n = ((p.page_mask + 1) - (walk.s.kv & p.page_mask)) * 8;
-#pragma unroll
-                    for (int c = 0; c < VG; ++c)
-                        for (int k = lane; k < n; k += 32)
-                            *reinterpret_cast<uint4*>(smem + S::OFF_V + s * S::TILE_BYTES + c * (BC * 128) + r0 * 128 + k * 16) = make_uint4(0, 0, 0, 0);
-                    khq::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) arrive_leader(&bars[B_VFULL + s]);
-                }
-            }
-        }
-    } else if (warp == 9) {
-        // ================================ MMA issuer ==============================================
-        const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
-        if (rank == 1 && lane == 0) arrive_leader(&bars[B_PEER]);
-        if (rank == 0) {
-            const uint32_t one = elect_one();
-            constexpr uint32_t IDESC_S = instr_desc(2 * BR, BC, false, BF16), IDESC_O = instr_desc(2 * BR, D, true, BF16);
-            constexpr uint32_t HI = desc_hi(1024);  // Q, K (K-major) and V (MN-major): 1024 bytes between 8-row groups
-            const uint32_t q_lo = desc_lo(sbase + S::OFF_Q, 16), k_lo = desc_lo(sbase + S::OFF_K, 16);
-            const uint32_t v_lo = desc_lo(sbase + S::OFF_V, 128 * 128);  // leading offset: the next 64-column group
-            bool ok = true;
-            // A wait costs some 300 cycles even when its barrier completed long ago: a barrier is tested in front of the last instructions
-            // before its use, and waited for only if that came out negative.
-            uint32_t k_there = 0, p_there = 0, v_there = 0;
-            int k_of = -1;  // the block that k_there is about
-            const auto need = [&](uint32_t there, uint64_t* bar, uint32_t parity) {
-                if (ok && !__any_sync(0xFFFFFFFFu, there)) ok = warp_wait(bar, parity, status);
-            };
-            // S = Q K^T of block g; the tests are of the weights and V of the block that is multiplied next
-            const auto issue_qk = [&](int g, bool test) {
-                const uint32_t s_tmem = tmem + S::TM_S + (uint32_t)(g % S::BUFFERS) * BC;
-                const int ks_at = g % S::STAGES;
-                need(k_of == g ? k_there : 0u, &bars[B_KFULL + ks_at], (uint32_t)((g / S::STAGES) & 1));
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t k_at = k_lo + (uint32_t)ks_at * (S::TILE_BYTES >> 4);
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    // byte offsets / 16: next 64-dim group = rows * 128 bytes, next K step = 32 bytes
-                    const uint32_t oa = (uint32_t)((ks >> 2) * (BR * 128) + (ks & 3) * 32) >> 4;
-                    const uint32_t ob = (uint32_t)((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4;
-                    if (ks == 0) umma2_ss<0>(one, s_tmem, q_lo + oa, HI, k_at + ob, HI, IDESC_S);
-                    else umma2_ss<1>(one, s_tmem, q_lo + oa, HI, k_at + ob, HI, IDESC_S);
-                    if (ks == D / 16 - 5 && test) {
-                        const int n = g - S::AHEAD;
-                        p_there = mbar_test(&bars[B_PREADY + 2 * (n % S::BUFFERS)], (uint32_t)((n / S::BUFFERS) & 1));
-                        v_there = mbar_test(&bars[B_VFULL + n % S::STAGES], (uint32_t)((n / S::STAGES) & 1));
-                    }
-                }
-                umma2_commit(one, &bars[B_SFULL + g % S::BUFFERS]);
-                umma2_commit(one, &bars[B_KFREE + ks_at]);
-            };
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8) {
+            // ================================ producer of Q and K: the CTA's 64 keys of a block as [group][64 keys][128 B] =============
+            // boxes: 64 keys x all groups, or page x one group
+            const int per_half = p.page_shift >= 6 ? 1 : 1 << (6 - p.page_shift), boxes = p.page_shift >= 6 ? 1 : per_half * S::G;
             int g = 0, i = 0;
-            bool more = walk.begin(p, n_items);
-            if (more) ok = tile::warp_wait(&bars[B_PEER], 0u, status);
-            for (; ok && more; more = walk.step(p, n_items), ++i) {
-                ok = tile::warp_wait(&bars[B_QFULL], (uint32_t)(i & 1), status);
-                if (!ok) break;
-                for (int j = 0; ok && j < min(S::AHEAD, walk.n); ++j) issue_qk(g + j, false);
-                if (!ok) break;
-                if (walk.n <= S::AHEAD) umma2_commit(one, &bars[B_QFREE]);
-                for (int j = 0; j < walk.n; ++j, ++g) {
-                    const int s = g % S::BUFFERS, vs = g % S::STAGES;
-                    const uint32_t par = (uint32_t)((g / S::BUFFERS) & 1), v_par = (uint32_t)((g / S::STAGES) & 1);
-                    p_there = v_there = 0;
-                    if (j + S::AHEAD < walk.n) {
-                        issue_qk(g + S::AHEAD, true);
-                        if (!ok) break;
-                        if (j + S::AHEAD + 1 == walk.n) umma2_commit(one, &bars[B_QFREE]);
-                    }
-                    need(p_there, &bars[B_PREADY + 2 * s], par);
-                    if ((walk.s.blk + j + 1) * BC > walk.s.kv) {
-                        // zeros that the other CTA's V producer may have stored
-                        if (ok) ok = warp_wait_cluster(&bars[B_VFULL + vs], v_par, status);
-                    } else {
-                        need(v_there, &bars[B_VFULL + vs], v_par);
-                    }
-                    // the first P V of a segment overwrites O: the one before has been read
-                    if (j == 0 && i > 0 && ok) ok = tile::warp_wait(&bars[B_OFREE], (uint32_t)((i - 1) & 1), status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t v_at = v_lo + (uint32_t)vs * (S::TILE_BYTES >> 4), p_tmem = tmem + S::TM_S + (uint32_t)s * BC;
+            bool ok = true;
+            Pages pages;
+            for (bool more = walk.begin(p, n_items); ok && more; more = walk.step(p, n_items), ++i) {
+                if (i > 0 && !(ok = tile::warp_wait(&bars[B_QFREE], (uint32_t)((i - 1) & 1), status))) break;
+                if (lane == 0) {
+                    if (rank == 0) khq::mbar_arrive_expect_tx(&bars[B_QFULL], 2u * (uint32_t)(rows * 128 * S::G));
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        if (kk == 4) {  // the other half of the keys: its weights come while the first half is multiplied
-                            need(p_there, &bars[B_PREADY + 2 * s + 1], par);
-                            if (!ok) break;
-                            tc_fence_after();
-                        }
-                        umma2_ts(one, tmem, p_tmem + kk * 8, v_at + ((uint32_t)(kk * 2048) >> 4), HI, IDESC_O, kk > 0 ? 1u : (uint32_t)(j > 0));  // 16 keys = 2048 bytes
-                        if (kk == 1) p_there = mbar_test(&bars[B_PREADY + 2 * s + 1], par);
-                        if (kk == 5) {
-                            k_of = g + 1 + S::AHEAD;
-                            k_there = mbar_test(&bars[B_KFULL + k_of % S::STAGES], (uint32_t)((k_of / S::STAGES) & 1));
+                    for (int c = 0; c < S::G; ++c)
+                        asm volatile(
+                            "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+                                sbase + S::OFF_Q + c * (BR * 128)),
+                            "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(in_leader(&bars[B_QFULL])), "r"(0), "r"(walk.s.h * p.n_rep), "r"(walk.s.row0 + rank * tok),
+                            "r"(c)
+                            : "memory");
+                }
+                pages.begin(p, walk.s, walk.s.blk, log_per);
+                const bool ahead = walk.more();  // the next segment's queries to L2: their load waits for this one's last Q K^T
+                Segment next = walk.s;
+                if (ahead) next_segment(p, n_items, next);
+                for (int j = 0; j < walk.n; ++j, ++g) {
+                    if (j == 0 && ahead && lane < S::G)
+                        asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(0),
+                                     "r"(next.h * p.n_rep), "r"(next.row0 + rank * tok), "r"(lane)
+                                     : "memory");
+                    const int s = g % S::STAGES, blk = walk.s.blk + j;
+                    const int at = pages.seek(p, walk.s, blk, log_per);
+                    // the page of this lane's box: keys rank * 64 + (lane / groups) pages further
+                    const int mine = p.page_shift >= 6 ? at + ((rank * 64) >> p.page_shift) : at + rank * per_half + lane / S::G;
+                    const int page = __shfl_sync(0xFFFFFFFFu, pages.now, mine & 31);
+                    if (g >= S::STAGES && !(ok = tile::warp_wait(&bars[B_KFREE + s], (uint32_t)((g / S::STAGES - 1) & 1), status))) break;
+                    if (rank == 0 && lane == 0) khq::mbar_arrive_expect_tx(&bars[B_KFULL + s], 2 * S::TILE_BYTES);
+                    __syncwarp();
+                    if (lane < boxes) {
+                        const int piece = lane / S::G, c = p.page_shift >= 6 ? 0 : lane % S::G;
+                        load_for_pair(sbase + S::OFF_K + s * S::TILE_BYTES + (p.page_shift >= 6 ? 0 : c * (64 * 128) + (piece << p.page_shift) * 128), &tm_k,
+                                      in_leader(&bars[B_KFULL + s]), p.page_shift == 7 ? rank * 64 : 0, c, walk.s.h, page);
+                    }
+                    __syncwarp();
+                }
+            }
+            // nothing may still be in flight when the pair leaves: the first CTA waits for the loads of both
+            if (!ok && rank == 0 && lane == 0)
+                for (int k = max(0, g - S::STAGES); k < g; ++k) wait_for(&bars[B_KFULL + k % S::STAGES], (uint32_t)((k / S::STAGES) & 1), status);
+        } else if (warp == 10) {
+            // ================================ producer of V: the CTA's d / 2 head dims as [group][128 keys][128 B] ======================
+            constexpr int VG = S::G / 2;
+            const int pieces = 1 << log_per, boxes = log_per == 0 ? 1 : pieces * VG;
+            int g = 0, lands = 0;
+            bool ok = true;
+            Pages pages;
+            for (bool more = walk.begin(p, n_items); ok && more; more = walk.step(p, n_items)) {
+                pages.begin(p, walk.s, walk.s.blk, log_per);
+                for (int j = 0; j < walk.n; ++j, ++g) {
+                    const int s = g % S::STAGES, blk = walk.s.blk + j, key0 = blk * BC;
+                    const int at = pages.seek(p, walk.s, blk, log_per);
+                    const int page = __shfl_sync(0xFFFFFFFFu, pages.now, (log_per == 0 ? at : at + lane / VG) & 31);
+                    if (g >= S::STAGES && !(ok = tile::warp_wait(&bars[B_VFREE + s], (uint32_t)((g / S::STAGES - 1) & 1), status))) break;
+                    const bool tail = key0 + BC > walk.s.kv && (walk.s.kv & p.page_mask) != 0;
+                    if (lane == 0) {
+                        if (tail) khq::mbar_arrive_expect_tx(&bars[B_VLAND], S::TILE_BYTES);
+                        else arrive_leader_expect(&bars[B_VFULL + s], S::TILE_BYTES);
+                    }
+                    __syncwarp();
+                    const uint32_t dst = sbase + S::OFF_V + s * S::TILE_BYTES;
+                    if (lane < boxes) {
+                        const int piece = log_per == 0 ? 0 : lane / VG, c = log_per == 0 ? 0 : lane % VG;
+                        const uint32_t to = dst + c * (BC * 128) + (piece << p.page_shift) * 128;
+                        if (tail) tma_load_5d(to, &tm_v, &bars[B_VLAND], 0, rank * VG + c, walk.s.h, page);
+                        else load_for_pair(to, &tm_v, in_leader(&bars[B_VFULL + s]), 0, rank * VG + c, walk.s.h, page);
+                    }
+                    __syncwarp();
+                    if (tail) {
+                        if (!(ok = tile::warp_wait(&bars[B_VLAND], (uint32_t)(lands++ & 1), status))) break;
+                        // the rest of the request's last page
+                        const int r0 = walk.s.kv - key0, n = ((p.page_mask + 1) - (walk.s.kv & p.page_mask)) * 8;
+#pragma unroll
+                        for (int c = 0; c < VG; ++c)
+                            for (int k = lane; k < n; k += 32)
+                                *reinterpret_cast<uint4*>(smem + S::OFF_V + s * S::TILE_BYTES + c * (BC * 128) + r0 * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+                        khq::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) arrive_leader(&bars[B_VFULL + s]);
+                    }
+                }
+            }
+        } else if (warp == 9) {
+            // ================================ MMA issuer ==============================================
+            const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+            if (rank == 1 && lane == 0) arrive_leader(&bars[B_PEER]);
+            if (rank == 0) {
+                const uint32_t one = elect_one();
+                constexpr uint32_t IDESC_S = instr_desc(2 * BR, BC, false, BF16), IDESC_O = instr_desc(2 * BR, D, true, BF16);
+                constexpr uint32_t HI = desc_hi(1024);  // Q, K (K-major) and V (MN-major): 1024 bytes between 8-row groups
+                const uint32_t q_lo = desc_lo(sbase + S::OFF_Q, 16), k_lo = desc_lo(sbase + S::OFF_K, 16);
+                const uint32_t v_lo = desc_lo(sbase + S::OFF_V, 128 * 128);  // leading offset: the next 64-column group
+                bool ok = true;
+                // A wait costs some 300 cycles even when its barrier completed long ago: a barrier is tested in front of the last instructions
+                // before its use, and waited for only if that came out negative.
+                uint32_t k_there = 0, p_there = 0, v_there = 0;
+                int k_of = -1;  // the block that k_there is about
+                const auto need = [&](uint32_t there, uint64_t* bar, uint32_t parity) {
+                    if (ok && !__any_sync(0xFFFFFFFFu, there)) ok = warp_wait(bar, parity, status);
+                };
+                // S = Q K^T of block g; the tests are of the weights and V of the block that is multiplied next
+                const auto issue_qk = [&](int g, bool test) {
+                    const uint32_t s_tmem = tmem + S::TM_S + (uint32_t)(g % S::BUFFERS) * BC;
+                    const int ks_at = g % S::STAGES;
+                    need(k_of == g ? k_there : 0u, &bars[B_KFULL + ks_at], (uint32_t)((g / S::STAGES) & 1));
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t k_at = k_lo + (uint32_t)ks_at * (S::TILE_BYTES >> 4);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        // byte offsets / 16: next 64-dim group = rows * 128 bytes, next K step = 32 bytes
+                        const uint32_t oa = (uint32_t)((ks >> 2) * (BR * 128) + (ks & 3) * 32) >> 4;
+                        const uint32_t ob = (uint32_t)((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4;
+                        if (ks == 0) umma2_ss<0>(one, s_tmem, q_lo + oa, HI, k_at + ob, HI, IDESC_S);
+                        else umma2_ss<1>(one, s_tmem, q_lo + oa, HI, k_at + ob, HI, IDESC_S);
+                        if (ks == D / 16 - 5 && test) {
+                            const int n = g - S::AHEAD;
+                            p_there = mbar_test(&bars[B_PREADY + 2 * (n % S::BUFFERS)], (uint32_t)((n / S::BUFFERS) & 1));
+                            v_there = mbar_test(&bars[B_VFULL + n % S::STAGES], (uint32_t)((n / S::STAGES) & 1));
                         }
                     }
+                    umma2_commit(one, &bars[B_SFULL + g % S::BUFFERS]);
+                    umma2_commit(one, &bars[B_KFREE + ks_at]);
+                };
+                int g = 0, i = 0;
+                bool more = walk.begin(p, n_items);
+                if (more) ok = tile::warp_wait(&bars[B_PEER], 0u, status);
+                for (; ok && more; more = walk.step(p, n_items), ++i) {
+                    ok = tile::warp_wait(&bars[B_QFULL], (uint32_t)(i & 1), status);
                     if (!ok) break;
-                    umma2_commit(one, &bars[B_PVDONE + (g & 1)]);
-                    umma2_commit(one, &bars[B_VFREE + vs]);
+                    for (int j = 0; ok && j < min(S::AHEAD, walk.n); ++j) issue_qk(g + j, false);
+                    if (!ok) break;
+                    if (walk.n <= S::AHEAD) umma2_commit(one, &bars[B_QFREE]);
+                    for (int j = 0; j < walk.n; ++j, ++g) {
+                        const int s = g % S::BUFFERS, vs = g % S::STAGES;
+                        const uint32_t par = (uint32_t)((g / S::BUFFERS) & 1), v_par = (uint32_t)((g / S::STAGES) & 1);
+                        p_there = v_there = 0;
+                        if (j + S::AHEAD < walk.n) {
+                            issue_qk(g + S::AHEAD, true);
+                            if (!ok) break;
+                            if (j + S::AHEAD + 1 == walk.n) umma2_commit(one, &bars[B_QFREE]);
+                        }
+                        need(p_there, &bars[B_PREADY + 2 * s], par);
+                        if ((walk.s.blk + j + 1) * BC > walk.s.kv) {
+                            // zeros that the other CTA's V producer may have stored
+                            if (ok) ok = warp_wait_cluster(&bars[B_VFULL + vs], v_par, status);
+                        } else {
+                            need(v_there, &bars[B_VFULL + vs], v_par);
+                        }
+                        // the first P V of a segment overwrites O: the one before has been read
+                        if (j == 0 && i > 0 && ok) ok = tile::warp_wait(&bars[B_OFREE], (uint32_t)((i - 1) & 1), status);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t v_at = v_lo + (uint32_t)vs * (S::TILE_BYTES >> 4), p_tmem = tmem + S::TM_S + (uint32_t)s * BC;
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            if (kk == 4) {  // the other half of the keys: its weights come while the first half is multiplied
+                                need(p_there, &bars[B_PREADY + 2 * s + 1], par);
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            umma2_ts(one, tmem, p_tmem + kk * 8, v_at + ((uint32_t)(kk * 2048) >> 4), HI, IDESC_O, kk > 0 ? 1u : (uint32_t)(j > 0));  // 16 keys = 2048 bytes
+                            if (kk == 1) p_there = mbar_test(&bars[B_PREADY + 2 * s + 1], par);
+                            if (kk == 5) {
+                                k_of = g + 1 + S::AHEAD;
+                                k_there = mbar_test(&bars[B_KFULL + k_of % S::STAGES], (uint32_t)((k_of / S::STAGES) & 1));
+                            }
+                        }
+                        if (!ok) break;
+                        umma2_commit(one, &bars[B_PVDONE + (g & 1)]);
+                        umma2_commit(one, &bars[B_VFREE + vs]);
+                    }
                 }
             }
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ================================ softmax + epilogue ======================================

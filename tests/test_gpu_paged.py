@@ -212,12 +212,15 @@ def test_prestep_in_place_and_without_pages(cuda_ops):
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------------------------
-def attend(dtype, H_q, H_kv, d, page, ctx, new, gated=True, seed=0, poison=True, holes=(), layout="tokens", extra=2, scale=None, sharp=2.0, max_new=None):
+def attend(dtype, H_q, H_kv, d, page, ctx, new, gated=True, seed=0, poison=True, holes=(), layout="tokens", extra=2, scale=None, sharp=2.0, max_new=None,
+           shared=0):
     from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import paged_attention
 
     gen = torch.Generator(device="cuda").manual_seed(seed)
     dt, T = DT[dtype], sum(max(n, 0) for n in new)
     table, pool = make_table(ctx, new, page, torch.Generator().manual_seed(seed))
+    for row in table[1:]:  # the same pages at the front of every request
+        row[:shared] = table[0][:shared]
     cap = T + extra
     rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")
     q_gate = rand(cap, H_q, 2 * d)
@@ -331,6 +334,11 @@ def test_attention_missing_pages(cuda_ops, new):
     big = 1 << 30
     holes = [(0, 1, -1), (0, 3, big), (2, 0, -5), (2, 2, 2147483647)] + [(1, c, -1) for c in range(-(-(20 + new[1]) // 32))]
     attend("fp16", 24, 4, 256, 32, ctx, new, holes=holes, poison=False)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [30, 1, 100]])
+def test_attention_shared_pages(cuda_ops, new):
+    attend("bf16", 24, 4, 256, 32, [200, 130, 300], new, shared=4)
 
 
 @pytest.mark.parametrize("new", [1, 40])
