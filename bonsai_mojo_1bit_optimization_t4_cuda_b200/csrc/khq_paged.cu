@@ -15,7 +15,9 @@ namespace khq_paged {
 // ---- the plan of a step --------------------------------------------------------------------------
 // One cluster.  Every CTA sums up the lengths of all requests for itself (8 bytes a request) and keeps three running sums in shared
 // memory: tokens, pages taken, pages given back.  From those any moved page is found by bisection: the pages of ended requests are
-// read where they stand in their table rows, on top of the free ones.  Behind one barrier (the table is complete, the number of free pages has
+// read where they stand in their table rows, on top of the free ones.  The row of a request whose pages ran out once may have any mixture of
+// pages and none.  Whoever meets an entry that is no page tells the cluster, and behind the barrier the ended rows' pages are
+// counted, a warp per row, and moved once more (3172 requests, 100 ended rows of some 200 entries: counting them in every step cost 6 of 32 us).  Behind one barrier (the table is complete, the number of free pages has
 // been read and may be overwritten) two CTAs cut the step into the attention's items and its workers' stretches, and the others write
 // positions and slots.  Latency bounds it: a chain of some ten loads, scans and bisections (a bisection step in shared memory is 30 cycles,
 // in global memory some 500).  256 requests with a token each: 7.5 us; 3172 requests with 130 355 tokens: 25.
@@ -74,6 +76,20 @@ __device__ __forceinline__ void block_scan2(int& a, int& b, int* part, int& tota
     }
 }
 
+// The page behind `skip` others in a table row that has more of them, eight entries at a time.
+__device__ __forceinline__ int page_behind(const int* row, int held, int n_pages, int skip) {
+    int found = -1;
+    for (int i0 = 0; i0 < held && found < 0; i0 += 8) {
+        int e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = i0 + i < held ? row[i0 + i] : -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((unsigned)e[i] < (unsigned)n_pages && skip-- == 0) found = e[i];
+    }
+    return found;
+}
+
 // The last i in [0, n) with cum[i] <= x; cum[0] = 0 <= x < cum[n].
 __device__ __forceinline__ int find(const int* cum, int n, int x) {
     int lo = 0, hi = n;
@@ -85,12 +101,15 @@ __device__ __forceinline__ int find(const int* cum, int n, int x) {
     return lo;
 }
 
-__global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS) khq_paged_plan_kernel(const PlanArgs a) {
+__global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS, 1) khq_paged_plan_kernel(const PlanArgs a) {
     extern __shared__ int sums[];  // tokens, pages taken, pages given back: requests + 1 running sums each
     __shared__ int part[64];
     __shared__ Cut cuts[MAX_WORKERS + 1];
+    __shared__ int holes;                               // this CTA has met an entry that is no page in an ended request's row
+    __shared__ unsigned mixed[PLAN_MAX_REQUESTS / 32];  // bit by request: it has ended, and its pages are not its row's first entries
     int *const cu = sums, *const taken = cu + a.requests + 1, *const back = taken + a.requests + 1;
     const int tid = threadIdx.x, rank = blockIdx.x, B = a.requests, page = 1 << a.page_shift;
+    if (tid == 0) holes = 0;
     khq::pdl_wait();
     khq::pdl_trigger();
     const bool pool = a.free_list != nullptr;
@@ -113,23 +132,7 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         const int first = min(sum_tok + incl - min(n, a.max_tokens), a.max_tokens), end = min(sum_tok + incl, a.max_tokens);
         sum_tok = min(sum_tok + total, a.max_tokens);
         const int kept = end - first, held = pages(ctx);
-        int t = 0, r = 0;
-        if (b < B && pool) {
-            if (asked >= 0) {
-                t = pages(ctx + kept) - held;
-            } else {
-                r = held;
-                const int* row = a.table + b * a.table_stride;
-                if (held > 0 && row[held - 1] < 0) {  // its pages ran out: the last ones are none
-                    int lo = 0;
-                    while (lo < r) {
-                        const int mid = (lo + r) >> 1;
-                        if (row[mid] >= 0) lo = mid + 1;
-                        else r = mid;
-                    }
-                }
-            }
-        }
+        int t = b < B && pool && asked >= 0 ? pages(ctx + kept) - held : 0, r = b < B && pool && asked < 0 ? held : 0;
         const int mine_t = t, mine_r = r;
         int total_t, total_r;
         block_scan2(t, r, part, total_t, total_r);
@@ -152,49 +155,91 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         back[B] = sum_back;
     }
     __syncthreads();
-    // the free pages with the ones given back on top; pages are taken from the top
-    const int stack = count + sum_back;
-    const auto given_back = [&](int r) {
-        const int b = find(back, B, r);
-        return a.table[b * a.table_stride + (r - back[b])];
-    };
-    const auto nth_taken = [&](int j) {
-        const int i = stack - 1 - j;
-        return i < 0 ? -1 : i < count ? a.free_list[i] : given_back(i - count);
-    };
-    {
-        // ---- table entries and the free list ------------------------------------------------------------
-        const int at = rank * PLAN_THREADS + tid, step = PLAN_CTAS * PLAN_THREADS;
+    // ---- table entries and the free list: the free pages with the ones given back on top; pages are taken from the top ----
+    const bool some_back = sum_back > 0;
+    bool counted = false;  // `back` counts pages; at first the entries of the rows
+#pragma unroll 1
+    for (;;) {
+        const int stack = count + sum_back, at = rank * PLAN_THREADS + tid, step = PLAN_CTAS * PLAN_THREADS;
+        const auto given_back = [&](int r) {
+            const int b = find(back, B, r), nth = r - back[b];
+            const int* row = a.table + b * a.table_stride;
+            return counted && (mixed[b >> 5] >> (b & 31)) & 1u ? page_behind(row, pages(ctx_of(b)), a.n_pages, nth) : row[nth];
+        };
+        bool none = false;
         for (int j = at; j < sum_taken; j += step) {
-            const int b = find(taken, B, j);
-            a.table[b * a.table_stride + pages(ctx_of(b)) + (j - taken[b])] = nth_taken(j);
+            const int b = find(taken, B, j), i = stack - 1 - j;
+            a.table[b * a.table_stride + pages(ctx_of(b)) + (j - taken[b])] = i < 0 ? -1 : i < count ? a.free_list[i] : given_back(i - count);
         }
-        for (int r = at; r < sum_back; r += step)
-            if (count + r < a.n_pages) a.free_list[count + r] = given_back(r);
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    if (rank == 0) {
-        int drop = dropped, unused = 0, total_drop, u;
-        block_scan2(drop, unused, part, total_drop, u);
-        if (tid == 0) {
-            a.cu_new[B] = sum_tok;
-            a.info[0] = sum_tok;
-            a.info[1] = min(sum_taken, stack);
-            a.info[2] = sum_back;
-            a.info[3] = max(sum_taken - stack, 0);
-            a.info[4] = total_drop;
+        for (int r = at; r < sum_back; r += step) {
+            const int page_no = given_back(r);
+            none |= (unsigned)page_no >= (unsigned)a.n_pages;
+            if (count + r < a.n_pages) a.free_list[count + r] = page_no;
         }
+        if (none) holes = 1;
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (rank == 0 && !counted) {
+            int drop = dropped, unused = 0, total_drop, u;
+            block_scan2(drop, unused, part, total_drop, u);
+            if (tid == 0) {
+                a.cu_new[B] = sum_tok;
+                a.info[0] = sum_tok;
+                a.info[4] = total_drop;
+            }
+        }
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (counted || !some_back) break;
+        int met = 0;
+        if ((tid & 31) < PLAN_CTAS)
+            asm volatile("{.reg .b32 p; mapa.shared::cluster.u32 p, %1, %2; ld.shared::cluster.u32 %0, [p];}" : "=r"(met) : "r"(khq::smem_u32(&holes)), "r"(tid & 31) : "memory");
+        counted = __any_sync(0xFFFFFFFFu, met);
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // nobody's shared memory goes before it has been read
+        if (!counted) break;
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        sum_back = 0;
+        for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
+            const int b = b0 + tid, held = b < B && a.new_lens[b] < 0 ? pages(ctx_of(b)) : 0;
+            int r = 0, unused = 0, total, u;
+            unsigned mix = 0;
+            for (unsigned ended = __ballot_sync(0xFFFFFFFFu, held > 0); ended != 0; ended &= ended - 1) {
+                const int who = __ffs(ended) - 1, n_held = __shfl_sync(0xFFFFFFFFu, held, who);
+                const int* row = a.table + (b - (tid & 31) + who) * a.table_stride;
+                int n = 0, last = -1;  // this lane's pages, the last one's place
+#pragma unroll 8
+                for (int i = tid & 31; i < n_held; i += 32)
+                    if ((unsigned)row[i] < (unsigned)a.n_pages) {
+                        ++n;
+                        last = i;
+                    }
+                n = __reduce_add_sync(0xFFFFFFFFu, n);
+                last = __reduce_max_sync(0xFFFFFFFFu, last);
+                if ((tid & 31) == who) r = n;
+                if (last >= n) mix |= 1u << who;
+            }
+            if ((tid & 31) == 0 && b < B) mixed[b >> 5] = mix;
+            const int mine = r;
+            block_scan2(r, unused, part, total, u);
+            if (b < B) back[b] = sum_back + r - mine;
+            sum_back += total;
+        }
+        if (tid == 0) back[B] = sum_back;
+        __syncthreads();
     }
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     // the pages' sums have done their work: in their place the requests' lengths, and the items' sums
     int *const ctx_lens = back, *const first_item = taken;
     for (int b = tid; b < B; b += PLAN_THREADS) ctx_lens[b] = ctx_of(b);
     if (rank < 2) {
         // ---- the items of the attention: the first CTA the chunks', the second the decodes' ----------------
-        if (rank == 0 && tid == 0 && pool) {
-            const int left = max(stack - sum_taken, 0);
-            a.info[5] = left;
-            *a.free_count_out = left;
+        if (rank == 0 && tid == 0) {
+            const int stack = count + sum_back;
+            a.info[1] = min(sum_taken, stack);
+            a.info[2] = sum_back;
+            a.info[3] = max(sum_taken - stack, 0);
+            if (pool) {
+                const int left = min(max(stack - sum_taken, 0), a.n_pages);  // (a page that was free already makes one too many)
+                a.info[5] = left;
+                *a.free_count_out = left;
+            }
         }
         const bool decodes = rank == 1;
         const int tile_tokens = decodes ? a.sched.decode_tokens : a.sched.tile_tokens, tile_keys = decodes ? a.sched.decode_keys : TILE_KEYS;
@@ -329,6 +374,10 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
                 }
             }
         }
+    }
+    if (some_back && !counted) {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
 

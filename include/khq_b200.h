@@ -364,7 +364,7 @@ int launch_khq_engine_step(khq_engine* engine, const khq_engine_layer* layers, c
  *
  * The plan.  ctx_lens (requests): tokens that a request has in the cache; new_lens (requests): tokens that the step adds, -1: the
  * request has ended (its pages go back, once: its tokens are 0 in the next plan; pages that
- * requests share must not be given back by more than one), both int32.  block_table (requests, table_stride) int32: page numbers, max_pages of a row in
+ * requests share must not be given back by more than one; entries of its row that are no page of the pool are passed over), both int32.  block_table (requests, table_stride) int32: page numbers, max_pages of a row in
  * use.  free_list (n_pages) int32, free_count (1) int32: the free pages are the first free_count entries and are taken from the
  * end, for requests in row order; pages that come back stand behind the others, in row order, before any is taken, and are
  * written to free_list; free_count_out may be free_count.  free_list == NULL: the table has the new tokens' pages already.  Written: the

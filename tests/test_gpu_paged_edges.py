@@ -1,0 +1,102 @@
+"""The paged operators where a pool runs out, a row ends, or a value is not a number."""
+import random
+
+import pytest
+import torch
+
+import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _clean(cuda_ops):
+    yield
+    assert cuda_ops.lib.khq_b200_paged_status() == 0
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+class Pool:
+    """Steps of a plan on lists: what a request that ended had of the pool goes back, whatever its row has between the pages."""
+
+    def __init__(self, requests, width, page, n_pages):
+        self.page, self.n_pages = page, n_pages
+        self.table, self.lens = [[-1] * width for _ in range(requests)], [0] * requests
+        self.free = list(range(n_pages))
+
+    def step(self, new):
+        back = [p for row, c, n in zip(self.table, self.lens, new) if n < 0 for p in row[:-(-c // self.page)] if 0 <= p < self.n_pages]
+        self.free += back
+        taken = missing = 0
+        for b, n in enumerate(new):
+            for col in range(-(-self.lens[b] // self.page), -(-(self.lens[b] + n) // self.page) if n >= 0 else 0):
+                self.table[b][col] = self.free.pop() if self.free else -1
+                taken, missing = taken + (self.table[b][col] >= 0), missing + (self.table[b][col] < 0)
+        self.slots = [self.table[b][at // self.page] * self.page + at % self.page if self.table[b][at // self.page] >= 0 else -1
+                      for b, n in enumerate(new) for at in range(self.lens[b], self.lens[b] + max(n, 0))]
+        self.lens = [0 if n < 0 else c + n for c, n in zip(self.lens, new)]
+        return taken, len(back), missing
+
+    def check(self):
+        held = [p for row, c in zip(self.table, self.lens) for p in row[:-(-c // self.page)] if p >= 0]
+        assert sorted(held + self.free) == list(range(self.n_pages))  # every page exactly once
+
+
+def run_steps(requests, width, page, n_pages, steps, max_new):
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan
+
+    pool = Pool(requests, width, page, n_pages)
+    table, free, count = i32(pool.table), i32(pool.free), i32([n_pages])
+    plan = PagedPlan(requests, requests * max_new, page, 24, 4, 256, max_new=max_new)
+    for new in steps(pool):
+        lens = list(pool.lens)
+        plan.build(i32(lens), i32(new), table, free, count)
+        taken, back, missing = pool.step(new)
+        pool.check()
+        assert table.tolist() == pool.table
+        assert count.item() == len(pool.free) and free.tolist()[:len(pool.free)] == pool.free
+        assert plan.slots.tolist()[:len(pool.slots)] == pool.slots
+        assert plan.info.tolist()[:6] == [len(pool.slots), taken, back, missing, 0, len(pool.free)]
+    return pool
+
+
+def test_plan_row_with_a_hole_ends(cuda_ops):
+    """A request whose pages ran out takes more of them later: its row is page, none, page.  It ends, and another one takes its pages."""
+    pool = run_steps(2, 4, 16, 3, lambda _: [[20, 30], [-1, 10], [0, -1], [32, 0]], 64)
+    assert min(pool.table[0][:2]) >= 0 and len(pool.free) == 1
+    run_steps(2, 5, 16, 3, lambda _: [[16, 48], [-1, 0], [0, 16], [0, -1], [48, 0]], 64)
+
+
+def test_plan_row_with_holes_at_its_end(cuda_ops):
+    """page, none, page, none."""
+    run_steps(3, 8, 16, 3, lambda _: [[16, 16, 32], [-1, 0, 16], [0, 0, 16], [0, 0, -1], [32, 0, 0]], 64)
+
+
+@pytest.mark.parametrize("requests,n_pages,page,longest", [(5, 9, 16, 60), (40, 60, 32, 300), (1100, 900, 16, 40), (6, 700, 16, 5000)])
+def test_plan_pool_that_runs_out_again_and_again(cuda_ops, requests, n_pages, page, longest):
+    """Rows with holes of every kind, of up to some hundred pages, ending and starting anew."""
+    rng = random.Random(requests)
+    width = 4 * -(-longest // page) + 2
+
+    def steps(pool):
+        for _ in range(40):
+            new = [rng.choice([0, 0, 1, 1, rng.randint(1, longest), rng.randint(1, longest)]) for _ in range(requests)]
+            new = [-1 if c > 0 and (c + n > width * page or rng.random() < 0.15) else n for c, n in zip(pool.lens, new)]
+            yield new
+
+    run_steps(requests, width, page, n_pages, steps, longest)
+
+
+def test_plan_gives_back_pages_of_the_pool_only(cuda_ops):
+    """Numbers that the pool does not have, and more pages than it has room for."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan
+
+    plan = PagedPlan(2, 8, 16, 24, 4, 256)
+    free, count = i32([4, 2, 9, 9, 9]), i32([2])
+    plan.build(i32([64, 0]), i32([-1, 0]), i32([[1, 5, 1 << 30, 3], [-1] * 4]), free, count)
+    assert free.tolist()[:4] == [4, 2, 1, 3] and count.item() == 4 and plan.info.tolist()[:6] == [0, 0, 2, 0, 0, 4]
+    plan.build(i32([64, 0]), i32([-1, 0]), i32([[1, 3, 1, 3], [-1] * 4]), free, count)  # pages that are free already
+    assert count.item() == 5 and plan.info[5].item() == 5
