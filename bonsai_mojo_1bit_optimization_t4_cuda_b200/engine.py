@@ -344,7 +344,7 @@ class BatchEngine:
         from . import paged
 
         tokens, c = int(self.write_pos[seq]), int(self.boundary[seq])
-        pages = paged.prompt_pages(block_row, tokens, k_cache, v_cache, u_cache, H_KV, D)
+        pages = paged.prompt_pages(block_row, tokens, k_cache, v_cache, u_cache, H_KV, D, self.ring_k[layer].device)
         tb, P, st = self.tables[layer], self.pay[layer], current_stream()
         if c:
             runs = paged.page_runs(pages, c, u_cache, int(self.row_off[seq]))

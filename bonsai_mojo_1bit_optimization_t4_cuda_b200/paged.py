@@ -229,10 +229,12 @@ def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scal
 
 
 # ---- a finished prompt: from pages to code words --------------------------------------------------------------------------------
-def prompt_pages(block_row: torch.Tensor, tokens: int, k_cache, v_cache, u_cache, H_kv: int, d: int) -> torch.Tensor:
+def prompt_pages(block_row: torch.Tensor, tokens: int, k_cache, v_cache, u_cache, H_kv: int, d: int, device: Optional[torch.device] = None) -> torch.Tensor:
     """The pages of a prompt's ``tokens`` tokens as an int64 tensor, checked: fp16 caches of one shape with token-major pages (a page is a run of
     page_size * H_kv contiguous rows), ``u_cache`` and ``v_cache`` with the same distance between pages, page numbers inside the
-    cache.  Waits for the device (the page numbers)."""
+    cache, all on ``device`` (of the state that takes them; None: any GPU).  Waits for the device (the page numbers)."""
+    if block_row.device.type != "cuda" or (device is not None and block_row.device != device):
+        raise ValueError(f"block_row: wants a tensor on {device or 'a CUDA device'}, got {block_row.device}")
     shape = k_cache.shape
     for name, c in (("k_cache", k_cache), ("v_cache", v_cache), ("u_cache", u_cache)):
         if c.shape != shape or c.dim() != 4 or c.shape[2:] != (H_kv, d) or c.dtype is not torch.float16 or c.device != block_row.device:

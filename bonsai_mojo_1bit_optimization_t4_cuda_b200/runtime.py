@@ -553,7 +553,7 @@ class KhqRuntime:
             return False
         if tokens <= 0:
             raise ValueError(f"khq_adopt_pages: {tokens} tokens")
-        pages = paged.prompt_pages(block_row, tokens, k_cache, v_cache, u_cache, L.H_kv, L.D)
+        pages = paged.prompt_pages(block_row, tokens, k_cache, v_cache, u_cache, L.H_kv, L.D, L._t["ring_k"].device)
         Tn, kv = L._t, L.H_kv * L.D
         n_chunks = max(0, min(tokens // KHQ_CHUNK - 1, L.cap // KHQ_CHUNK))
         if n_chunks > 0:

@@ -1,0 +1,37 @@
+"""The paged operators' host side: what is refused before anything reaches the GPU."""
+import pytest
+import torch
+
+from bonsai_mojo_1bit_optimization_t4_cuda_b200 import paged
+
+
+def test_prompt_pages_on_the_host_are_refused():
+    """Their addresses would go to kernels."""
+    cache = torch.zeros(4, 16, 4, 256, dtype=torch.float16)
+    row = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
+    for device in (None, torch.device("cuda", 0)):
+        with pytest.raises(ValueError, match="CUDA|cuda:0"):
+            paged.prompt_pages(row, 40, cache, cache, cache, 4, 256, *([device] if device else []))
+
+
+def test_adopting_pages_on_the_host_is_refused():
+    """Through the runtime, before any launch."""
+    import numpy as np
+
+    import cases
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.runtime import KhqRuntime
+
+    class Ops:
+        def compress_runs(self, *args):
+            raise AssertionError("host addresses given to a kernel")
+
+    rng = np.random.default_rng(0)
+    k, v = cases.synth.make_kv(rng, 128, cases.synth.channel_scales(rng), cases.synth.channel_scales(rng))
+    table = cases.synth.make_tables(rng, 3, k.reshape(-1, 256), v.reshape(-1, 256))
+    rt = KhqRuntime(Ops(), device="cpu")
+    assert rt.khq_activate([table], max_seq=1024)
+    rt.khq_init_layer(3, 24, 4, 256)
+    cache = torch.zeros(5, 128, 4, 256, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        rt.khq_adopt_pages(3, cache, cache, cache, torch.arange(5, dtype=torch.int32), 640)
+    assert rt.layers[3].write_pos == 0
