@@ -177,6 +177,7 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
             if (count + r < a.n_pages) a.free_list[count + r] = page_no;
         }
         if (none) holes = 1;
+        __syncwarp();  // the cluster's barrier wants whole warps, and the loops above end lane by lane
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         if (rank == 0 && !counted) {
             int drop = dropped, unused = 0, total_drop, u;
@@ -187,12 +188,14 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
                 a.info[4] = total_drop;
             }
         }
+        __syncwarp();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (counted || !some_back) break;
         int met = 0;
         if ((tid & 31) < PLAN_CTAS)
             asm volatile("{.reg .b32 p; mapa.shared::cluster.u32 p, %1, %2; ld.shared::cluster.u32 %0, [p];}" : "=r"(met) : "r"(khq::smem_u32(&holes)), "r"(tid & 31) : "memory");
         counted = __any_sync(0xFFFFFFFFu, met);
+        __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // nobody's shared memory goes before it has been read
         if (!counted) break;
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -494,6 +494,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_leader(&bars[B_PREADY + 2 * buf + h]);
+                    __syncwarp();  // the next access to tensor memory wants the whole warp
                 }
                 l_run = (m_l == m_used ? l_run : l_run * exp2f(m_l - m_used)) + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
                 m_l = m_used;
@@ -541,6 +542,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             if (!ok) break;
             tc_fence_after();
             if (more) hole_next = fetch_holes(next, ((last + 1) ^ grp) & 1);  // (a block past the segment's end: no key, no hole)
+            __syncwarp();
             if (whole) {
                 const float inv = l_run > 0.0f ? 1.0f / l_run : l_run == 0.0f ? 0.0f : l_run;  // a NaN stays one
                 const auto spot = [&](int row, int chunk) { return reinterpret_cast<uint4*>(stage + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); };

@@ -100,3 +100,8 @@ def test_plan_gives_back_pages_of_the_pool_only(cuda_ops):
     assert free.tolist()[:4] == [4, 2, 1, 3] and count.item() == 4 and plan.info.tolist()[:6] == [0, 0, 2, 0, 0, 4]
     plan.build(i32([64, 0]), i32([-1, 0]), i32([[1, 3, 1, 3], [-1] * 4]), free, count)  # pages that are free already
     assert count.item() == 5 and plan.info[5].item() == 5
+
+
+def test_plan_lanes_with_more_to_move_than_others(cuda_ops):
+    """More pages than the plan's threads, by five: the last rounds of its loops are of a part of a warp."""
+    run_steps(3, 8300, 16, 8200, lambda _: [[16 * 8192 + 65, 0, 0], [-1, 1, 0], [0, 16 * 8192 + 65, 17]], 16 * 8192 + 65)
