@@ -65,6 +65,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
 __device__ __forceinline__ void arrive_leader_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(in_leader(bar)), "r"(bytes) : "memory");
 }
+// What this warp stored before is visible to who waits at cluster scope.  (An arrival says nothing of that beyond its own CTA otherwise.)
+__device__ __forceinline__ void release_to_leader(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
+}
 // The page numbers of a segment's blocks, 32 / per_block blocks in the lanes and as many on their way.  A block has `per_block` pages
 // (pages of 128 tokens and less).  n_pages stands for a page that is not there: a copy from it fills in zeros.
 struct Pages {
@@ -280,7 +284,7 @@ khq_paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                                 *reinterpret_cast<uint4*>(smem + S::OFF_V + s * S::TILE_BYTES + c * (BC * 128) + r0 * 128 + k * 16) = make_uint4(0, 0, 0, 0);
                         khq::fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) arrive_leader(&bars[B_VFULL + s]);
+                        if (lane == 0) release_to_leader(&bars[B_VFULL + s]);
                     }
                 }
             }

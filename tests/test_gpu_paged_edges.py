@@ -105,3 +105,28 @@ def test_plan_gives_back_pages_of_the_pool_only(cuda_ops):
 def test_plan_lanes_with_more_to_move_than_others(cuda_ops):
     """More pages than the plan's threads, by five: the last rounds of its loops are of a part of a warp."""
     run_steps(3, 8300, 16, 8200, lambda _: [[16 * 8192 + 65, 0, 0], [-1, 1, 0], [0, 16 * 8192 + 65, 17]], 16 * 8192 + 65)
+
+
+@pytest.mark.parametrize("d,H_q,H_kv", [(256, 24, 4), (128, 20, 4)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_attention_stale_rows_stay_out_every_time(cuda_ops, d, H_q, H_kv, page):
+    """NaN behind every request's last token, in both halves of the head dims: overwritten by either CTA of a pair before the products."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan, paged_attention
+
+    torch.manual_seed(page)
+    ctx, new = [0, 3, 100, 250, 511, 640], [129, 30, 27, 64, 130, 21]
+    counts = [-(-(c + n) // page) for c, n in zip(ctx, new)]
+    table = [list(range(sum(counts[:b]), sum(counts[:b + 1]))) + [-1] * (max(counts) - counts[b]) for b in range(len(ctx))]
+    T = sum(new)
+    plan = PagedPlan(len(ctx), T, page, H_q, H_kv, d).build(i32(ctx), i32(new), i32(table))
+    q = torch.randn(T, H_q, d, device="cuda").half()
+    kc, vc = (torch.randn(sum(counts), page, H_kv, d, device="cuda").half() for _ in range(2))
+    for b, (c, n) in enumerate(zip(ctx, new)):
+        if (c + n) % page:
+            kc[table[b][counts[b] - 1], (c + n) % page:], vc[table[b][counts[b] - 1], (c + n) % page:] = float("nan"), float("nan")
+    outs = torch.empty(40, T, H_q, d, dtype=torch.float16, device="cuda")
+    for o in outs:
+        paged_attention(plan, q, kc, vc, i32(table), o, d ** -0.5)
+    want, _, tol, _ = ref.attention(q, torch.nan_to_num(kc), torch.nan_to_num(vc), table, ctx, new, d ** -0.5)
+    assert ((outs[0].double() - want).abs() <= tol).all()
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
