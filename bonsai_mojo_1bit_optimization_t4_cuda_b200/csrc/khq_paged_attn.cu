@@ -325,7 +325,7 @@ int launch_kernels(const khq_paged_attn_args& a, Params p, const Schedule& sched
         if (rc == 0) rc = cache_map(&mv, a.v_cache, a.v_cache_stride, a.page_size, a.H_kv, D, a.n_pages, decode::box_tokens<D>(a.page_size), decode::box_groups<D>(a.page_size), BF16);
         if (rc != 0) return rc;
         err = khq::launch_pdl(decode::khq_paged_decode_kernel<D, BF16>, (unsigned)w.ctas, 0, (size_t)decode::Shape<D>::SMEM, stream,
-                              (unsigned)(decode::WARPS * 32), mk, mv, p, (int)sched.chunks);
+                              (unsigned)(decode::WARPS * 32), mk, mv, p);
         if (err != cudaSuccess) return static_cast<int>(err);
     }
     // rows of a request for the decode kernel, at most

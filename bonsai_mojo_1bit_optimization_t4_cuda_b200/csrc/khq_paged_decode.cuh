@@ -53,7 +53,7 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t at, uint32_t (&r)[4]) {
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(WARPS * 32, 1)
-khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p, int beside) {
+khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
     using S = Shape<D>;
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BARS);
@@ -73,10 +73,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         prefetch_map(warp & 1 ? &tm_k : &tm_v);
     }
     __syncthreads();
-    // Behind the chunk kernel of the same step (`beside`) there is nothing to wait for: that one lets this one start once everything before
-    // both is complete, and they share no row.  So these CTAs come in as the pairs run out of work.  The end waits instead, or the
-    // kernel behind could start before the chunk kernel is complete.
-    if (!beside) khq::pdl_wait();
+    khq::pdl_wait();
     khq::pdl_trigger();
 
     // ---- this CTA's stretch of the key blocks ------------------------------------------------------
@@ -84,10 +81,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     int n_items, length, share;
     const bool work = first_segment(p, blockIdx.x, in, n_items, length, share);
     if (tid == 0) p.meta[blockIdx.x].n = 0;  // overwritten below if a segment goes on in the next CTA
-    if (!work) {
-        if (beside) khq::pdl_wait();
-        return;
-    }
+    if (!work) return;
     // what is left of the stretch from the item's begin on, and the item's blocks in it
     const auto of_stretch = [](const Segment& s, int left) { return min(s.n_blocks, left - DECODE_OVER) - s.blk; };
     int left_in = length, n_in = of_stretch(in, length), left = length, n_seg = n_in;
@@ -351,7 +345,6 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             ++cur.blk;
         }
     }
-    if (beside) khq::pdl_wait();
 }
 
 }  // namespace decode
