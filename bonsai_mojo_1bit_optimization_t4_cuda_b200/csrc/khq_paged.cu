@@ -115,12 +115,13 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
     const bool pool = a.free_list != nullptr;
     const int count = pool ? min(max(*a.free_count, 0), a.n_pages) : 0;
     // table pages that `tokens` tokens lie in
-    const auto pages = [&](int tokens) { return (int)min(((long long)tokens + page - 1) >> a.page_shift, (long long)a.max_pages); };
-    const auto ctx_of = [&](int b) { return (int)min((long long)max(a.ctx_lens[b], 0), (long long)a.max_pages << a.page_shift); };
+    const int row_tokens = a.max_pages << a.page_shift;  // 2^30 at most
+    const auto pages = [&](int tokens) { return (tokens + page - 1) >> a.page_shift; };
+    const auto ctx_of = [&](int b) { return min(max(a.ctx_lens[b], 0), row_tokens); };
     int sum_tok = 0, sum_taken = 0, sum_back = 0, dropped = 0;
     int ctx_next = tid < B ? ctx_of(tid) : 0, asked_next = tid < B ? a.new_lens[tid] : 0;
     for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid, ctx = ctx_next, asked = asked_next, n = min(max(asked, 0), a.max_new);
+        const int b = b0 + tid, ctx = ctx_next, asked = asked_next, n = min(min(max(asked, 0), a.max_new), row_tokens - ctx);
         if (b + PLAN_THREADS < B) {  // the next round's lengths are on their way
             ctx_next = ctx_of(b + PLAN_THREADS);
             asked_next = a.new_lens[b + PLAN_THREADS];
@@ -359,7 +360,7 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
                 while (t < sum_tok && cu[b + 1] <= t) ++b;
                 pos[i] = t < sum_tok ? ctx_lens[b] + (t - cu[b]) : -1;
                 const int col = pos[i] >> a.page_shift;
-                page_of[i] = t < sum_tok && col < a.max_pages ? a.table[b * a.table_stride + col] : -1;
+                page_of[i] = t < sum_tok ? a.table[b * a.table_stride + col] : -1;
             }
             long long slot[4];
 #pragma unroll

@@ -164,7 +164,10 @@ class PagedPlan:
         """``ctx_lens`` / ``new_lens`` (requests) int32: tokens in the cache and tokens to come, -1: the request has ended.
         ``block_table`` (requests, max_pages) int32.  With ``free_list`` (n_pages) and ``free_count`` (1) int32 the pages of the new
         tokens are taken from it and entered in the table, and those of ended requests go back; ``free_count`` is brought up
-        to date, or left as it is and the new count written to ``free_count_out``.  Without, the table has all pages already."""
+        to date, or left as it is and the new count written to ``free_count_out``.  Without, the table has all pages already.
+
+        Tokens beyond a request's table row, ``max_new`` or ``max_tokens`` are dropped, not moved elsewhere: ``info[4]`` counts them and
+        ``cu_new`` has the rows that are left."""
         rc = self._build(self._at, ctx_lens, new_lens, block_table, free_list, free_count, free_count_out)
         if rc != 0:
             if rc == _NO_FIT:

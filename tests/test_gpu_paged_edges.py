@@ -130,3 +130,20 @@ def test_attention_stale_rows_stay_out_every_time(cuda_ops, d, H_q, H_kv, page):
     want, _, tol, _ = ref.attention(q, torch.nan_to_num(kc), torch.nan_to_num(vc), table, ctx, new, d ** -0.5)
     assert ((outs[0].double() - want).abs() <= tol).all()
     assert all(torch.equal(o, outs[0]) for o in outs[1:])
+
+
+@pytest.mark.parametrize("pool", [False, True])
+def test_plan_drops_what_the_row_has_no_room_for(cuda_ops, pool):
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan
+
+    plan = PagedPlan(4, 64, 16, 24, 4, 256)
+    table = i32([[0, 1], [2, 3], [4, 5], [6, -1 if pool else 7]])
+    args = (i32([7, 8, 9] + [-1] * 7), i32([3])) if pool else ()
+    plan.build(i32([30, 32, 40, 5]), i32([5, 3, 2, 20]), table, *args)
+    assert plan.cu_new.tolist() == [0, 2, 2, 2, 22]
+    assert plan.kv_lens.tolist() == [32, 32, 32, 25]
+    last = 9 if pool else 7
+    assert table.tolist() == [[0, 1], [2, 3], [4, 5], [6, last]]
+    assert plan.positions.tolist() == [30, 31] + list(range(5, 25)) + [-1] * 42
+    assert plan.slots.tolist() == [30, 31] + list(range(6 * 16 + 5, 7 * 16)) + list(range(last * 16, last * 16 + 9)) + [-1] * 42
+    assert plan.info.tolist()[:5] == [22, int(pool), 0, 0, 8]
