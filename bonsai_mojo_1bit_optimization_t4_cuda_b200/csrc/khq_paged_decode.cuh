@@ -309,7 +309,7 @@ khq_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 #pragma unroll
                     for (int v = 0; v < WARPS; ++v) {
                         const float2 a = ml[v * DECODE_ROWS + r];
-                        L += a.x == -INFINITY ? 0.0f : a.y * ex2_approx(a.x - Mr);
+                        L += a.x == -INFINITY ? a.y : a.y * ex2_approx(a.x - Mr);  // no maximum: 0, or NaN where every score was one
                     }
                     const int t = (r * p.rep_mul) >> 16, row = cur.row0 + t, head = cur.h * p.n_rep + (r - t * p.n_rep);
                     const bool live = row < p.tokens;

@@ -147,3 +147,44 @@ def test_plan_drops_what_the_row_has_no_room_for(cuda_ops, pool):
     assert plan.positions.tolist() == [30, 31] + list(range(5, 25)) + [-1] * 42
     assert plan.slots.tolist() == [30, 31] + list(range(6 * 16 + 5, 7 * 16)) + list(range(last * 16, last * 16 + 9)) + [-1] * 42
     assert plan.info.tolist()[:5] == [22, int(pool), 0, 0, 8]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H_q,H_kv,d,ctx,new", [(24, 4, 256, [100, 7, 300], [1, 1, 1]), (24, 4, 256, [20000, 9], [1, 2]), (20, 4, 128, [40, 9000], [2, 1]),
+                                               (24, 4, 256, [300, 20, 3000], [40, 1, 30]), (20, 4, 128, [5000], [90])])
+def test_attention_rows_that_are_not_numbers(cuda_ops, dtype, H_q, H_kv, d, ctx, new):
+    """A query of NaNs: NaN in that row's output and lse, nowhere else.  The same for a key of NaNs in the rows that attend it."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan, paged_attention
+
+    torch.manual_seed(len(ctx))
+    page, T = 64, sum(new)
+    counts = [-(-(c + n) // page) for c, n in zip(ctx, new)]
+    table = [list(range(sum(counts[:b]), sum(counts[:b + 1]))) + [-1] * (max(counts) - counts[b]) for b in range(len(ctx))]
+    pool = sum(counts)
+    plan = PagedPlan(len(ctx), T, page, H_q, H_kv, d, max_new=max(new)).build(i32(ctx), i32(new), i32(table))
+    q = torch.randn(T, H_q, d, device="cuda").to(dtype)
+    kc, vc = (torch.randn(pool, page, H_kv, d, device="cuda").to(dtype) for _ in range(2))
+    rows = sorted({0, T // 2, T - 1})
+    bad_q = q.clone()
+    for t in rows:
+        bad_q[t, (5 * t) % H_q] = float("nan")
+    want, want_lse, tol, lse_tol = ref.attention(q, kc, vc, table, ctx, new, d ** -0.5)
+
+    def check(queries, keys, bad):
+        out, lse = torch.full_like(q, 7.0), torch.full((T, H_q), 7.0, device="cuda")
+        paged_attention(plan, queries, keys, vc, i32(table), out, d ** -0.5, lse=lse)
+        assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+        assert ((out.double() - want).abs() <= tol)[~bad].all() and ((lse.double() - want_lse).abs() <= lse_tol)[~bad].all()
+
+    bad = torch.zeros(T, H_q, dtype=torch.bool, device="cuda")
+    for t in rows:
+        bad[t, (5 * t) % H_q] = True
+    check(bad_q, kc, bad)
+    # the first request's keys of the last kv head, from its first new token's page on: its rows of that head
+    first = ctx[0] // page
+    bad_k = kc.clone()
+    for col in range(first, counts[0]):
+        bad_k[table[0][col], :, H_kv - 1] = float("nan")
+    bad = torch.zeros_like(bad)
+    bad[:new[0], (H_kv - 1) * (H_q // H_kv):] = True
+    check(q, bad_k, bad)
