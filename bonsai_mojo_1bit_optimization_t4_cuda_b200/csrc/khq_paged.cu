@@ -118,7 +118,8 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
     const int row_tokens = a.max_pages << a.page_shift;  // 2^30 at most
     const auto pages = [&](int tokens) { return (tokens + page - 1) >> a.page_shift; };
     const auto ctx_of = [&](int b) { return min(max(a.ctx_lens[b], 0), row_tokens); };
-    int sum_tok = 0, sum_taken = 0, sum_back = 0, dropped = 0;
+    int sum_tok = 0, sum_taken = 0, sum_back = 0;
+    long long dropped = 0;
     int ctx_next = tid < B ? ctx_of(tid) : 0, asked_next = tid < B ? a.new_lens[tid] : 0;
     for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
         const int b = b0 + tid, ctx = ctx_next, asked = asked_next, n = min(min(max(asked, 0), a.max_new), row_tokens - ctx);
@@ -144,7 +145,7 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
             if (rank == 0) {
                 a.cu_new[b] = first;
                 a.kv_lens[b] = asked < 0 ? 0 : ctx + kept;
-                dropped += min(max(asked, 0) - kept, 1 << 20);
+                dropped += max(asked, 0) - kept;
             }
         }
         sum_taken += total_t;
@@ -181,12 +182,13 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
         __syncwarp();  // the cluster's barrier wants whole warps, and the loops above end lane by lane
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         if (rank == 0 && !counted) {
-            int drop = dropped, unused = 0, total_drop, u;
-            block_scan2(drop, unused, part, total_drop, u);
+            // the sum of 2^10 x 16 counts below 2^31, in words of 21 bits
+            int low = (int)(dropped & 0x1FFFFF), high = (int)(dropped >> 21), total_low, total_high;
+            block_scan2(low, high, part, total_low, total_high);
             if (tid == 0) {
                 a.cu_new[B] = sum_tok;
                 a.info[0] = sum_tok;
-                a.info[4] = total_drop;
+                a.info[4] = (int)min(((long long)total_high << 21) + total_low, 0x7FFFFFFFLL);
             }
         }
         __syncwarp();

@@ -188,3 +188,15 @@ def test_attention_rows_that_are_not_numbers(cuda_ops, dtype, H_q, H_kv, d, ctx,
     bad = torch.zeros_like(bad)
     bad[:new[0], (H_kv - 1) * (H_q // H_kv):] = True
     check(q, bad_k, bad)
+
+
+def test_plan_counts_dropped_rows_up_to_the_largest_int(cuda_ops):
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan
+
+    plan = PagedPlan(4096, 8, 16, 24, 4, 256)
+    lens, table = i32([0] * 4096), torch.zeros(4096, 4, dtype=torch.int32, device="cuda")
+    for new, dropped in ((1 << 20, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1), (1000, 4096 * 1000 - 8)):
+        plan.build(lens, i32([new] * 4096), table)
+        assert plan.info.tolist()[:5] == [8, 0, 0, 0, dropped]
+    plan.build(lens, i32([2 ** 31 - 1] + [0] * 4095), table)
+    assert plan.info[4].item() == 2 ** 31 - 1 - 8
