@@ -237,15 +237,14 @@ __global__ void __cluster_dims__(PLAN_CTAS, 1, 1) __launch_bounds__(PLAN_THREADS
     if (rank < 2) {
         // ---- the items of the attention: the first CTA the chunks', the second the decodes' ----------------
         if (rank == 0 && tid == 0) {
-            const int stack = count + sum_back;
+            const int stack = count + sum_back;  // 0 without a pool
+            const int left = pool ? min(max(stack - sum_taken, 0), a.n_pages) : 0;  // (a page that was free already makes one too many)
             a.info[1] = min(sum_taken, stack);
             a.info[2] = sum_back;
             a.info[3] = max(sum_taken - stack, 0);
-            if (pool) {
-                const int left = min(max(stack - sum_taken, 0), a.n_pages);  // (a page that was free already makes one too many)
-                a.info[5] = left;
-                *a.free_count_out = left;
-            }
+            a.info[5] = left;
+            a.info[6] = a.info[7] = 0;
+            if (pool) *a.free_count_out = left;
         }
         const bool decodes = rank == 1;
         const int tile_tokens = decodes ? a.sched.decode_tokens : a.sched.tile_tokens, tile_keys = decodes ? a.sched.decode_keys : TILE_KEYS;

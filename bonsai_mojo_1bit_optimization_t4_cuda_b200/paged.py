@@ -103,7 +103,7 @@ class PagedPlan:
     ``max_tokens``).  ``max_new`` also says which attention kernel serves the step, so a plan of decode steps is given its 1.
     After ``build`` (device tensors, rewritten by the next one): ``cu_new`` (requests + 1), ``kv_lens`` (requests),
     ``positions`` and ``slots`` (max_tokens; -1 behind the last token), ``info`` (tokens, pages taken, pages given back, pages missing,
-    tokens dropped, pages free, 0, 0).
+    tokens dropped, pages free, 0, 0; the pages' words are 0 without a free list).
 
     The attention's scratch memory belongs to the plan, so its calls belong on one stream; ``new_workspace`` makes scratch for another."""
 

@@ -371,7 +371,7 @@ int launch_khq_engine_step(khq_engine* engine, const khq_engine_layer* layers, c
  * table entries of taken pages; cu_new (requests + 1) int32, the first row of each request in the step's ragged tensors; kv_lens
  * (requests) int32, its tokens behind the step (0: ended); positions (max_tokens) int32 and slots (max_tokens) int64 of the rows,
  * slot = page * page_size + position % page_size, -1 behind the last row; info (8) int32: rows, pages taken, pages given back, pages
- * missing, rows dropped (2^31 - 1: that many or more), pages free; schedule: what the attention runs from, schedule_bytes >= khq_b200_paged_schedule_bytes(...)
+ * missing, rows dropped (2^31 - 1: that many or more), pages free (0 without a free_list), 0, 0; schedule: what the attention runs from, schedule_bytes >= khq_b200_paged_schedule_bytes(...)
  * at 16 bytes (like positions and slots).  A request gets at most max_new tokens and
  * what its table row has room for, and all together max_tokens; the rest is dropped (a length beyond the row counts as the row's end).  When pages run out, the table
  * gets -1 and so do the slots: such tokens are not stored and not attended, and what ends later gives back what it got.  Returns -100 (arguments), -103 (a page size, head counts, more than

@@ -200,3 +200,16 @@ def test_plan_counts_dropped_rows_up_to_the_largest_int(cuda_ops):
         assert plan.info.tolist()[:5] == [8, 0, 0, 0, dropped]
     plan.build(lens, i32([2 ** 31 - 1] + [0] * 4095), table)
     assert plan.info[4].item() == 2 ** 31 - 1 - 8
+
+
+def test_plan_without_a_pool_has_no_free_pages(cuda_ops):
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan
+
+    plan = PagedPlan(1, 8, 16, 24, 4, 256)
+    table = i32([[-1, -1]])
+    plan.info.fill_(77)
+    plan.build(i32([0]), i32([8]), table, i32([0, 1, 2]), i32([3]))
+    assert plan.info.tolist() == [8, 1, 0, 0, 0, 2, 0, 0]
+    plan.info.fill_(77)
+    plan.build(i32([0]), i32([8]), table)
+    assert plan.info.tolist() == [8, 0, 0, 0, 0, 0, 0, 0]
