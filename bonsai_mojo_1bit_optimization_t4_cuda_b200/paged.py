@@ -105,7 +105,8 @@ class PagedPlan:
     ``positions`` and ``slots`` (max_tokens; -1 behind the last token), ``info`` (tokens, pages taken, pages given back, pages missing,
     tokens dropped, pages free, 0, 0; the pages' words are 0 without a free list).
 
-    The attention's scratch memory belongs to the plan, so its calls belong on one stream; ``new_workspace`` makes scratch for another."""
+    The attention's scratch memory belongs to the plan, so its calls belong on one stream; ``new_workspace`` makes scratch for another.
+    The plan's tensors are, like any, the stream's that is current when it is made: a plan that others use is kept until they are done."""
 
     def __init__(self, max_requests: int, max_tokens: int, page_size: int, H_q: int, H_kv: int, d: int, max_new: Optional[int] = None, device="cuda"):
         self.lib = _lib.load()
@@ -125,7 +126,7 @@ class PagedPlan:
         empty = lambda count, dt: torch.empty(count, dtype=dt, device=torch.device("cuda", self.device))
         self._cu_new, self._kv_lens = empty(self.max_requests + 1, torch.int32), empty(self.max_requests, torch.int32)
         self.positions, self.slots = empty(self.max_tokens, torch.int32), empty(self.max_tokens, torch.int64)
-        self.info = torch.zeros(8, dtype=torch.int32, device=self.positions.device)
+        self.info = empty(8, torch.int32)  # (filled here, a build on another stream could be overtaken by it)
         self.schedule, self._workspace_bytes = empty(n, torch.uint8), w
         self.workspace = self.new_workspace()
         fn = lambda name: ctypes.cast(getattr(self.lib, name), ctypes.c_void_p).value

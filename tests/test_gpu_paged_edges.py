@@ -213,3 +213,19 @@ def test_plan_without_a_pool_has_no_free_pages(cuda_ops):
     plan.info.fill_(77)
     plan.build(i32([0]), i32([8]), table)
     assert plan.info.tolist() == [8, 0, 0, 0, 0, 0, 0, 0]
+
+
+def test_plan_built_at_once_on_another_stream(cuda_ops):
+    """The plan is made while the current stream is busy and built on an idle one: nothing of the first may come in behind."""
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.paged import PagedPlan
+
+    lens, new, table = i32([5, 0]), i32([3, 20]), i32([[0, -1], [1, 2]])
+    PagedPlan(2, 32, 16, 24, 4, 256).build(lens, new, table)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(20_000_000)  # some 10 ms
+    plan = PagedPlan(2, 32, 16, 24, 4, 256)
+    with torch.cuda.stream(side):
+        plan.build(lens, new, table)
+    torch.cuda.synchronize()
+    assert plan.info.tolist() == [23, 0, 0, 0, 0, 0, 0, 0] and plan.cu_new.tolist() == [0, 3, 23]
