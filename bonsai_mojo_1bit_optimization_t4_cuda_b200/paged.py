@@ -10,7 +10,8 @@ raw K and V of all requests of a server share a pool of pages until a prompt is 
 
 with ragged ``q`` (tokens, H_q, d), ``k`` and ``v`` (tokens, H_kv, d), request by request in the order of the lengths, and
 caches (n_pages, page_size, H_kv, d), fp16 or bf16.  Lengths, tables and slots stay on the device; nothing here waits for it or
-allocates, so a step can be captured into a CUDA graph at its largest size and replayed with other lengths.
+allocates, so a step can be captured into a CUDA graph at its largest size and replayed with other lengths.  Where the host waits for a step's results anyway,
+``plan.check()`` raises if a wait inside the attention's kernels has run out (they never hang).
 
 When a prompt is complete, ``KhqRuntime.khq_adopt_pages`` or ``BatchEngine.load_pages`` compresses its pages (fp16, K un-rotated from ``u_cache``)
 and the sequence goes on in code words.
@@ -23,7 +24,7 @@ from typing import Optional
 import torch
 
 from . import lib as _lib
-from .lib import KhqLibraryError, check
+from .lib import KhqLaunchError, KhqLibraryError, check
 
 _TYPES = {torch.float16: "fp16", torch.bfloat16: "bf16"}
 _NO_FIT = -1000  # of the extension: a tensor is not what the plan asks for
@@ -54,6 +55,22 @@ def _load_host():
             raise KhqLibraryError("the paged operators' extension is stale: build it anew")
         _host = host
     return _host
+
+
+# ---- waits that ran out ------------------------------------------------------------------------------------------------------
+def _read_status(device) -> int:
+    with torch.cuda.device(device):
+        torch.cuda.current_stream().synchronize()
+        return int(_lib.load().khq_b200_paged_status())
+
+
+def check_status(device=None) -> None:
+    """Raises ``KhqLaunchError`` if a wait inside a ``paged_attention`` on ``device`` (None: the current one) has run out since the last look: the
+    kernels then go on without data, and outputs since that look are not to be trusted.  Waits for the current stream, so it belongs where the host
+    waits anyway, and not into a capture.  The word is the GPU's, shared by all plans on it, and is cleared."""
+    st = _read_status(device)
+    if st != 0:
+        raise KhqLaunchError("paged_attention: outputs since the last look are not to be trusted, khq_b200_paged_status", st)
 
 
 # ---- what does not fit, in words (a call comes here only when the extension has refused it) ------------------------------------------------
@@ -160,6 +177,10 @@ class PagedPlan:
     def kv_lens(self) -> torch.Tensor:
         return self._kv_lens[:self.requests]
 
+    def check(self) -> None:
+        """``check_status`` of the plan's GPU."""
+        check_status(self.device)
+
     def build(self, ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_list: Optional[torch.Tensor] = None,
               free_count: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None) -> "PagedPlan":
         """``ctx_lens`` / ``new_lens`` (requests) int32: tokens in the cache and tokens to come, -1: the request has ended.
@@ -236,7 +257,8 @@ def paged_attention(plan: PagedPlan, q, k_cache, v_cache, block_table, out, scal
 def prompt_pages(block_row: torch.Tensor, tokens: int, k_cache, v_cache, u_cache, H_kv: int, d: int, device: Optional[torch.device] = None) -> torch.Tensor:
     """The pages of a prompt's ``tokens`` tokens as an int64 tensor, checked: fp16 caches of one shape with token-major pages (a page is a run of
     page_size * H_kv contiguous rows), ``u_cache`` and ``v_cache`` with the same distance between pages, page numbers inside the
-    cache, all on ``device`` (of the state that takes them; None: any GPU).  Waits for the device (the page numbers)."""
+    cache, all on ``device`` (of the state that takes them; None: any GPU).  Waits for the device (the page numbers), and raises if a wait of the attention
+    that the prompt went through may have run out (``check_status``)."""
     if block_row.device.type != "cuda" or (device is not None and block_row.device != device):
         raise ValueError(f"block_row: wants a tensor on {device or 'a CUDA device'}, got {block_row.device}")
     shape = k_cache.shape
@@ -256,6 +278,7 @@ def prompt_pages(block_row: torch.Tensor, tokens: int, k_cache, v_cache, u_cache
     pages = block_row[:n].long()
     if n and bool(((pages < 0) | (pages >= shape[0])).any()):
         raise ValueError("block_row: a page that is not in the cache")
+    check_status(pages.device)
     return pages
 
 

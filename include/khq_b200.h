@@ -428,7 +428,8 @@ typedef struct khq_paged_attn_args {
 size_t khq_b200_paged_workspace_bytes(int max_new, int H_q, int H_kv, int d); /* of the current device; 0: bad arguments */
 int launch_khq_paged_attn_fp16(const khq_paged_attn_args* args, khq_stream_t stream);
 int launch_khq_paged_attn_bf16(const khq_paged_attn_args* args, khq_stream_t stream);
-/* Reads and clears the status word of the paged attention on the current device (synchronises): 0 clean, 1 a bounded wait ran out, 2
+/* Reads and clears the status word of the paged attention on the current device, by a blocking copy on the default stream: call it where the
+ * attention's streams have been waited for.  0 clean, 1 a bounded wait ran out, 2
  * misaligned shared memory. */
 int khq_b200_paged_status(void);
 

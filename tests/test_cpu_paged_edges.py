@@ -35,3 +35,19 @@ def test_adopting_pages_on_the_host_is_refused():
     with pytest.raises(ValueError):
         rt.khq_adopt_pages(3, cache, cache, cache, torch.arange(5, dtype=torch.int32), 640)
     assert rt.layers[3].write_pos == 0
+
+
+@pytest.mark.parametrize("word", [1, 2, -1])
+def test_a_wait_that_ran_out_is_reported(monkeypatch, word):
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.lib import KhqLaunchError
+
+    seen = []
+    monkeypatch.setattr(paged, "_read_status", lambda device: seen.append(device) or word)
+    plan = object.__new__(paged.PagedPlan)
+    plan.device = 3
+    with pytest.raises(KhqLaunchError, match="not to be trusted") as e:
+        plan.check()
+    assert e.value.code == word and seen == [3]
+    monkeypatch.setattr(paged, "_read_status", lambda device: 0)
+    plan.check()
+    paged.check_status()

@@ -229,3 +229,33 @@ def test_plan_built_at_once_on_another_stream(cuda_ops):
         plan.build(lens, new, table)
     torch.cuda.synchronize()
     assert plan.info.tolist() == [23, 0, 0, 0, 0, 0, 0, 0] and plan.cu_new.tolist() == [0, 3, 23]
+
+
+def test_pages_behind_a_wait_that_ran_out_are_not_compressed(cuda_ops, monkeypatch):
+    import numpy as np
+
+    import cases
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200 import paged
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.engine import BatchEngine
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.lib import KhqLaunchError
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.runtime import KhqRuntime
+
+    paged.check_status()  # clean, on this GPU
+    rng = np.random.default_rng(0)
+    k, v = cases.synth.make_kv(rng, 128, cases.synth.channel_scales(rng), cases.synth.channel_scales(rng))
+    tables = cases.synth.make_tables(rng, 3, k.reshape(-1, 256), v.reshape(-1, 256), vq_scale=1.0 / 16.0)
+    rt = KhqRuntime(cuda_ops)
+    assert rt.khq_activate([tables], max_seq=512)
+    rt.khq_init_layer(3, 24, 4, 256)
+    eng = BatchEngine([tables], [128], [128])
+    kc, vc, uc = (torch.ones(3, 128, 4, 256, dtype=torch.float16, device="cuda") for _ in range(3))
+    word = [1]
+    monkeypatch.setattr(paged, "_read_status", lambda device: word[0])
+    with pytest.raises(KhqLaunchError):
+        rt.khq_adopt_pages(3, kc, vc, uc, i32([0, 1, 2]), 300)
+    with pytest.raises(KhqLaunchError):
+        eng.load_pages(0, 0, kc, vc, uc, i32([0, 1]))
+    assert rt.layers[3].write_pos == 0 and (eng.ring_k[0] == 0).all() and (eng.pay[0]["k_mask"] == 0).all()
+    word[0] = 0
+    assert rt.khq_adopt_pages(3, kc, vc, uc, i32([0, 1, 2]), 300)
+    eng.load_pages(0, 0, kc, vc, uc, i32([0, 1]))
