@@ -19,11 +19,12 @@ and the sequence goes on in code words.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from typing import Optional
 
 import torch
 
-from . import lib as _lib
+from . import build, lib as _lib
 from .lib import KhqLaunchError, KhqLibraryError, check
 
 _TYPES = {torch.float16: "fp16", torch.bfloat16: "bf16"}
@@ -46,10 +47,12 @@ def _load_host():
     """The extension that looks at a call's tensors and launches (csrc/khq_paged_host.cpp)."""
     global _host
     if _host is None:
+        path = build.host_path()
         try:
-            from . import _khq_paged_host as host
+            spec = importlib.util.spec_from_file_location("_khq_paged_host", path)
+            host = importlib.util.module_from_spec(spec)
         except ImportError as e:
-            raise KhqLibraryError(f"the paged operators' extension cannot be loaded ({e}): build it with "
+            raise KhqLibraryError(f"the paged operators' extension cannot be loaded ({e}): build it for this torch and Python with "
                                   "`python -m bonsai_mojo_1bit_optimization_t4_cuda_b200.build`") from e
         if host.info_bytes() != ctypes.sizeof(_PlanInfo):
             raise KhqLibraryError("the paged operators' extension is stale: build it anew")

@@ -51,3 +51,36 @@ def test_a_wait_that_ran_out_is_reported(monkeypatch, word):
     monkeypatch.setattr(paged, "_read_status", lambda device: 0)
     plan.check()
     paged.check_status()
+
+
+def test_the_library_is_built_without_torch(monkeypatch, tmp_path, capsys):
+    """One source stands for all: what matters is that nvcc runs and that the extension's absence ends nothing."""
+    import sys
+
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200 import build
+
+    monkeypatch.setattr(build, "LIB_PATH", tmp_path / build.LIB_NAME)
+    monkeypatch.setattr(build, "SOURCES", ["khq_calib.cu"])
+    monkeypatch.setattr(build, "host_path", lambda: tmp_path / "host.so", raising=False)
+    monkeypatch.setattr(build, "HOST_PATH", tmp_path / "host.so", raising=False)
+    monkeypatch.setitem(sys.modules, "torch", None)  # an import of it raises
+    assert build.build() == build.LIB_PATH
+    assert (tmp_path / build.LIB_NAME).exists() and not (tmp_path / "host.so").exists()
+    assert "extension was not built" in capsys.readouterr().err
+    with pytest.raises(ImportError):
+        build.build_host()
+
+
+def test_an_extension_for_another_torch_or_python_is_not_taken(monkeypatch):
+    from importlib import metadata
+
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200 import build
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200.lib import KhqLibraryError
+
+    build.build_host()
+    assert not build.needs_host_build()
+    monkeypatch.setattr(metadata, "version", lambda name: "1.0.0")
+    assert build.needs_host_build()
+    monkeypatch.setattr(paged, "_host", None)
+    with pytest.raises(KhqLibraryError, match="build it"):
+        paged._load_host()
