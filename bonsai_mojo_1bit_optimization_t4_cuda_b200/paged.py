@@ -98,6 +98,8 @@ def _look_flat(t, name: str, numel: Optional[int], dtype, device: int) -> None:
 
 
 def _look_step(plan: "PagedPlan", what: str, q) -> int:
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"{what}: q: a tensor, got {type(q).__name__}")
     if q.dtype not in _TYPES:
         raise TypeError(f"{what}: fp16 or bf16, got {q.dtype}")
     T = q.shape[0] if q.dim() else 0
@@ -201,14 +203,20 @@ class PagedPlan:
         return self
 
     def _look_at_build(self, ctx_lens, new_lens, block_table, free_list, free_count, free_count_out) -> None:
+        if not isinstance(ctx_lens, torch.Tensor):
+            raise TypeError(f"ctx_lens: a tensor, got {type(ctx_lens).__name__}")
         dev, n = self.device, ctx_lens.numel()
         if not 0 < n <= self.max_requests:
             raise ValueError(f"PagedPlan.build: {n} requests, built for 1 to {self.max_requests}")
         _look_flat(ctx_lens, "ctx_lens", n, torch.int32, dev)
         _look_flat(new_lens, "new_lens", n, torch.int32, dev)
         _look(block_table, "block_table", (n, None), torch.int32, dev)
+        if block_table.shape[1] == 0:
+            raise ValueError("block_table: has no columns")
         if free_list is None:
-            raise ValueError("PagedPlan.build: free_count without free_list")
+            if free_count is not None or free_count_out is not None:
+                raise ValueError("PagedPlan.build: free_count without free_list")
+            return
         if free_count is None:
             raise ValueError("PagedPlan.build: free_list without free_count")
         _look_flat(free_list, "free_list", None, torch.int32, dev)

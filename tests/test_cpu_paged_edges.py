@@ -84,3 +84,28 @@ def test_an_extension_for_another_torch_or_python_is_not_taken(monkeypatch):
     monkeypatch.setattr(paged, "_host", None)
     with pytest.raises(KhqLibraryError, match="build it"):
         paged._load_host()
+
+
+def test_refusals_say_what_does_not_fit():
+    plan = object.__new__(paged.PagedPlan)
+    plan.device, plan.max_requests, plan.max_tokens = -1, 4, 8  # -1: where host tensors are
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    for args, error, text in (
+        ((i32(2), i32(2), i32(2, 0), None, None, None), ValueError, "block_table"),
+        ((i32(2), i32(3), i32(2, 1), None, None, None), ValueError, "new_lens"),
+        ((i32(2), i32(2), i32(2, 1), None, i32(1), None), ValueError, "free_count without"),
+        ((i32(2), i32(2), i32(2, 1), None, None, i32(1)), ValueError, "free_count without"),
+        ((i32(2), i32(2), i32(2, 1), i32(5), None, None), ValueError, "free_list without"),
+        ((i32(2), i32(2), i32(2, 1), i32(5), i32(2), None), ValueError, "free_count"),
+        (([0, 0], i32(2), i32(2, 1), None, None, None), TypeError, "ctx_lens"),
+        ((i32(2), [0, 0], i32(2, 1), None, None, None), TypeError, "new_lens"),
+    ):
+        with pytest.raises(error, match=text):
+            plan._look_at_build(*args)
+    plan._look_at_build(i32(2), i32(2), i32(2, 1), None, None, None)  # nothing to say
+    plan._prestep = plan._attention = lambda *args: paged._NO_FIT
+    plan._at = 0
+    with pytest.raises(TypeError, match="q"):
+        paged.paged_prestep(plan, 7, None, None, None, None, None, None, None)
+    with pytest.raises(TypeError, match="q"):
+        paged.paged_attention(plan, None, None, None, None, None, 0.1)
