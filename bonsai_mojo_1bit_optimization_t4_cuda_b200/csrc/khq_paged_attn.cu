@@ -353,7 +353,8 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     if (a.tokens <= 0 || a.max_tokens <= 0 || a.max_new <= 0 || a.requests <= 0 || a.max_pages <= 0 || a.n_pages <= 0 || a.H_q <= 0 || a.H_kv <= 0 || !a.q ||
         !a.k_cache || !a.v_cache || !a.block_table || !a.schedule || !a.out || !a.workspace)
         return -100;
-    if (!(a.scale > 0.0f) || !(a.scale <= 3.0e38f)) return -100;
+    const float scale_log2e = a.scale * 1.4426950408889634f;
+    if (!(a.scale > 0.0f) || !(scale_log2e <= 3.0e38f)) return -100;
     const int shift = a.page_size == 16 ? 4 : a.page_size == 32 ? 5 : a.page_size == 64 ? 6 : a.page_size == 128 ? 7 : -1;
     if (shift < 0 || (a.d != 128 && a.d != 256) || !heads_ok(a.H_q, a.H_kv) || a.table_stride < a.max_pages) return -103;
     const void* ptrs[] = {a.q, a.gate, a.k_cache, a.v_cache, a.out, a.schedule};
@@ -392,7 +393,7 @@ int launch_attn(const khq_paged_attn_args* args, bool bf16, cudaStream_t stream)
     p.H_kv = a.H_kv;
     p.n_rep = a.H_q / a.H_kv;
     p.rep_mul = 65536 / p.n_rep + 1;
-    p.scale_log2e = a.scale * 1.4426950408889634f;
+    p.scale_log2e = scale_log2e;
     if (a.d == 256) return bf16 ? launch_kernels<256, true>(a, p, sched, w, stream) : launch_kernels<256, false>(a, p, sched, w, stream);
     return bf16 ? launch_kernels<128, true>(a, p, sched, w, stream) : launch_kernels<128, false>(a, p, sched, w, stream);
 }

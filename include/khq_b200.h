@@ -413,7 +413,7 @@ int launch_khq_paged_prestep_bf16(const khq_paged_prestep_args* args, khq_stream
  * tokens are part of the products: a V that is not finite reaches rows of the same request in front of it, with weight 0.)  schedule is
  * a plan's, max_tokens, max_new, requests, page_size, d and the head counts the same as there; `tokens` rows of q, gate,
  * out and lse exist, rows that the plan has beyond them are skipped.  Page numbers outside 0..n_pages-1 are not attended.  Rows behind the plan's last are left alone.
- * scale > 0.  workspace: khq_b200_paged_workspace_bytes(...) at 256 bytes; calls that may run at the same time need their own.  Returns -100, -103,
+ * 0 < scale <= 2e38.  workspace: khq_b200_paged_workspace_bytes(...) at 256 bytes; calls that may run at the same time need their own.  Returns -100, -103,
  * -104, -105, -107 / -108 (no tensor map). */
 typedef struct khq_paged_attn_args {
     const void *q, *gate, *k_cache, *v_cache, *block_table, *schedule;

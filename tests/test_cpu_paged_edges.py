@@ -109,3 +109,15 @@ def test_refusals_say_what_does_not_fit():
         paged.paged_prestep(plan, 7, None, None, None, None, None, None, None)
     with pytest.raises(TypeError, match="q"):
         paged.paged_attention(plan, None, None, None, None, None, 0.1)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_a_scale_that_overflows_is_refused(dtype):
+    """2.5e38 is finite, its product with log2 e is not."""
+    from test_cpu_paged import ATTN, ATTN_ARGS, call
+
+    from bonsai_mojo_1bit_optimization_t4_cuda_b200 import build, lib
+
+    build.build()
+    assert call(getattr(lib.load(), "launch_khq_paged_attn_" + dtype), ATTN_ARGS, ATTN, scale=2.5e38, schedule_bytes=100) == -100
+    assert call(getattr(lib.load(), "launch_khq_paged_attn_" + dtype), ATTN_ARGS, ATTN, scale=2e38, schedule_bytes=100) == -105  # the next look
