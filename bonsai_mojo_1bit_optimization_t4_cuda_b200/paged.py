@@ -14,7 +14,8 @@ allocates, so a step can be captured into a CUDA graph at its largest size and r
 ``plan.check()`` raises if a wait inside the attention's kernels has run out (they never hang).
 
 When a prompt is complete, ``KhqRuntime.khq_adopt_pages`` or ``BatchEngine.load_pages`` compresses its pages (fp16, K un-rotated from ``u_cache``)
-and the sequence goes on in code words.
+and the sequence goes on in code words; its later tokens go through the framework's other pre-step, whose angles are fp32 (``include/khq_b200.h`` has the
+difference).  bf16 pages have no such way out: they, and single tokens over raw pages, are for callers who do not compress.
 """
 from __future__ import annotations
 

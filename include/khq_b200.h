@@ -389,7 +389,9 @@ size_t khq_b200_paged_schedule_bytes(int requests, int max_tokens, int max_new, 
 int launch_khq_paged_plan(const khq_paged_plan_args* args, khq_stream_t stream);
 
 /* The pre-step of `tokens` rows: head RMS norms of q and k (fp32 weights of d, or NULL), rotation of the pairs (i, i + rotary_dim / 2) of the first
- * rotary_dim dims (a multiple of 16, 0: none) at the rows' positions, q to q_out (which may be q), K rotated, V and, unless
+ * rotary_dim dims (a multiple of 16, 0: none) at the rows' positions (angles in fp64, so a far position costs no accuracy;
+ * launch_khq_prestep_fp16 and its batched form keep the reference's fp32 angle and fp16 rounding between norm and rotation, so a K row that they make for
+ * the same token differs by some 2e-3 of values around 3 up to position 32768, by 7e-3 at 131072, 1.3e-2 at 262143), q to q_out (which may be q), K rotated, V and, unless
  * u_cache is NULL, K not rotated into the slots of the caches.  fp32 inside, each stored value rounded once.  Rows with position < 0 are
  * left alone, rows whose slot is not in the cache get their q only.  q (tokens, H_q, d), k and v (tokens, H_kv, d), caches (n_pages, page_size,
  * H_kv, d): strides in elements (multiples of 8), the last dim contiguous; pointers at 16 bytes.  Returns -100, -103, -104. */
