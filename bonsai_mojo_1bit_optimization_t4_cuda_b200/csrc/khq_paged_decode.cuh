@@ -12,6 +12,10 @@
 // One warp a scheduler, so a unit's chain of latencies counts (2100 cycles for 16 keys at d 128): 16 KB a unit and one wait for both halves
 // of it keep the chain below the time that memory takes.  64 sequences of 4200 tokens, d 256: 185 us; with eight warps and half the
 // ring for each 235; with K and V waited for one after the other, and one chain of products instead of two, 251.
+//
+// The weights enter the product with V as 16-bit values, the instruction's type and what the chunk kernel does: half a step of it (2^-11, bf16 2^-8) of sum w |v|,
+// about what the output's own rounding takes.  Their sum is of the fp32 values.  A second product with what the rounding left out would add to the chain of
+// a unit, which is just below memory's time.
 #pragma once
 
 namespace khq_paged {

@@ -5,7 +5,8 @@
 // a CTA.  So a chunk of 21 tokens with six heads per kv head fills a CTA's rows instead of 1/6 of six tiles, and a tile's rows attend almost the same keys.
 // Per block of 128 keys the pair computes S = Q K^T (M 256) and O += P V, each CTA keeping half of the K block (64 keys) and half of
 // the V block (d / 2 head dims).  As in khq_prefill_pair.cuh, whose comments give the reasons: two groups of four softmax warps take the blocks in turn, a
-// thread per row; P goes back over S in tensor memory in two halves; O is rescaled only when a maximum has grown by 2^8.
+// thread per row; P goes back over S in tensor memory in two halves; O is rescaled only when a maximum has grown by 2^8.  P is of
+// 16 bits, V's type in the instruction, as everywhere in the prompt kernels (half a step of it of sum w |v|); the weights' sum is of the fp32 values.
 //
 // Work: the key blocks of all (kv head, item) pairs stand in one row and each CTA pair takes an equal stretch of it, so any mix of chunks and
 // single tokens is even.  A segment that begins or ends inside a pair's stretch leaves records, which khq_paged_merge_kernel
