@@ -61,8 +61,7 @@ def test_the_library_is_built_without_torch(monkeypatch, tmp_path, capsys):
 
     monkeypatch.setattr(build, "LIB_PATH", tmp_path / build.LIB_NAME)
     monkeypatch.setattr(build, "SOURCES", ["khq_calib.cu"])
-    monkeypatch.setattr(build, "host_path", lambda: tmp_path / "host.so", raising=False)
-    monkeypatch.setattr(build, "HOST_PATH", tmp_path / "host.so", raising=False)
+    monkeypatch.setattr(build, "host_path", lambda: tmp_path / "host.so")
     monkeypatch.setitem(sys.modules, "torch", None)  # an import of it raises
     assert build.build() == build.LIB_PATH
     assert (tmp_path / build.LIB_NAME).exists() and not (tmp_path / "host.so").exists()
